@@ -82,6 +82,12 @@ SIGNATURES: dict[str, tuple] = {
     "hexcuda_attn_lut_i8_window": (I, [I, P, P, P, P, P, I, I, I, I, I32, I, I32, I]),
     "hexcuda_kv_cache_update_i8": (I, [I, P, P, P, P, I, I, I, I]),
     "hexcuda_rope_pair_f16": (I, [I, P, P, P, P, I64]),
+    "hexcuda_qk_norm_rope": (I, [I, I, P, I64, P, I64, P, I64, P, P, P, P, P, P, P, P, P, P, I, I, I, I,
+                                 I, I, I, I, I, I, F]),
+    "hexcuda_paged_attn": (I, [I, I, P, P, P, P, P, P, P, P, P, SZ, I, I, I, I, I, I, I, I, I, F, I]),
+    "hexcuda_paged_attn_workspace": (I, [I, P]),
+    "hexcuda_cache_scores": (I, [I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I]),
+    "hexcuda_cache_evict": (I, [I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I]),
     "hexcuda_gemm_i16": (I, [I, P, P, P, I, I, I]),
     "hexcuda_conv2d_hmx": (I, [I, P, P, P, P, I, I, I, I, I, I, I, I, I]),
     "hexcuda_mix_mlp_i8": (I, [I, P, P, P, P, P, P, P, I, I, I, I, I32, I, I32, I]),
@@ -143,6 +149,11 @@ SIGNATURES: dict[str, tuple] = {
     "hexcuda_host_attn_lut_i8_window": (I, [P, P, P, P, P, I, I, I, I, I32, I, I32, I]),
     "hexcuda_host_kv_cache_update_i8": (I, [P, P, P, P, I, I, I, I]),
     "hexcuda_host_rope_pair_f16": (I, [P, P, P, P, I64]),
+    "hexcuda_host_qk_norm_rope": (I, [I, P, I64, P, I64, P, I64, P, P, P, P, P, P, P, P, P, P, I, I, I,
+                                      I, I, I, I, I, I, I, F]),
+    "hexcuda_host_paged_attn": (I, [I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I]),
+    "hexcuda_host_cache_scores": (I, [I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I]),
+    "hexcuda_host_cache_evict": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I]),
     "hexcuda_host_gemm_i16": (I, [P, P, P, I, I, I]),
     "hexcuda_host_conv2d_hmx": (I, [P, P, P, P, I, I, I, I, I, I, I, I, I]),
     "hexcuda_host_mix_mlp_i8": (I, [P, P, P, P, P, P, P, I, I, I, I, I32, I, I32, I]),

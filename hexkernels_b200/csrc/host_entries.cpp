@@ -1347,6 +1347,208 @@ HX_EXPORT int hexcuda_host_rope_pair_f16(const uint16_t *x, const uint16_t *cos_
     });
 }
 
+// ---- paged cache: one device, every operand staged in one scratch buffer ----
+
+namespace {
+
+// A host buffer that a call reads, writes (read first: what the call leaves
+// alone comes back unchanged) or both; `dev` is its place on the device.
+struct HostBuf {
+    void *host;
+    size_t bytes;
+    bool out;
+    uint8_t *dev = nullptr;
+    template <typename T>
+    T *at() const {
+        return reinterpret_cast<T *>(dev);
+    }
+};
+
+// Stages the buffers on device slot 0 (a null host pointer stays null), runs
+// launch(), and copies the written ones back once it finished without error.
+int run_on_first(std::vector<HostBuf> &bufs, const std::function<int()> &launch) {
+    Dev *d = get_dev(0);
+    if (!d) return HEXCUDA_ERR_NODEV;
+    size_t total = 0;
+    for (const HostBuf &b : bufs) total += b.host ? (b.bytes + 255) / 256 * 256 : 0;
+    uint8_t *p = reinterpret_cast<uint8_t *>(scratch(d, kSlotOut, total));
+    if (!p) return hexcuda_last_error();
+    for (HostBuf &b : bufs) {
+        if (!b.host) continue;
+        b.dev = p;
+        p += (b.bytes + 255) / 256 * 256;
+        if (b.bytes)
+            if (int rc = check(cudaMemcpyAsync(b.dev, b.host, b.bytes, cudaMemcpyHostToDevice,
+                                               d->stream),
+                               "h2d"))
+                return rc;
+    }
+    if (int rc = launch()) {
+        cudaStreamSynchronize(d->stream);
+        return rc;
+    }
+    if (int rc = hexcuda_sync(0)) return rc;
+    for (const HostBuf &b : bufs)
+        if (b.out && b.host && b.bytes)
+            if (int rc = check(cudaMemcpyAsync(b.host, b.dev, b.bytes, cudaMemcpyDeviceToHost,
+                                               d->stream),
+                               "d2h"))
+                return rc;
+    return hexcuda_sync(0);
+}
+
+HostBuf host_in(const void *p, int64_t count, size_t size) {
+    return HostBuf{const_cast<void *>(p), count > 0 ? (size_t)count * size : 0, false};
+}
+HostBuf host_out(void *p, int64_t count, size_t size) {
+    return HostBuf{p, count > 0 ? (size_t)count * size : 0, true};
+}
+// sizes of a cache's buffers in elements; 0 when a factor is not positive
+int64_t volume(std::initializer_list<int64_t> factors) {
+    int64_t n = 1;
+    for (int64_t f : factors) n = f > 0 ? n * f : 0;
+    return n;
+}
+
+}  // namespace
+
+HX_EXPORT int hexcuda_host_qk_norm_rope(int dtype, const void *q, int64_t q_stride, const void *k,
+                                        int64_t k_stride, const void *v, int64_t v_stride,
+                                        const void *q_gain, const void *k_gain, const float *cos_t,
+                                        const float *sin_t, const int32_t *positions,
+                                        const int32_t *slots, void *q_out, void *k_pages,
+                                        void *v_pages, float *scores, int tokens, int heads,
+                                        int kv_heads, int head_dim, int rot_dim, int halves,
+                                        int norm, int table_len, int num_pages, int page_size,
+                                        float eps) {
+    // the launcher's own checks, on a call that has nothing to launch
+    auto call = [&](const std::vector<HostBuf> *b, int n) {
+        auto at = [&](int i, const void *host) { return b ? (*b)[(size_t)i].at<void>() : const_cast<void *>(host); };
+        return hexcuda_qk_norm_rope(
+            0, dtype, at(0, q), q_stride, at(1, k), k_stride, at(2, v), v_stride, at(3, q_gain),
+            at(4, k_gain), (const float *)at(5, cos_t), (const float *)at(6, sin_t),
+            (const int32_t *)at(7, positions), (const int32_t *)at(8, slots), at(9, q_out),
+            at(10, k_pages), at(11, v_pages), (float *)at(12, scores), n, heads, kv_heads, head_dim,
+            rot_dim, halves, norm, table_len, num_pages, page_size, eps);
+    };
+    if (tokens <= 0 || heads < 0 || kv_heads < 0 || head_dim < 1 || rot_dim < 0)
+        return call(nullptr, std::min(tokens, 0));
+    if (int rc = call(nullptr, 0)) return rc;
+    auto rows = [&](int64_t stride, int64_t n) { return n > 0 ? (tokens - 1) * stride + n * head_dim : 0; };
+    const int64_t pages = volume({num_pages, kv_heads, page_size});
+    const int64_t turns = volume({table_len, rot_dim / 2});
+    std::vector<HostBuf> b{host_in(heads ? q : nullptr, rows(q_stride, heads), 2),
+                           host_in(kv_heads ? k : nullptr, rows(k_stride, kv_heads), 2),
+                           host_in(kv_heads ? v : nullptr, rows(v_stride, kv_heads), 2),
+                           host_in(q_gain, head_dim, 2),
+                           host_in(k_gain, head_dim, 2),
+                           host_in(cos_t, turns, 4),
+                           host_in(sin_t, turns, 4),
+                           host_in(positions, tokens, 4),
+                           host_in(slots, tokens, 4),
+                           host_out(q_out, volume({tokens, heads, head_dim}), 2),
+                           host_out(k_pages, pages * head_dim, 2),
+                           host_out(v_pages, pages * head_dim, 2),
+                           host_out(scores, pages, 4)};
+    return run_on_first(b, [&] { return call(&b, tokens); });
+}
+
+HX_EXPORT int hexcuda_host_paged_attn(int dtype, const void *q, const void *k_pages,
+                                      const void *v_pages, const int32_t *block_table,
+                                      const int32_t *kv_lens, const int32_t *q_offs, void *out,
+                                      float *lse, int batch, int total_q, int max_q, int heads,
+                                      int kv_heads, int head_dim, int num_pages, int page_size,
+                                      int max_pages, float scale, int causal) {
+    if (int rc = check_paged("host_paged_attn", dtype, block_table, kv_lens, q_offs, batch, total_q,
+                             max_q, heads, kv_heads, head_dim, num_pages, page_size, max_pages,
+                             scale))
+        return rc;
+    if (batch == 0 || total_q == 0) return HEXCUDA_OK;
+    if (int rc = null_check("host_paged_attn", {q, k_pages, v_pages, out})) return rc;
+    size_t space = 0;
+    if (int rc = hexcuda_paged_attn_workspace(0, &space)) return rc;
+    const int64_t qn = volume({total_q, heads, head_dim});
+    const int64_t pages = volume({num_pages, kv_heads, page_size, head_dim});
+    std::vector<HostBuf> b{host_in(q, qn, 2),
+                           host_in(k_pages, pages, 2),
+                           host_in(v_pages, pages, 2),
+                           host_in(block_table, volume({batch, max_pages}), 4),
+                           host_in(kv_lens, batch, 4),
+                           host_in(q_offs, (int64_t)batch + 1, 4),
+                           host_out(out, qn, 2),
+                           host_out(lse, volume({total_q, heads}), 4)};
+    return run_on_first(b, [&] {
+        Dev *d = get_dev(0);
+        void *work = scratch(d, kSlotIn0, space);
+        if (!work) return hexcuda_last_error();
+        return hexcuda_paged_attn(0, dtype, b[0].dev, b[1].dev, b[2].dev, b[3].at<int32_t>(),
+                                  b[4].at<int32_t>(), b[5].at<int32_t>(), b[6].dev,
+                                  b[7].at<float>(), work, space, batch, total_q, max_q, heads,
+                                  kv_heads, head_dim, num_pages, page_size, max_pages, scale,
+                                  causal);
+    });
+}
+
+HX_EXPORT int hexcuda_host_cache_scores(int dtype, const void *q, const float *lse,
+                                        const void *k_pages, const int32_t *block_table,
+                                        const int32_t *kv_lens, const int32_t *q_offs,
+                                        float *scores, int batch, int total_q, int max_q, int heads,
+                                        int kv_heads, int head_dim, int num_pages, int page_size,
+                                        int max_pages, float scale, int causal) {
+    if (int rc = check_paged("host_cache_scores", dtype, block_table, kv_lens, q_offs, batch,
+                             total_q, max_q, heads, kv_heads, head_dim, num_pages, page_size,
+                             max_pages, scale))
+        return rc;
+    if (batch == 0 || total_q == 0) return HEXCUDA_OK;
+    if (int rc = null_check("host_cache_scores", {q, lse, k_pages, scores})) return rc;
+    const int64_t slots = volume({num_pages, kv_heads, page_size});
+    std::vector<HostBuf> b{host_in(q, volume({total_q, heads, head_dim}), 2),
+                           host_in(lse, volume({total_q, heads}), 4),
+                           host_in(k_pages, slots * head_dim, 2),
+                           host_in(block_table, volume({batch, max_pages}), 4),
+                           host_in(kv_lens, batch, 4),
+                           host_in(q_offs, (int64_t)batch + 1, 4),
+                           host_out(scores, slots, 4)};
+    return run_on_first(b, [&] {
+        return hexcuda_cache_scores(0, dtype, b[0].dev, b[1].at<float>(), b[2].dev,
+                                    b[3].at<int32_t>(), b[4].at<int32_t>(), b[5].at<int32_t>(),
+                                    b[6].at<float>(), batch, total_q, max_q, heads, kv_heads,
+                                    head_dim, num_pages, page_size, max_pages, scale, causal);
+    });
+}
+
+HX_EXPORT int hexcuda_host_cache_evict(void *k_pages, void *v_pages, float *scores,
+                                       const int32_t *block_table, const int32_t *dst_table,
+                                       const int32_t *kv_lens, int32_t *new_lens, int32_t *kept,
+                                       int batch, int kv_heads, int head_dim, int num_pages,
+                                       int page_size, int max_pages, int dst_max_pages, int budget,
+                                       int sink, int recent) {
+    auto call = [&](const std::vector<HostBuf> *b, int n) {
+        auto at = [&](int i, const void *host) { return b ? (*b)[(size_t)i].at<void>() : const_cast<void *>(host); };
+        return hexcuda_cache_evict(0, at(0, k_pages), at(1, v_pages), (float *)at(2, scores),
+                                   (const int32_t *)at(3, block_table),
+                                   (const int32_t *)at(4, dst_table),
+                                   (const int32_t *)at(5, kv_lens), (int32_t *)at(6, new_lens),
+                                   (int32_t *)at(7, kept), n, kv_heads, head_dim, num_pages,
+                                   page_size, max_pages, dst_max_pages, budget, sink, recent);
+    };
+    if (int rc = call(nullptr, std::min(batch, 0))) return rc;
+    if (batch == 0) return HEXCUDA_OK;
+    if (int rc = null_check("host_cache_evict",
+                            {k_pages, v_pages, scores, block_table, kv_lens, new_lens, kept}))
+        return rc;
+    const int64_t slots = volume({num_pages, kv_heads, page_size});
+    std::vector<HostBuf> b{host_out(k_pages, slots * head_dim, 2),
+                           host_out(v_pages, slots * head_dim, 2),
+                           host_out(scores, slots, 4),
+                           host_in(block_table, volume({batch, max_pages}), 4),
+                           host_in(dst_table, volume({batch, dst_max_pages}), 4),
+                           host_in(kv_lens, batch, 4),
+                           host_out(new_lens, batch, 4),
+                           host_out(kept, volume({batch, kv_heads, budget}), 4)};
+    return run_on_first(b, [&] { return call(&b, batch); });
+}
+
 HX_EXPORT int hexcuda_host_ffn_hmx_i8(const uint8_t *X, const int8_t *W1, const int32_t *b1,
                                       const int8_t *W2, const int32_t *b2, int8_t *out, int M,
                                       int D, int Dff, int sh1, int sh2) {

@@ -77,6 +77,11 @@ int replicate_rows(const std::vector<void *> &douts, int64_t rows, size_t row_by
 void replica_clear();
 void collective_release();
 
+// The argument checks that the entries over a paged cache share (paged_attn.cu).
+int check_paged(const char *name, int dtype, const void *table, const void *kv_lens,
+                const void *q_offs, int batch, int total_q, int max_q, int heads, int kv_heads,
+                int head_dim, int num_pages, int page_size, int max_pages, float scale);
+
 // Watchdog budget for device-side bounded waits, in nanoseconds of
 // %globaltimer.  A wait that exceeds it sets the device error word.
 constexpr unsigned long long kWaitBudgetNs = 4000000000ull;
@@ -88,6 +93,7 @@ enum : int {
     kErrWaitAccum = 4,     // accumulator hand-off wait expired
     kErrWaitOther = 8,
     kErrWaitPart = 16,     // GEMM tail split: wait for another CTA's partial expired
+    kErrIndex = 32,        // paged cache: an index in device memory was out of range
 };
 
 }  // namespace hx

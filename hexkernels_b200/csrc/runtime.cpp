@@ -288,6 +288,11 @@ static int sync_one(Dev *d) {
         return rc;
     if (word) {
         cudaMemset(d->err_word, 0, sizeof(int));
+        if (word == kErrIndex)
+            return fail(HEXCUDA_ERR_ARG,
+                        "device %d: a page, slot, position, length or row offset in device memory "
+                        "was out of range; what it named was skipped",
+                        d->ordinal);
         return fail(HEXCUDA_ERR_TIMEOUT,
                     "device %d: a bounded device-side wait expired (flags 0x%x); outputs of "
                     "the last launch are invalid",

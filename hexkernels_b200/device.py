@@ -5,6 +5,8 @@ launches go to torch's current stream so torch.cuda.Event timing brackets them.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 from ._lib import check, load
 
 
@@ -26,6 +28,13 @@ def bind_stream(dev: int, stream=None) -> None:
 
     s = stream if stream is not None else torch.cuda.current_stream()
     check(load().hexcuda_set_stream(dev, s.cuda_stream))
+
+
+def paged_attn_workspace(dev: int) -> int:
+    """Bytes of device memory that a ``paged_attn`` call takes as workspace."""
+    n = C.c_size_t()
+    check(load().hexcuda_paged_attn_workspace(dev, C.byref(n)))
+    return n.value
 
 
 def sync(dev: int = -1) -> None:

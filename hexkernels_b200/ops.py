@@ -805,3 +805,134 @@ def rowreduce(x, op: int) -> np.ndarray:
     out = np.empty(R, np.float32)
     check(load().hexcuda_host_rowreduce_f32(_p(x), _p(out), R, Cc, op))
     return out
+
+
+# ------------------------------------------------------- paged key / value cache
+
+FLOAT16, BFLOAT16 = 0, 1
+
+
+def _kind(*arrays) -> int:
+    """Element type code of 16-bit heads: float16 arrays, or uint16 arrays of
+    bfloat16 bit patterns (NumPy has no bfloat16)."""
+    dtypes = {a.dtype for a in arrays if a is not None}
+    if dtypes == {np.dtype(np.float16)}:
+        return FLOAT16
+    if dtypes == {np.dtype(np.uint16)}:
+        return BFLOAT16
+    raise TypeError(f"expected all float16 or all uint16 (bfloat16 bits), got {dtypes}")
+
+
+def _heads(x):
+    """[tokens, heads, dim] with each token's heads contiguous, and the token
+    stride in elements; copied only when the heads are not contiguous."""
+    T, H, D = x.shape
+    size = x.itemsize
+    if x.strides[2] != size or (H > 1 and x.strides[1] != D * size) or (
+            T > 1 and (x.strides[0] % size or x.strides[0] < H * D * size)):
+        x = np.ascontiguousarray(x)
+    return x, (x.strides[0] // size if T > 1 else H * D)
+
+
+def _inplace(a, shape, what):
+    if not (a.flags.c_contiguous and a.flags.writeable) or a.shape != shape:
+        raise ValueError(f"{what}: expected a writeable C-contiguous array of shape {shape}")
+    return a
+
+
+def qk_norm_rope(q, k, v, k_pages, v_pages, cos, sin, positions, slots, q_gain=None, k_gain=None,
+                 scores=None, halves: bool = True, norm: bool = True,
+                 eps: float = 1e-6) -> np.ndarray:
+    """RMS norm and rotation of new tokens' query and key heads (q [T, H, D],
+    k and v [T, KV, D]); returns the queries and writes keys and values to
+    their slots of k_pages / v_pages [pages, KV, page_size, D] in place, where
+    scores [pages, KV, page_size] becomes 0.  cos / sin [positions, rot / 2]."""
+    kind = _kind(q, k, v, k_pages, v_pages, q_gain, k_gain)
+    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+    T, H, D = q.shape
+    KV = k.shape[1]
+    assert k.shape == v.shape == (T, KV, D)
+    pages, page = k_pages.shape[0], k_pages.shape[2]
+    _inplace(k_pages, (pages, KV, page, D), "k_pages")
+    _inplace(v_pages, (pages, KV, page, D), "v_pages")
+    cos, sin = _c(cos, np.float32), _c(sin, np.float32)
+    assert cos.shape == sin.shape
+    positions, slots = _c(positions, np.int32), _c(slots, np.int32)
+    assert positions.shape == slots.shape == (T,)
+    gains = [None if g is None else np.ascontiguousarray(g) for g in (q_gain, k_gain)]
+    assert all(g is None or g.shape == (D,) for g in gains)
+    if scores is not None:
+        _inplace(_c(scores, np.float32), (pages, KV, page), "scores")
+    out = np.zeros((T, H, D), q.dtype)
+    pp = lambda a: None if a is None else _p(a)
+    check(load().hexcuda_host_qk_norm_rope(
+        kind, _p(q), qs, _p(k), ks, _p(v), vs, pp(gains[0]), pp(gains[1]), _p(cos), _p(sin),
+        _p(positions), _p(slots), _p(out), _p(k_pages), _p(v_pages), pp(scores), T, H, KV, D,
+        2 * cos.shape[1], int(halves), int(norm), cos.shape[0], pages, page, eps))
+    return out
+
+
+def _paged(q, k_pages, block_table, kv_lens, q_offs, max_q):
+    block_table, kv_lens = _c(block_table, np.int32), _c(kv_lens, np.int32)
+    q_offs = _c(q_offs, np.int32)
+    B, wide = block_table.shape
+    T, H, D = q.shape
+    pages, KV, page, D2 = k_pages.shape
+    assert D == D2 and kv_lens.shape == (B,) and q_offs.shape == (B + 1,)
+    if max_q is None:
+        max_q = int(np.diff(q_offs).max(initial=0))
+    return block_table, kv_lens, q_offs, (B, T, max(0, max_q), H, KV, D, pages, page, wide)
+
+
+def paged_attn(q, k_pages, v_pages, block_table, kv_lens, q_offs, scale: float | None = None,
+               causal: bool = True, max_q: int | None = None):
+    """Attention of new tokens q [T, H, D] over a paged cache; returns (out
+    [T, H, D], lse [T, H]).  Rows that no sequence names come back as zeros."""
+    kind = _kind(q, k_pages, v_pages)
+    q, k_pages, v_pages = (np.ascontiguousarray(a) for a in (q, k_pages, v_pages))
+    assert k_pages.shape == v_pages.shape
+    table, lens, offs, dims = _paged(q, k_pages, block_table, kv_lens, q_offs, max_q)
+    out, lse = np.zeros_like(q), np.zeros(q.shape[:2], np.float32)
+    check(load().hexcuda_host_paged_attn(
+        kind, _p(q), _p(k_pages), _p(v_pages), _p(table), _p(lens), _p(offs), _p(out), _p(lse),
+        *dims, q.shape[2] ** -0.5 if scale is None else scale, int(causal)))
+    return out, lse
+
+
+def cache_scores(q, lse, k_pages, block_table, kv_lens, q_offs, scores,
+                 scale: float | None = None, causal: bool = True, max_q: int | None = None):
+    """Adds to scores [pages, KV, page_size], in place, the attention weight
+    that the new tokens q gave to each cached one (lse from paged_attn)."""
+    kind = _kind(q, k_pages)
+    q, k_pages, lse = np.ascontiguousarray(q), np.ascontiguousarray(k_pages), _c(lse, np.float32)
+    table, lens, offs, dims = _paged(q, k_pages, block_table, kv_lens, q_offs, max_q)
+    assert lse.shape == q.shape[:2]
+    _inplace(_c(scores, np.float32), k_pages.shape[:3], "scores")
+    check(load().hexcuda_host_cache_scores(
+        kind, _p(q), _p(lse), _p(k_pages), _p(table), _p(lens), _p(offs), _p(scores), *dims,
+        q.shape[2] ** -0.5 if scale is None else scale, int(causal)))
+    return scores
+
+
+def cache_evict(k_pages, v_pages, scores, block_table, kv_lens, budget: int, sink: int = 0,
+                recent: int = 0, dst_table=None):
+    """Cuts every sequence and key head to at most `budget` cached tokens (the
+    first `sink`, the last `recent`, the highest scores between), moving their
+    rows of k_pages, v_pages and scores in place or to the pages of dst_table;
+    returns (kept [B, KV, budget] with -1 behind the last, new lengths [B])."""
+    _kind(k_pages, v_pages)
+    pages, KV, page, D = k_pages.shape
+    for a, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        _inplace(a, (pages, KV, page, D), what)
+    _inplace(_c(scores, np.float32), (pages, KV, page), "scores")
+    table, lens = _c(block_table, np.int32), _c(kv_lens, np.int32)
+    B, wide = table.shape
+    assert lens.shape == (B,)
+    dst = None if dst_table is None else _c(dst_table, np.int32)
+    assert dst is None or dst.shape[0] == B
+    kept, new = np.full((B, KV, max(0, budget)), -1, np.int32), np.zeros(B, np.int32)
+    check(load().hexcuda_host_cache_evict(
+        _p(k_pages), _p(v_pages), _p(scores), _p(table), None if dst is None else _p(dst),
+        _p(lens), _p(new), _p(kept), B, KV, D, pages, page, wide, 0 if dst is None else dst.shape[1],
+        budget, sink, recent))
+    return kept, new

@@ -500,6 +500,89 @@ int hexcuda_kv_cache_update_i8(int dev, int8_t *k_cache, int8_t *v_cache, const 
  * aligned. */
 int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, const uint16_t *sin_t,
                           uint16_t *out, int64_t n_pairs);
+/* ---- Paged key / value cache of 16-bit floating-point heads ----
+ * dtype: HEXCUDA_F16 (binary16) or HEXCUDA_BF16 (bfloat16) of q, K, V, gains
+ * and out.  k_pages and v_pages are [num_pages][kv_heads][page_size][head_dim];
+ * token j of sequence b lies in page block_table[b * max_pages + j / page_size]
+ * at offset j % page_size.  kv_lens[b] counts the cached tokens, the new ones
+ * of the call included (they are the last); the new tokens of sequence b are
+ * rows q_offs[b] .. q_offs[b + 1] - 1 of q [total_q][heads][head_dim] (q_offs
+ * has batch + 1 ascending entries; rows that no sequence names are left as
+ * they are).  Query head h uses key head h / (heads / kv_heads).  With
+ * causal != 0 new token t of q_len sees cached tokens up to its own place
+ * kv_len - q_len + t; without it every cached token (cross attention over an
+ * encoder's states).  Nothing past kv_lens[b] is used, whatever it holds
+ * (not-a-number included).  A new token's own K and V must be finite when
+ * other tokens of its chunk are to be.
+ * Tables, lengths, offsets, slots and positions are device data: an entry out
+ * of range is skipped, never followed, and the next hexcuda_sync returns
+ * HEXCUDA_ERR_ARG.  Page, token and row counts are below 2^31; element offsets
+ * are 64-bit.  Nothing is allocated and nothing is read back, so calls can be
+ * captured into CUDA graphs (with hexcuda_set_timing(0)). */
+#define HEXCUDA_F16 0
+#define HEXCUDA_BF16 1
+/* RMS norm and rotation of new tokens' heads, and their way into the cache.
+ * Token t's heads start at q + t * q_stride, k + t * k_stride, v + t *
+ * v_stride (elements; e.g. columns of one projection's output).  Per query and
+ * key head: y = x * rsqrt(mean(x^2) + eps) * gain (gain [head_dim], null for
+ * 1; norm == 0: y = x), then the first rot_dim columns turn by cos_t / sin_t
+ * [table_len][rot_dim / 2] fp32 at row positions[t]: columns (i, i + rot_dim /
+ * 2) when halves != 0, (2 i, 2 i + 1) otherwise; fp32 throughout, one rounding.
+ * Queries go to q_out [tokens][heads][head_dim] (may be q itself when q_stride
+ * is heads * head_dim), keys and values (unchanged) to slot slots[t] = page *
+ * page_size + offset, and scores [num_pages][kv_heads][page_size] (may be
+ * null) is set to 0 there.  A negative slot marks padding: nothing of that
+ * token is read or written.  Slots of one call are distinct.  kv_heads 0: only
+ * queries, slots may be null (every token is taken); v and v_pages may both be
+ * null.  head_dim 1 to 256. */
+int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_stride, const void *k,
+                         int64_t k_stride, const void *v, int64_t v_stride, const void *q_gain,
+                         const void *k_gain, const float *cos_t, const float *sin_t,
+                         const int32_t *positions, const int32_t *slots, void *q_out,
+                         void *k_pages, void *v_pages, float *scores, int tokens, int heads,
+                         int kv_heads, int head_dim, int rot_dim, int halves, int norm,
+                         int table_len, int num_pages, int page_size, float eps);
+/* Attention of new tokens over the cache: out [total_q][heads][head_dim] =
+ * softmax(scale * q K^T) V over the tokens a row sees, lse [total_q][heads]
+ * (fp32, may be null) = log sum exp of its scaled scores.  A row that sees
+ * nothing gets zeros and minus infinity.  scale > 0.  max_q: the largest
+ * number of new tokens of a sequence as far as known (it chooses between
+ * kernels; a wrong one costs time only).  workspace: device memory of
+ * hexcuda_paged_attn_workspace bytes, 16-byte aligned, its contents free;
+ * calls that may run at the same time (two streams, two graphs) need one each. */
+int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *k_pages, const void *v_pages,
+                       const int32_t *block_table, const int32_t *kv_lens, const int32_t *q_offs,
+                       void *out, float *lse, void *workspace, size_t workspace_bytes, int batch,
+                       int total_q, int max_q, int heads, int kv_heads, int head_dim,
+                       int num_pages, int page_size, int max_pages, float scale, int causal);
+/* Bytes of workspace that serve every paged_attn call on this device. */
+int hexcuda_paged_attn_workspace(int dev, size_t *bytes);
+/* Attention weight collected by cached tokens: scores [num_pages][kv_heads]
+ * [page_size] (fp32) of each token that a row sees grows by the sum over those
+ * rows and the key head's query heads of exp(scale * q . K - lse), lse as
+ * paged_attn wrote it for the same q, cache and lengths (rows with minus
+ * infinity add nothing).  Sequences may share pages. */
+int hexcuda_cache_scores(int dev, int dtype, const void *q, const float *lse, const void *k_pages,
+                         const int32_t *block_table, const int32_t *kv_lens, const int32_t *q_offs,
+                         float *scores, int batch, int total_q, int max_q, int heads, int kv_heads,
+                         int head_dim, int num_pages, int page_size, int max_pages, float scale,
+                         int causal);
+/* Cut every sequence to min(kv_lens[b], budget) tokens, each key head on its
+ * own: the first `sink`, the last `recent` and, between them, the tokens of the
+ * highest scores (ties to the lowest index, not-a-number below everything).
+ * Those stay in their order: kept [batch][kv_heads][budget] lists the old
+ * places (-1 behind the last), their K, V and score rows move to tokens 0, 1,
+ * ... of the pages that dst_table [batch][dst_max_pages] names, new_lens[b]
+ * (may be kv_lens itself) is the new length.  dst_table null or naming the
+ * same pages in the same places: in place.  Otherwise its pages must not be
+ * among those that block_table names for cached tokens, nor one page be named
+ * for two sequences; in place, sequences share no pages.  K and V elements are
+ * 16-bit, of either type.  sink + recent <= budget. */
+int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *scores,
+                        const int32_t *block_table, const int32_t *dst_table,
+                        const int32_t *kv_lens, int32_t *new_lens, int32_t *kept, int batch,
+                        int kv_heads, int head_dim, int num_pages, int page_size, int max_pages,
+                        int dst_max_pages, int budget, int sink, int recent);
 /* int8 decoder block: causal LUT-softmax self-attention of X [S][D] (u8)
  * with scores clamp_i8(X.X^T >> 2), h = clamp_u8(X + clamp_i8(P.X >> 8)),
  * then out int8 = sat_i8(h + sat_i8((act_lut[clamp_i8((h.W1 >> 8) + b1) + 128]
@@ -784,6 +867,30 @@ int hexcuda_host_kv_cache_update_i8(int8_t *k_cache, int8_t *v_cache, const int8
                                     int head_dim);
 int hexcuda_host_rope_pair_f16(const uint16_t *x, const uint16_t *cos_t, const uint16_t *sin_t,
                                uint16_t *out, int64_t n_pairs);
+/* The paged-cache operators on host memory, on device slot 0 (the pages are
+ * copied in and, where written, out again: for tests and small models). */
+int hexcuda_host_qk_norm_rope(int dtype, const void *q, int64_t q_stride, const void *k,
+                              int64_t k_stride, const void *v, int64_t v_stride,
+                              const void *q_gain, const void *k_gain, const float *cos_t,
+                              const float *sin_t, const int32_t *positions, const int32_t *slots,
+                              void *q_out, void *k_pages, void *v_pages, float *scores, int tokens,
+                              int heads, int kv_heads, int head_dim, int rot_dim, int halves,
+                              int norm, int table_len, int num_pages, int page_size, float eps);
+int hexcuda_host_paged_attn(int dtype, const void *q, const void *k_pages, const void *v_pages,
+                            const int32_t *block_table, const int32_t *kv_lens,
+                            const int32_t *q_offs, void *out, float *lse, int batch, int total_q,
+                            int max_q, int heads, int kv_heads, int head_dim, int num_pages,
+                            int page_size, int max_pages, float scale, int causal);
+int hexcuda_host_cache_scores(int dtype, const void *q, const float *lse, const void *k_pages,
+                              const int32_t *block_table, const int32_t *kv_lens,
+                              const int32_t *q_offs, float *scores, int batch, int total_q,
+                              int max_q, int heads, int kv_heads, int head_dim, int num_pages,
+                              int page_size, int max_pages, float scale, int causal);
+int hexcuda_host_cache_evict(void *k_pages, void *v_pages, float *scores,
+                             const int32_t *block_table, const int32_t *dst_table,
+                             const int32_t *kv_lens, int32_t *new_lens, int32_t *kept, int batch,
+                             int kv_heads, int head_dim, int num_pages, int page_size,
+                             int max_pages, int dst_max_pages, int budget, int sink, int recent);
 int hexcuda_host_gemm_i16(const int16_t *A, const int16_t *B, int32_t *C, int M, int N, int K);
 int hexcuda_host_conv2d_hmx(const uint8_t *in, const int8_t *W, const int32_t *bias, void *out,
                             int store, int act, int c_in, int ih, int iw, int c_out, int kh, int kw,
