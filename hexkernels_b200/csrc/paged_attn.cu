@@ -1,5 +1,6 @@
-// paged_attn.cu -- attention of new tokens over a paged key / value cache,
-// the entry point and the CUDA-core path.
+// paged_attn.cu -- attention of new tokens over a paged key / value cache:
+// the entry point, the choice between its kernels, the join of partial
+// results, and the CUDA-core path.
 //
 //   out[r, h] = sum_j softmax_j(scale * q[r, h] . K[j]) V[j],
 //   lse[r, h] = log sum_j exp(scale * q[r, h] . K[j])
@@ -9,7 +10,7 @@
 // zeros and minus infinity.
 #include <math.h>
 
-#include "paged.cuh"
+#include "paged_tc.cuh"
 
 namespace hx {
 
@@ -117,7 +118,134 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
     }
 }
 
+// Joins the parts of the items that several CTAs worked on: block (c, y) those
+// of the item that starts in CTA c and ends in a later one, one warp per row.
+// The parts are taken in CTA order:
+//   M = max m_k,  out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a) {
+    tc::grid_dependency_wait();
+    const int c = blockIdx.x, lane = threadIdx.x & 31;
+    const PartRec r = a.recs[c];
+    const int i = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (r.nparts == 0 || i >= r.ntok * a.group) return;
+    const int t = i / a.group;
+    const int row = t / a.tok * 128 + (t % a.tok) * a.group + i % a.group;
+    auto slot = [&](int k) { return ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * kPartRows + row; };
+    float top = -INFINITY;
+    for (int k = lane; k < r.nparts; k += 32) {
+        const float2 ml = reinterpret_cast<const float2 *>(a.part_ml)[slot(k)];
+        if (ml.y != 0.0f) top = fmaxf(top, ml.x);
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int V = D / 32;
+    float acc[V], sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; v++) acc[v] = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < r.nparts; k++) {
+        const float2 ml = reinterpret_cast<const float2 *>(a.part_ml)[slot(k)];
+        // (a part without a visible key has no output)
+        const float w = ml.y == 0.0f ? 0.0f : tc::ex2(ml.x - top);
+        if (w == 0.0f) continue;
+        sum += w * ml.y;
+        const float *o = a.part_o + slot(k) * D + lane * V;
+        if constexpr (V == 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(o);
+            acc[0] += w * x.x;
+            acc[1] += w * x.y;
+            acc[2] += w * x.z;
+            acc[3] += w * x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2 *>(o);
+            acc[0] += w * x.x;
+            acc[1] += w * x.y;
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t at = (int64_t)(r.row0 + t) * a.heads + r.h * a.group + i % a.group;
+    T *out = reinterpret_cast<T *>(a.out) + at * D + lane * V;
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int v = 0; v < V; v += 2) w[v / 2] = pack2<T>(acc[v] * inv, acc[v + 1] * inv);
+    if constexpr (V == 4)
+        *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+    else
+        *reinterpret_cast<uint32_t *>(out) = w[0];
+    if (a.lse && lane == 0)
+        a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// The join starts while the kernel before it on the stream still runs, and
+// waits for it on the device (a programmatic dependent launch).
+template <typename T, int D>
+int launch_join(Dev *d, const PagedTc &a, int rows) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)d->sms, (unsigned)((rows + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = d->stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return check(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a), "launch paged_join");
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encode_map(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims,
+               const cuuint64_t *strides, const cuuint32_t *box) {
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
+                cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return fail(HEXCUDA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+        fn = reinterpret_cast<EncodeTiledFn>(p);
+    }
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank,
+                          const_cast<void *>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(HEXCUDA_ERR_CUDA, "cuTensorMapEncodeTiled (paged cache) failed (%d)", (int)r);
+    return HEXCUDA_OK;
+}
+
+size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
+
 }  // namespace
+
+int make_page_map(CUtensorMap *map, const void *base, int64_t rows, int dim, int frag) {
+    const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)frag};
+    return encode_map(map, base, 2, dims, strides, box);
+}
+
+int make_query_map(CUtensorMap *map, const void *base, int total_q, int heads, int dim, int group,
+                   int tok) {
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)total_q};
+    const cuuint64_t strides[2] = {(cuuint64_t)dim * 2, (cuuint64_t)heads * dim * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tok};
+    return encode_map(map, base, 3, dims, strides, box);
+}
+
+bool paged_tc_fits(const void *q, const void *k, const void *v, const void *out, int heads,
+                   int kv_heads, int dim, int num_pages, int page_size) {
+    const uintptr_t bits = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
+    return (dim == 64 || dim == 128) && page_size % 8 == 0 && (bits & 15u) == 0 &&
+           heads / kv_heads <= 128 &&
+           (int64_t)num_pages * kv_heads * page_size <= 0x7fffff00;
+}
+
 }  // namespace hx
 
 using namespace hx;
@@ -126,7 +254,9 @@ HX_EXPORT int hexcuda_paged_attn_workspace(int dev, size_t *bytes) {
     Dev *d = get_dev(dev);
     if (!d) return HEXCUDA_ERR_NODEV;
     if (!bytes) return fail(HEXCUDA_ERR_ARG, "paged_attn_workspace: null pointer");
-    *bytes = 256;
+    // one record and two partial results per CTA, one CTA per SM
+    *bytes = round_up(sizeof(PartRec) * d->sms, 256) +
+             (size_t)d->sms * 2 * kPartRows * (128 + 2) * sizeof(float);
     return HEXCUDA_OK;
 }
 
@@ -154,6 +284,46 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
                     workspace_bytes, need);
     PagedSeqs s{block_table, kv_lens, q_offs, batch, total_q, num_pages, page_size,
                 max_pages, causal, d->err_word};
+    const int group = heads / kv_heads;
+    // Up to 32 query rows share a key head: the decoding kernel.
+    const int64_t rows = (int64_t)(max_q < 1 ? 1 : max_q) * group;
+    if (rows <= 32 &&
+        paged_tc_fits(q, k_pages, v_pages, out, heads, kv_heads, head_dim, num_pages, page_size)) {
+        const int n = rows <= 16 ? 16 : 32;
+        PagedTc a;
+        a.s = s;
+        a.heads = heads;
+        a.kv_heads = kv_heads;
+        a.group = group;
+        a.tok = n / group;
+        const int low = page_size & -page_size;
+        a.frag = low < kKeys ? low : kKeys;
+        a.map_rows = num_pages * kv_heads * page_size;
+        a.min_tiles = 2;
+        a.scale_log2 = scale * 1.4426950408889634f;
+        a.out = out;
+        a.lse = lse;
+        uint8_t *p = reinterpret_cast<uint8_t *>(workspace);
+        a.recs = reinterpret_cast<PartRec *>(p);
+        p += round_up(sizeof(PartRec) * d->sms, 256);
+        a.part_ml = reinterpret_cast<float *>(p);
+        a.part_o = a.part_ml + (size_t)d->sms * 2 * kPartRows * 2;
+        CUtensorMap mq, mk, mv;
+        if (int rc = make_query_map(&mq, q, total_q, heads, head_dim, group, a.tok)) return rc;
+        if (int rc = make_page_map(&mk, k_pages, a.map_rows, head_dim, a.frag)) return rc;
+        if (int rc = make_page_map(&mv, v_pages, a.map_rows, head_dim, a.frag)) return rc;
+        launch_begin(d);
+        if (int rc = launch_paged_dec(d, mq, mk, mv, a, dtype, head_dim, n)) return rc;
+        const bool half = dtype == HEXCUDA_F16;
+        if (int rc = head_dim == 128
+                         ? (half ? launch_join<__half, 128>(d, a, n)
+                                 : launch_join<__nv_bfloat16, 128>(d, a, n))
+                         : (half ? launch_join<__half, 64>(d, a, n)
+                                 : launch_join<__nv_bfloat16, 64>(d, a, n)))
+            return rc;
+        note_mech(kMechTcgen05 | kMechTma);
+        return launch_end(d, "paged_attn", 2);
+    }
     launch_begin(d);
     const int ny = batch < 1024 ? batch : 1024;
     const dim3 grid((unsigned)((d->sms * 16 + ny - 1) / ny), (unsigned)ny);

@@ -1,0 +1,534 @@
+// paged_dec.cu -- attention of a few new tokens per sequence over the paged
+// cache (decoding: at most 32 query rows share a key head) on the tensor
+// cores, keys on the M side.
+//
+// A decode step reads every cached key and value once and does little with
+// them, so it is bound by HBM; the 128-row MMA tile is spent on keys, not on
+// the few queries:
+//     S^T [128 keys x N rows] = K Q^T      A = K as it lies in the pages
+//     O^T [D x N rows]       += V^T P^T    A = V as it lies (MN-major)
+// with N = 16 or 32 query rows (tokens x heads of one key head).  A softmax
+// thread owns one key: it reads its N scores from tensor memory, subtracts the
+// row's reference maximum, takes 2^x, adds to its own N partial sums and
+// writes P^T (N contiguous 16-bit values, the MN-major B operand) to shared
+// memory.  Maxima over keys are only needed when some score exceeds its row's
+// reference by 2^8 (or at an item's first tile); a vote per tile finds that
+// out, then the reference moves and O^T is rescaled.  Row sums are reduced
+// over the threads once per item.
+//
+// Per CTA (one per SM): warp 0 TMA, one lane per page fragment; warp 1 tensor
+// memory and MMA issue, S^T of the next tile before P V of this one; warps 4-7
+// softmax.  Key and value tiles of 128 tokens go through rings of 3 stages
+// (dim 128; 6 at dim 64), 192 KB of loads in flight per SM.
+//
+// Every wait is bounded; see mbar_wait.
+#include <math.h>
+
+#include "paged_tc.cuh"
+
+namespace hx {
+namespace {
+
+template <int D, int N>
+struct DecSmem {
+    static constexpr int kSubs = D / 64;
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kTile = kSubs * kSubTile;
+    static constexpr int kQTile = kSubs * N * 128;
+    static constexpr int kK = 0;
+    static constexpr int kV = kK + kStages * kTile;
+    static constexpr int kQ = kV + kStages * kTile;        // 2 buffers
+    static constexpr int kP = kQ + 2 * kQTile;             // 2 buffers of 128 x N
+    static constexpr int kRed = kP + 2 * kKeys * N * 2;    // [4][N] maxima or sums, [N] results
+    static constexpr int kPlan = kRed + 5 * N * 4;
+    static constexpr int kBar = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;
+    // q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2],
+    // o_free, drain, k_full, k_empty, v_full, v_empty [stages]
+    static constexpr int kNumBars = 14 + 4 * kStages;
+    static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
+};
+
+// Or of a condition over the softmax warps (named barrier 1).
+__device__ __forceinline__ bool vote_or(bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)p)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() {
+    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+}
+
+// N per-lane values reduced over the warp; lane l gets column l * N / 32.
+template <int N, bool MAX>
+__device__ __forceinline__ float reduce_columns(float (&v)[N], int lane) {
+#pragma unroll
+    for (int n = N / 2, o = 16; n > 0; n >>= 1, o >>= 1) {
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+            const float got = __shfl_xor_sync(0xffffffffu, send, o);
+            v[i] = MAX ? fmaxf(keep, got) : keep + got;
+        }
+    }
+    if constexpr (N == 16) {
+        const float got = __shfl_xor_sync(0xffffffffu, v[0], 1);
+        v[0] = MAX ? fmaxf(v[0], got) : v[0] + got;
+    }
+    return v[0];
+}
+
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[16]) {
+    tc::tmem_ld_32x32b_x16(taddr, r);
+    tc::tmem_ld_wait(r);
+}
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[32]) {
+    tc::tmem_ld_32x32b_x32(taddr, r);
+    tc::tmem_ld_wait(r);
+}
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[16]) {
+    tc::tmem_st_32x32b_x16(taddr, r);
+    tc::tmem_st_wait();
+}
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[32]) {
+    tc::tmem_st_32x32b_x32(taddr, r);
+    tc::tmem_st_wait();
+}
+
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(256, 1)
+    paged_dec_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const PagedTc a) {
+    using L = DecSmem<D, N>;
+    constexpr int kSubs = L::kSubs, S = L::kStages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_empty = bars + 6;
+    uint64_t *p_full = bars + 8, *pv_done = bars + 10, *o_free = bars + 12, *drain = bars + 13;
+    uint64_t *k_full = bars + 14, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err_word = a.s.err_word;
+    tc::launch_dependents();
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            tc::mbar_init(&q_full[i], 1);
+            tc::mbar_init(&q_empty[i], 1);
+            tc::mbar_init(&s_full[i], 1);
+            tc::mbar_init(&s_empty[i], 4);
+            tc::mbar_init(&p_full[i], 4);
+            tc::mbar_init(&pv_done[i], 1);
+        }
+        tc::mbar_init(o_free, 4);
+        tc::mbar_init(drain, 1);
+        for (int i = 0; i < S; i++) {
+            tc::mbar_init(&k_full[i], 1);
+            tc::mbar_init(&k_empty[i], 1);
+            tc::mbar_init(&v_full[i], 1);
+            tc::mbar_init(&v_empty[i], 1);
+        }
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+        tc::tma_prefetch_desc(&tmQ);
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+    }
+    constexpr uint32_t kCols = N == 16 ? 64 : 128;   // S0, S1, O of N columns each
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, kCols);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    const bool any = plan_run<256>(a, a.tok, plan);
+    tc::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_o = tmem_base + 2 * N;
+
+    if (!any) {
+        // nothing to do but free the tensor memory
+    } else if (warp == 0) {
+        // --------------------------------------------------------------- TMA
+        Walk w = plan.start;
+        int seg = 0, st = 0;
+        uint32_t ph = 0, armed = 0, armed_q = 0;      // stages and phases last loaded
+        uint32_t k_ph = 0, v_ph = 0, q_ph = 0, armed_v = 0;
+        bool ok = true;
+        int row = frag_row(a, w, w.j0, lane);
+        do {
+            const int qb = seg & 1;
+            ok = tc::mbar_wait(&q_empty[qb], ((seg >> 1) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) {
+                tc::mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(a.tok * a.group * 128 * kSubs));
+                for (int c = 0; c < kSubs; c++)
+                    tc::tma_load_3d(smem + L::kQ + qb * L::kQTile + c * N * 128, &tmQ, &q_full[qb],
+                                    c * 64, w.h * a.group, w.first + w.rt * a.tok);
+            }
+            armed_q |= 1u << qb;
+            q_ph = (q_ph & ~(1u << qb)) | (((uint32_t)(seg >> 1) & 1u) << qb);
+            const int j1 = w.j1;
+            Walk cur = w;
+            for (int j = cur.j0; j < j1; j++) {
+                const int count = frag_count(row);
+                ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
+                armed |= 1u << st;
+                k_ph = (k_ph & ~(1u << st)) | (ph << st);
+                // the next tile's pages, while the value stage drains
+                int row_next = -1;
+                if (j + 1 < j1) row_next = frag_row(a, cur, j + 1, lane);
+                ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
+                armed_v |= 1u << st;
+                v_ph = (v_ph & ~(1u << st)) | (ph << st);
+                row = row_next;
+                if (++st == S) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+            seg++;
+            if (!ok || !w.next(a, a.tok)) break;
+            row = frag_row(a, w, w.j0, lane);
+        } while (true);
+        if (lane == 0) {
+            // drain our own loads (a no-op when every load was consumed)
+            const uint64_t t0 = tc::globaltimer();
+            auto drain_wait = [&](uint64_t *bar, uint32_t par) {
+                while (!tc::mbar_try_wait(bar, par) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            };
+            for (int i = 0; i < 2; i++)
+                if (armed_q >> i & 1) drain_wait(&q_full[i], q_ph >> i & 1);
+            for (int i = 0; i < S; i++) {
+                if (armed >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
+                if (armed_v >> i & 1) drain_wait(&v_full[i], v_ph >> i & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ----------------------------------------------------------- MMA
+            constexpr uint32_t idesc_s = tc::idesc_f16_f32(kKeys, N, false, false, kBf16);
+            constexpr uint32_t idesc_o = tc::idesc_f16_f32(128, N, true, true, kBf16);
+            const uint32_t sK = tc::smem_u32(smem + L::kK), sV = tc::smem_u32(smem + L::kV);
+            const uint32_t sQ = tc::smem_u32(smem + L::kQ), sP = tc::smem_u32(smem + L::kP);
+            Walk w = plan.start;
+            int seg = 0, st = 0;
+            uint32_t ph = 0, g = 0;
+            bool ok = true, issued = false;
+            // the tile whose P V is still to be issued
+            bool pending = false, pend_first = false;
+            int pend_st = 0, pend_seg = 0;
+            uint32_t pend_ph = 0;
+            auto issue_pv = [&](uint32_t gp) {
+                const int buf = gp & 1;
+                ok = tc::mbar_wait(&v_full[pend_st], pend_ph, abort_flag, err_word, kErrWaitFull) &&
+                     tc::mbar_wait(&p_full[buf], (gp >> 1) & 1, abort_flag, err_word, kErrWaitFull) &&
+                     (!pend_first || tc::mbar_wait(o_free, (pend_seg & 1) ^ 1, abort_flag, err_word,
+                                                   kErrWaitAccum));
+                if (!ok) return;
+                tc::tc_fence_after();
+                const uint32_t vb = sV + pend_st * L::kTile, pb = sP + buf * (kKeys * N * 2);
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; k++)
+                    // (dim 64: the second 64 of the 128 rows repeat the first, unread)
+                    tc::mma_ss<tc::MmaKind::F16>(
+                        tmem_o, tc::sdesc_mnmajor_sw128(vb + k * 2048, D == 128 ? kSubTile : 0, 1024),
+                        tc::sdesc_mnmajor_narrow<N * 2>(pb + k * 16 * N * 2), idesc_o,
+                        (!pend_first || k > 0) ? 1u : 0u);
+                tc::mma_commit(&v_empty[pend_st]);
+                tc::mma_commit(&pv_done[buf]);
+            };
+            do {
+                const int qb = seg & 1;
+                ok = tc::mbar_wait(&q_full[qb], (seg >> 1) & 1, abort_flag, err_word, kErrWaitFull);
+                for (int j = w.j0; j < w.j1 && ok; j++, g++) {
+                    const int buf = g & 1;
+                    ok = tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
+                         tc::mbar_wait(&s_empty[buf], ((g >> 1) & 1) ^ 1, abort_flag, err_word,
+                                       kErrWaitAccum);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t kb = sK + st * L::kTile, qt = sQ + qb * L::kQTile;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)
+                        tc::mma_ss<tc::MmaKind::F16>(
+                            tmem_base + buf * N,
+                            tc::sdesc_kmajor_sw128(kb + (k >> 2) * kSubTile + (k & 3) * 32),
+                            tc::sdesc_kmajor_sw128(qt + (k >> 2) * (N * 128) + (k & 3) * 32), idesc_s,
+                            k > 0 ? 1u : 0u);
+                    issued = true;
+                    tc::mma_commit(&k_empty[st]);
+                    tc::mma_commit(&s_full[buf]);
+                    if (j == w.j1 - 1) tc::mma_commit(&q_empty[qb]);
+                    if (pending) issue_pv(g - 1);
+                    pending = true;
+                    pend_first = j == w.j0;
+                    pend_st = st;
+                    pend_ph = ph;
+                    pend_seg = seg;
+                    if (++st == S) {
+                        st = 0;
+                        ph ^= 1;
+                    }
+                }
+                seg++;
+            } while (ok && w.next(a, a.tok));
+            if (ok && pending) issue_pv(g - 1);
+            if (issued) {
+                tc::mma_commit(drain);
+                const uint64_t t0 = tc::globaltimer();
+                while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // ----------------------------------------------------------- softmax
+        const int key = threadIdx.x - 128, qw = warp & 3;
+        const uint32_t lane_base = (uint32_t)(qw * 32) << 16;
+        float *red = reinterpret_cast<float *>(smem + L::kRed);     // [4][N]
+        float *res = red + 4 * N;                                   // [N]
+        Walk w = plan.start;
+        int st = 0;
+        uint32_t ph = 0, g = 0;
+        T *out = reinterpret_cast<T *>(a.out);
+        bool run = true;
+        do {
+            const int t0 = w.rt * a.tok, ntok = min(a.tok, w.q_len - t0);
+            const int nrows = ntok * a.group;
+            const int seen0 = min(w.kv_len, seen_by(a.s, w.kv_len, w.q_len, t0));   // fewest keys
+            float m[N], l[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                m[n] = -INFINITY;
+                l[n] = 0.0f;
+            }
+            for (int j = w.j0; j < w.j1; j++, g++) {
+                const int buf = g & 1;
+                bool ok = tc::mbar_wait(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                tc::tc_fence_after();
+                float x[N];
+                if (ok) {
+                    uint32_t r[N];
+                    load_columns(tmem_base + buf * N + lane_base, r);
+#pragma unroll
+                    for (int n = 0; n < N; n++) x[n] = __uint_as_float(r[n]) * a.scale_log2;
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s_empty[buf]);
+                const int kk = j * kKeys + key;
+                if (j * kKeys + kKeys > seen0) {
+                    // the rows of token t see the keys before seen_by(t)
+                    int t = t0, i = 0;
+#pragma unroll
+                    for (int n = 0; n < N; n++) {
+                        if (kk >= min(w.kv_len, seen_by(a.s, w.kv_len, w.q_len, t))) x[n] = -INFINITY;
+                        if (++i == a.group) {
+                            i = 0;
+                            t++;
+                        }
+                    }
+                }
+                bool high = j == w.j0;
+#pragma unroll
+                for (int n = 0; n < N; n++) high |= x[n] > m[n] + 8.0f;
+                if (vote_or(high || !ok)) {
+                    float top[N];
+#pragma unroll
+                    for (int n = 0; n < N; n++) top[n] = x[n];
+                    const float mine = reduce_columns<N, true>(top, lane);
+                    if (N == 32 || (lane & 1) == 0) red[qw * N + (N == 32 ? lane : lane >> 1)] = mine;
+                    // (the tile before this one has its P V done: O is stable)
+                    if (ok && j > w.j0)
+                        ok = tc::mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
+                                           kErrWaitAccum);
+                    if (vote_or(!ok)) {
+                        run = false;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    float corr[N];
+                    bool moved = false;
+#pragma unroll
+                    for (int n = 0; n < N; n++) {
+                        const float t4 = fmaxf(fmaxf(red[n], red[N + n]), fmaxf(red[2 * N + n], red[3 * N + n]));
+                        corr[n] = 1.0f;
+                        if (t4 > m[n] + 8.0f || (j == w.j0 && t4 > m[n])) {
+                            corr[n] = tc::ex2(m[n] - t4);
+                            m[n] = t4;
+                            l[n] *= corr[n];
+                            moved = true;
+                        }
+                    }
+                    if (moved && j > w.j0) {
+                        uint32_t o[N];
+                        load_columns(tmem_o + lane_base, o);
+#pragma unroll
+                        for (int n = 0; n < N; n++)
+                            o[n] = __float_as_uint(__uint_as_float(o[n]) * corr[n]);
+                        store_columns(tmem_o + lane_base, o);
+                    }
+                }
+                // P^T of this key: N weights relative to the references
+                uint32_t pk[N / 2];
+#pragma unroll
+                for (int n = 0; n < N; n += 2) {
+                    const float p0 = tc::ex2(x[n] - (m[n] == -INFINITY ? 0.0f : m[n]));
+                    const float p1 = tc::ex2(x[n + 1] - (m[n + 1] == -INFINITY ? 0.0f : m[n + 1]));
+                    l[n] += p0;
+                    l[n + 1] += p1;
+                    pk[n / 2] = pack2<T>(p0, p1);
+                }
+                // its buffer was last read by the P V of tile g - 2
+                if (ok && g >= 2)
+                    ok = tc::mbar_wait(&pv_done[buf], ((g - 2) >> 1) & 1, abort_flag, err_word,
+                                       kErrWaitAccum);
+                const int valid = w.kv_len - j * kKeys;
+                if (valid < kKeys) {
+                    if (ok) ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                    if (ok) clear_rows<kSubs>(smem + L::kV + st * L::kTile, key, valid);
+                }
+                if (ok) {
+                    uint4 *prow = reinterpret_cast<uint4 *>(smem + L::kP + buf * (kKeys * N * 2) +
+                                                            key * N * 2);
+                    const int sw = N == 16 ? (key >> 2) & 1 : (key >> 1) & 3;
+#pragma unroll
+                    for (int c = 0; c < N / 8; c++)
+                        prow[c ^ sw] = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                }
+                tc::fence_proxy_async_smem();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&p_full[buf]);
+                if (++st == S) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+            if (!run) break;
+            // ---- end of the segment: row sums over the keys, O^T / l
+            bool ok = tc::mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
+                                    kErrWaitAccum);
+            float mine = reduce_columns<N, false>(l, lane);
+            if (N == 32 || (lane & 1) == 0) red[qw * N + (N == 32 ? lane : lane >> 1)] = mine;
+            if (vote_or(!ok)) break;
+            tc::tc_fence_after();
+            const bool whole = w.j0 == 0 && w.j1 == w.nt;
+            const int slot = blockIdx.x * 2 + (w.j0 == 0 ? 1 : 0);
+            if (key < N) {
+                const float sum = (red[key] + red[N + key]) + (red[2 * N + key] + red[3 * N + key]);
+                float top = 0.0f;
+#pragma unroll
+                for (int n = 0; n < N; n++) top = key == n ? m[n] : top;
+                res[key] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (key < nrows) {
+                    if (!whole) {
+                        float *ml = a.part_ml + ((size_t)slot * kPartRows + key) * 2;
+                        ml[0] = top;
+                        ml[1] = sum;
+                    } else if (a.lse) {
+                        const int64_t r = (int64_t)(w.first + t0 + key / a.group) * a.heads +
+                                          w.h * a.group + key % a.group;
+                        a.lse[r] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                    }
+                }
+            }
+            softmax_sync();
+            uint32_t o[N];
+            load_columns(tmem_o + lane_base, o);
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(o_free);
+            if (key < D) {
+                if (whole) {
+                    int t = 0, i = 0;
+#pragma unroll
+                    for (int n = 0; n < N; n++) {
+                        if (n < nrows)
+                            out[((int64_t)(w.first + t0 + t) * a.heads + w.h * a.group + i) * D + key] =
+                                from_f32<T>(__uint_as_float(o[n]) * res[n]);
+                        if (++i == a.group) {
+                            i = 0;
+                            t++;
+                        }
+                    }
+                } else {
+                    float *po = a.part_o + (size_t)slot * kPartRows * D + key;
+#pragma unroll
+                    for (int n = 0; n < N; n++)
+                        if (n < nrows) po[n * D] = __uint_as_float(o[n]);
+                }
+            }
+            Walk last = w;
+            if (!w.next(a, a.tok)) {
+                if (key == 0) note_parts(a, plan, last, a.tok);
+                break;
+            }
+        } while (true);
+    }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tc::tmem_dealloc(tmem_base, kCols);
+    }
+}
+
+template <typename T, int D, int N>
+int launch_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+               const PagedTc &a) {
+    using L = DecSmem<D, N>;
+    static_assert(L::kTotal <= 232448, "shared memory of one CTA");
+    static bool attr_done[64] = {};
+    if (!attr_done[d->ordinal & 63]) {
+        if (int rc = check(cudaFuncSetAttribute(paged_dec_kernel<T, D, N>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                L::kTotal),
+                           "cudaFuncSetAttribute(paged_dec)"))
+            return rc;
+        attr_done[d->ordinal & 63] = true;
+    }
+    paged_dec_kernel<T, D, N><<<d->sms, 256, L::kTotal, d->stream>>>(mq, mk, mv, a);
+    return HEXCUDA_OK;
+}
+
+}  // namespace
+
+int launch_paged_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                     PagedTc &a, int dtype, int dim, int rows) {
+    if (dtype == HEXCUDA_F16) {
+        if (dim == 128)
+            return rows == 16 ? launch_dec<__half, 128, 16>(d, mq, mk, mv, a)
+                              : launch_dec<__half, 128, 32>(d, mq, mk, mv, a);
+        return rows == 16 ? launch_dec<__half, 64, 16>(d, mq, mk, mv, a)
+                          : launch_dec<__half, 64, 32>(d, mq, mk, mv, a);
+    }
+    if (dim == 128)
+        return rows == 16 ? launch_dec<__nv_bfloat16, 128, 16>(d, mq, mk, mv, a)
+                          : launch_dec<__nv_bfloat16, 128, 32>(d, mq, mk, mv, a);
+    return rows == 16 ? launch_dec<__nv_bfloat16, 64, 16>(d, mq, mk, mv, a)
+                      : launch_dec<__nv_bfloat16, 64, 32>(d, mq, mk, mv, a);
+}
+
+}  // namespace hx

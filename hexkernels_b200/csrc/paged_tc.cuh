@@ -1,0 +1,243 @@
+// paged_tc.cuh -- what the tensor-core kernels over the paged cache share:
+// the tensor maps, the loads of a 128-key tile page by page, and the even
+// split of a ragged batch over the CTAs.
+//
+// Split.  A work item is (sequence, key head, tile of query rows) and takes
+// ceil(keys its last row sees / 128) key tiles, at least one (a row that sees
+// nothing is still written).  The tiles of all items, in that order, are
+// numbered 0 .. T - 1 and CTA c of C takes c T / C .. (c + 1) T / C - 1: a
+// run of items, the first and the last perhaps only in part.  Lengths live on
+// the device, so each CTA derives its own run from them (a prefix sum over the
+// sequences).  An item that is cut leaves one partial result per CTA: the
+// unnormalised output, the reference maximum and the sum of each row.  A
+// second kernel joins them, in CTA order, so results do not depend on timing.
+#pragma once
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace hx {
+
+constexpr int kKeys = 128;              // keys per tile
+constexpr int kSubTile = kKeys * 128;   // 64 columns of a key tile: 128 rows x 128 bytes
+constexpr int kPartRows = 256;          // rows of a partial result, at most
+
+struct PartRec {
+    int h, row0, ntok, nparts;          // nparts 0: the CTA's last item is not its to join
+};
+
+// What both attention kernels get.
+struct PagedTc {
+    PagedSeqs s;
+    int heads, kv_heads, group;
+    int tok;                 // tokens of a query tile: rows / group
+    int frag;                // rows of one page load: a power of two, 8 to 128
+    int map_rows;            // rows of the cache: a coordinate behind the last
+    int min_tiles;           // fewer tiles than this are not worth a CTA
+    float scale_log2;        // scale * log2(e)
+    void *out;
+    float *lse;
+    PartRec *recs;           // [grid]
+    float *part_ml;          // [grid][2][kPartRows][2]: reference maximum, sum
+    float *part_o;           // [grid][2][kPartRows][D]
+};
+
+// Tokens of a sequence without raising the error word (the plan has).
+__device__ __forceinline__ void quiet_seq(const PagedSeqs &s, int b, int &first, int &q_len,
+                                          int &kv_len) {
+    first = s.q_offs[b];
+    const int end = s.q_offs[b + 1];
+    q_len = first >= 0 && end >= first && end <= s.total_q ? end - first : 0;
+    const int n = s.kv_lens[b];
+    const long long cap = (long long)s.max_pages * s.page_size;
+    kv_len = n < 0 ? 0 : n > cap ? (int)cap : n;
+}
+
+// Key tiles that the tokens before `end` see.
+__device__ __forceinline__ int tiles_to(const PagedSeqs &s, int kv_len, int q_len, int end) {
+    const int seen = seen_by(s, kv_len, q_len, min(end, q_len) - 1);
+    return max(1, (seen + kKeys - 1) / kKeys);
+}
+
+// A CTA's run of items, one segment (item, key tiles j0 .. j1 - 1) at a time.
+// Every role of the CTA walks its own copy.
+struct Walk {
+    int b, h, rt, j0, j1, nt;
+    int first, q_len, kv_len;
+    long long pos, end;      // first tile of the segment, end of the run
+
+    // the segment at (b, h, rt, j0), pos
+    __device__ __forceinline__ void open(const PagedTc &a, int item_tok) {
+        nt = tiles_to(a.s, kv_len, q_len, (rt + 1) * item_tok);
+        const long long left = end - pos;
+        j1 = left < nt - j0 ? j0 + (int)left : nt;
+    }
+    __device__ __forceinline__ bool next(const PagedTc &a, int item_tok) {
+        pos += j1 - j0;
+        if (pos >= end) return false;
+        j0 = 0;
+        if (++rt * item_tok >= q_len) {
+            rt = 0;
+            if (++h == a.kv_heads) {
+                h = 0;
+                do {
+                    if (++b >= a.s.batch) return false;
+                    quiet_seq(a.s, b, first, q_len, kv_len);
+                } while (q_len == 0);
+            }
+        }
+        open(a, item_tok);
+        return true;
+    }
+};
+
+struct PlanShared {
+    long long sums[32];
+    Walk start;
+    int ctas;
+    long long total;
+};
+
+// Whole block.  Leaves this CTA's first segment in sh.start; false when it has
+// none.  item_tok: tokens of an item (one or two query tiles).
+template <int THREADS>
+__device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanShared &sh) {
+    const int per = (a.s.batch + THREADS - 1) / THREADS;
+    const int b0 = min(a.s.batch, (int)threadIdx.x * per), b1 = min(a.s.batch, b0 + per);
+    auto tiles_of = [&](int q_len, int kv_len) {
+        long long n = 0;
+        for (int t = item_tok; t - item_tok < q_len; t += item_tok)
+            n += tiles_to(a.s, kv_len, q_len, t);
+        return n;
+    };
+    long long mine = 0;
+    for (int b = b0; b < b1; b++) {
+        int first;
+        const int q_len = seq_q_len(a.s, b, first), kv_len = seq_kv_len(a.s, b);
+        mine += tiles_of(q_len, kv_len) * a.kv_heads;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) sh.sums[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) upto += sh.sums[w];
+        total += sh.sums[w];
+    }
+    const long long want = (total + a.min_tiles - 1) / a.min_tiles;
+    const int ctas = want < (int)gridDim.x ? (int)want : (int)gridDim.x;
+    const bool any = (int)blockIdx.x < ctas;
+    if (any) {
+        const long long lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1LL) * total / ctas;
+        if (upto - mine <= lo && lo < upto) {
+            long long at = lo - (upto - mine);
+            Walk w;
+            for (int b = b0; b < b1; b++) {
+                quiet_seq(a.s, b, w.first, w.q_len, w.kv_len);
+                const long long n = tiles_of(w.q_len, w.kv_len);
+                if (at >= n * a.kv_heads) {
+                    at -= n * a.kv_heads;
+                    continue;
+                }
+                w.b = b;
+                w.h = (int)(at / n);
+                at -= w.h * n;
+                for (w.rt = 0;; w.rt++) {
+                    const int nt = tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok);
+                    if (at < nt) break;
+                    at -= nt;
+                }
+                w.j0 = (int)at;
+                break;
+            }
+            w.pos = lo;
+            w.end = hi;
+            w.open(a, item_tok);
+            sh.start = w;
+            sh.ctas = ctas;
+            sh.total = total;
+        }
+    }
+    if (threadIdx.x == 0) a.recs[blockIdx.x] = PartRec{0, 0, 0, 0};
+    __syncthreads();
+    return any;
+}
+
+// One thread, once the CTA's last segment `w` is known: whether this CTA joins
+// its item's parts (it holds the first of several).
+__device__ __forceinline__ void note_parts(const PagedTc &a, const PlanShared &sh, const Walk &w,
+                                           int item_tok) {
+    PartRec r{0, 0, 0, 0};
+    if (w.j0 == 0 && w.j1 < w.nt) {
+        // the CTA that holds the item's last tile e - 1: the largest c with c T / C <= e - 1
+        const long long e = w.pos + w.nt;
+        r.h = w.h;
+        r.row0 = w.first + w.rt * item_tok;
+        r.ntok = min(item_tok, w.q_len - w.rt * item_tok);
+        r.nparts = (int)((e * sh.ctas - 1) / sh.total) - (int)blockIdx.x + 1;
+    }
+    a.recs[blockIdx.x] = r;
+}
+
+// ---- one warp: the page loads of a key tile ----
+
+// Lane f's fragment of tile j: the row of the cache where it starts, or -1
+// when no cached token lies in it.
+__device__ __forceinline__ int frag_row(const PagedTc &a, const Walk &w, int j, int lane) {
+    const int t = j * kKeys + lane * a.frag;
+    if (lane * a.frag >= kKeys || t >= w.kv_len) return -1;
+    const int i = t / a.s.page_size;
+    const int page = seq_page(a.s, w.b, i);
+    return page < 0 ? a.map_rows : (page * a.kv_heads + w.h) * a.s.page_size + (t - i * a.s.page_size);
+}
+// Fragments that hold cached tokens (the lanes with a row).
+__device__ __forceinline__ int frag_count(int row) {
+    return __popc(__ballot_sync(0xffffffffu, row >= 0));
+}
+template <int SUBS>
+__device__ __forceinline__ void load_frags(const PagedTc &a, uint8_t *dst, const CUtensorMap *map,
+                                           uint64_t *bar, int row, int count, int lane) {
+    if (lane == 0)
+        tc::mbar_arrive_expect_tx(bar, (uint32_t)(count * a.frag * 128 * SUBS));
+    __syncwarp();
+    if (row >= 0)
+        for (int c = 0; c < SUBS; c++)
+            tc::tma_load_2d(dst + c * kSubTile + lane * a.frag * 128, map, bar, c * 64, row);
+    __syncwarp();
+}
+
+// One thread per key: zeros in the value rows of a tile from `valid` on, which
+// no cached token fills (a weight of zero times not-a-number is not zero).
+template <int SUBS>
+__device__ __forceinline__ void clear_rows(uint8_t *tile, int key, int valid) {
+    if (key < valid) return;
+    for (int c = 0; c < SUBS; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            reinterpret_cast<uint4 *>(tile + c * kSubTile + key * 128)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- host side (paged_attn.cu) ----
+
+// The cache's pages as a matrix [num_pages * kv_heads * page_size][dim], box
+// 64 x frag; q as [total_q][heads][dim], box 64 x group x tok.  Both 128-byte
+// swizzle.
+int make_page_map(CUtensorMap *map, const void *base, int64_t rows, int dim, int frag);
+int make_query_map(CUtensorMap *map, const void *base, int total_q, int heads, int dim, int group,
+                   int tok);
+
+// Whether the tensor-core kernels take these tensors: TMA boxes start on 16
+// bytes and hold whole 8-row swizzle atoms, coordinates fit 31 bits.
+bool paged_tc_fits(const void *q, const void *k, const void *v, const void *out, int heads,
+                   int kv_heads, int dim, int num_pages, int page_size);
+
+int launch_paged_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                     PagedTc &a, int dtype, int dim, int rows);
+int launch_paged_pre(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                     PagedTc &a, int dtype, int dim);
+
+}  // namespace hx

@@ -438,6 +438,20 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr, uint32_t
     return d;
 }
 
+// MN-major operand of `ROW` = 32 or 64 bytes along M/N (16 or 32 16-bit
+// values, one chunk): K-rows of that many bytes, 8 rows an atom, swizzled over
+// as many bytes; consecutive 8-row K groups follow one another.
+template <int ROW>
+__device__ __forceinline__ uint64_t sdesc_mnmajor_narrow(uint32_t saddr) {
+    static_assert(ROW == 32 || ROW == 64, "one 32- or 64-byte swizzle row");
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((8u * ROW) >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)(ROW == 32 ? 6 : 4) << 61;
+    return d;
+}
+
 // The 32 x 64-byte block of a warp (lane i holding row row0 + i, 16 words)
 // stored with each row written by 4 consecutive lanes: staged through the
 // warp's 2 KB of shared memory (16-byte chunks XOR-swizzled by row pair, so
@@ -483,9 +497,11 @@ __device__ __forceinline__ void store_block32_coalesced(const uint32_t (&w)[8], 
     }
 }
 
-__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, bool b_mn_major = false) {
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, bool b_mn_major = false,
+                                                     bool a_mn_major = false, bool bf16 = false) {
     return (1u << 4)                          // D = f32
-           | (0u << 7) | (0u << 10)           // A, B = f16
+           | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10)   // A, B = f16 or both bf16
+           | ((a_mn_major ? 1u : 0u) << 15)   // A major-ness
            | ((b_mn_major ? 1u : 0u) << 16)   // B major-ness
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
