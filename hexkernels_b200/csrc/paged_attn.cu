@@ -285,11 +285,12 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
     PagedSeqs s{block_table, kv_lens, q_offs, batch, total_q, num_pages, page_size,
                 max_pages, causal, d->err_word};
     const int group = heads / kv_heads;
-    // Up to 32 query rows share a key head: the decoding kernel.
+    // Up to 32 query rows share a key head: the decoding kernel, of 16 or 32 rows.
+    // More: 128-row tiles.
     const int64_t rows = (int64_t)(max_q < 1 ? 1 : max_q) * group;
-    if (rows <= 32 &&
-        paged_tc_fits(q, k_pages, v_pages, out, heads, kv_heads, head_dim, num_pages, page_size)) {
-        const int n = rows <= 16 ? 16 : 32;
+    if (paged_tc_fits(q, k_pages, v_pages, out, heads, kv_heads, head_dim, num_pages, page_size)) {
+        const bool few = rows <= 32;
+        const int n = rows <= 16 ? 16 : few ? 32 : 128;
         PagedTc a;
         a.s = s;
         a.heads = heads;
@@ -313,13 +314,16 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
         if (int rc = make_page_map(&mk, k_pages, a.map_rows, head_dim, a.frag)) return rc;
         if (int rc = make_page_map(&mv, v_pages, a.map_rows, head_dim, a.frag)) return rc;
         launch_begin(d);
-        if (int rc = launch_paged_dec(d, mq, mk, mv, a, dtype, head_dim, n)) return rc;
+        if (int rc = few ? launch_paged_dec(d, mq, mk, mv, a, dtype, head_dim, n)
+                         : launch_paged_pre(d, mq, mk, mv, a, dtype, head_dim))
+            return rc;
         const bool half = dtype == HEXCUDA_F16;
+        const int join_rows = few ? n : 2 * n;      // of one item
         if (int rc = head_dim == 128
-                         ? (half ? launch_join<__half, 128>(d, a, n)
-                                 : launch_join<__nv_bfloat16, 128>(d, a, n))
-                         : (half ? launch_join<__half, 64>(d, a, n)
-                                 : launch_join<__nv_bfloat16, 64>(d, a, n)))
+                         ? (half ? launch_join<__half, 128>(d, a, join_rows)
+                                 : launch_join<__nv_bfloat16, 128>(d, a, join_rows))
+                         : (half ? launch_join<__half, 64>(d, a, join_rows)
+                                 : launch_join<__nv_bfloat16, 64>(d, a, join_rows)))
             return rc;
         note_mech(kMechTcgen05 | kMechTma);
         return launch_end(d, "paged_attn", 2);

@@ -1,0 +1,567 @@
+// paged_pre.cu -- attention of chunks of new tokens over the paged cache
+// (more than 32 query rows to a key head) on the tensor cores, queries on the
+// M side.
+//
+// A work item is 2 x 128 query rows of one key head: with group = heads /
+// kv_heads a tile holds tok = 128 / group tokens x group heads, so that the
+// heads that share a key head also share its key and value loads (rows past
+// tok * group are computed and dropped).  One softmax warpgroup per tile, one
+// query row per thread, so the tensor pipe works for one tile while the other
+// tile's warpgroup takes its exponentials; the order of the MMAs, the
+// two-halves hand-over of P and the lazy reference maximum are those of the
+// dense ping-pong kernel (attn_tc.cu).  New here are the loads (a key tile is
+// gathered page by page, one lane of the TMA warp per fragment), the ragged
+// batch (paged_tc.cuh: every CTA gets the same number of key tiles; an item
+// that is cut leaves partial results), and the values behind the last cached
+// token, which are zeroed before they meet a weight of zero.
+//
+// Per CTA (one per SM), 384 threads in three warpgroups: warp 0 TMA, warp 1
+// tensor memory and MMA issue; warpgroups 1 and 2 softmax of tiles a and b.
+// TMEM: S_a [0,128), S_b [128,256), O_a [256,..), O_b [384,..); P_x over S_x.
+//
+// Every wait is bounded; see mbar_wait.
+#include <math.h>
+
+#include "paged_tc.cuh"
+
+namespace hx {
+namespace {
+
+// The register file is split with setmaxnreg: the control warpgroup drops to
+// kRegsCtl, the softmax warpgroups rise to kRegsSoftmax (a whole score row of
+// 128 fp32 and its weights).
+constexpr int kRegsCtl = 104;
+constexpr int kRegsSoftmax = 200;
+constexpr int kRegsPool = 128 * kRegsCtl + 256 * kRegsSoftmax;
+
+template <int D>
+struct PreSmem {
+    static constexpr int kSubs = D / 64;
+    static constexpr int kStages = D == 128 ? 2 : 4;
+    static constexpr int kTile = kSubs * kSubTile;
+    static constexpr int kQ = 0;                           // Q_a, Q_b
+    static constexpr int kK = 2 * kTile;
+    static constexpr int kV = kK + kStages * kTile;
+    static constexpr int kPlan = kV + kStages * kTile;
+    static constexpr int kWalk = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;   // a Walk per softmax warp
+    static constexpr int kBar = (kWalk + 8 * (int)sizeof(Walk) + 15) / 16 * 16;
+    // q_full, q_empty, s_full[2], p_full[2], p_half[2], pv_done[2], o_free[2],
+    // drain, k_full, k_empty, v_full, v_empty [stages]
+    static constexpr int kNumBars = 13 + 4 * kStages;
+    static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
+};
+
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Tile x of segment w: its first token, its tokens, and the end of its key
+// tiles in the segment (j0 when it has none).
+__device__ __forceinline__ void tile_span(const PagedTc &a, const Walk &w, int x, int &t0, int &ntok,
+                                          int &hi) {
+    t0 = (2 * w.rt + x) * a.tok;
+    ntok = min(a.tok, w.q_len - t0);
+    hi = ntok > 0 ? max(w.j0, min(w.j1, tiles_to(a.s, w.kv_len, w.q_len, t0 + a.tok))) : w.j0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(384, 1)
+    paged_pre_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const PagedTc a) {
+    using L = PreSmem<D>;
+    constexpr int kSubs = L::kSubs, S = L::kStages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4;
+    uint64_t *p_half = bars + 6, *pv_done = bars + 8, *o_free = bars + 10, *drain = bars + 12;
+    uint64_t *k_full = bars + 13, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err_word = a.s.err_word;
+    const int item_tok = 2 * a.tok;
+    tc::launch_dependents();
+
+    if (threadIdx.x == 0) {
+        tc::mbar_init(q_full, 1);
+        tc::mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; x++) {
+            tc::mbar_init(&s_full[x], 1);
+            tc::mbar_init(&p_full[x], 4);
+            tc::mbar_init(&p_half[x], 4);
+            tc::mbar_init(&pv_done[x], 1);
+            tc::mbar_init(&o_free[x], 4);
+        }
+        tc::mbar_init(drain, 1);
+        for (int i = 0; i < S; i++) {
+            tc::mbar_init(&k_full[i], 1);
+            tc::mbar_init(&k_empty[i], 1);
+            tc::mbar_init(&v_full[i], 1);
+            tc::mbar_init(&v_empty[i], 1);
+        }
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+        tc::tma_prefetch_desc(&tmQ);
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    const bool any = plan_run<384>(a, item_tok, plan);
+    tc::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp < 4) {
+      // warpgroup 0: one setmaxnreg for all four warps, then the roles
+      tc::setmaxnreg_dec<kRegsCtl>();
+      if (!any) {
+        // nothing to do but free the tensor memory
+      } else if (warp == 0) {
+        // --------------------------------------------------------------- TMA
+        Walk w = plan.start;
+        int seg = 0, st = 0;
+        uint32_t ph = 0, armed_k = 0, armed_v = 0, k_ph = 0, v_ph = 0;
+        bool ok = true;
+        int row = frag_row(a, w, w.j0, lane);
+        do {
+            int t0, ntok_a, ntok_b, hi;
+            tile_span(a, w, 1, t0, ntok_b, hi);
+            tile_span(a, w, 0, t0, ntok_a, hi);
+            ok = tc::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) {
+                const int tiles = ntok_b > 0 ? 2 : 1;
+                tc::mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * a.tok * a.group * 128 * kSubs));
+                for (int x = 0; x < tiles; x++)
+                    for (int c = 0; c < kSubs; c++)
+                        tc::tma_load_3d(smem + L::kQ + x * L::kTile + c * kSubTile, &tmQ, q_full,
+                                        c * 64, w.h * a.group, w.first + t0 + x * a.tok);
+            }
+            const int j1 = w.j1;
+            for (int j = w.j0; j < j1; j++) {
+                const int count = frag_count(row);
+                ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
+                armed_k |= 1u << st;
+                k_ph = (k_ph & ~(1u << st)) | (ph << st);
+                // the next tile's pages, while the value stage drains
+                const int row_next = j + 1 < j1 ? frag_row(a, w, j + 1, lane) : -1;
+                ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
+                armed_v |= 1u << st;
+                v_ph = (v_ph & ~(1u << st)) | (ph << st);
+                row = row_next;
+                if (++st == S) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+            seg++;
+            if (!ok || !w.next(a, item_tok)) break;
+            row = frag_row(a, w, w.j0, lane);
+        } while (true);
+        if (lane == 0) {
+            // drain our own loads (a no-op when every load was consumed)
+            const uint64_t t0 = tc::globaltimer();
+            auto drain_wait = [&](uint64_t *bar, uint32_t par) {
+                while (!tc::mbar_try_wait(bar, par) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            };
+            // (the last segment whose Q was loaded: seg - 1, or seg when its
+            // key loop was left early, which seg++ has counted too)
+            if (seg > 0) drain_wait(q_full, (seg - 1) & 1);
+            for (int i = 0; i < S; i++) {
+                if (armed_k >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
+                if (armed_v >> i & 1) drain_wait(&v_full[i], v_ph >> i & 1);
+            }
+        }
+      } else if (warp == 1) {
+        if (lane == 0) {
+            // ----------------------------------------------------------- MMA
+            constexpr uint32_t idesc_s = tc::idesc_f16_f32(128, kKeys, false, false, kBf16);
+            constexpr uint32_t idesc_o = tc::idesc_f16_f32(128, D, true, false, kBf16);
+            const uint32_t sQ = tc::smem_u32(smem + L::kQ);
+            const uint32_t sK = tc::smem_u32(smem + L::kK);
+            const uint32_t sV = tc::smem_u32(smem + L::kV);
+            Walk w = plan.start;
+            int seg = 0, st = 0;
+            uint32_t ph = 0;
+            uint32_t n[2] = {0, 0}, segs[2] = {0, 0};    // key tiles and segments of each tile so far
+            bool issued = false, ok = true;
+            auto issue_s = [&](int x, int stage) {
+                const uint32_t kb = sK + stage * L::kTile, qb = sQ + x * L::kTile;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    const uint32_t off = (k >> 2) * kSubTile + (k & 3) * 32;
+                    tc::mma_ss<tc::MmaKind::F16>(tmem_base + x * 128, tc::sdesc_kmajor_sw128(qb + off),
+                                                 tc::sdesc_kmajor_sw128(kb + off), idesc_s,
+                                                 k > 0 ? 1u : 0u);
+                }
+                tc::mma_commit(&s_full[x]);
+                issued = true;
+            };
+            // O_x += P_x V for the keys of K steps k0 .. k0+3 (64 keys)
+            auto issue_pv = [&](int x, int stage, bool first, int k0) {
+                const uint32_t vb = sV + stage * L::kTile;
+#pragma unroll
+                for (int k = k0; k < k0 + 4; k++)
+                    tc::mma_ts_f16(tmem_base + 256 + x * 128, tmem_base + x * 128 + k * 8,
+                                   tc::sdesc_mnmajor_sw128(vb + k * 2048, kSubTile, 1024), idesc_o,
+                                   (!first || k > 0) ? 1u : 0u);
+            };
+            do {
+                int t0, ntok, hi[2];
+                tile_span(a, w, 0, t0, ntok, hi[0]);
+                tile_span(a, w, 1, t0, ntok, hi[1]);
+                const int j0 = w.j0, j1 = w.j1;
+                ok = tc::mbar_wait(q_full, seg & 1, abort_flag, err_word, kErrWaitFull) &&
+                     tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                if (!ok) break;
+                tc::tc_fence_after();
+                for (int x = 0; x < 2; x++)
+                    if (hi[x] > j0) issue_s(x, st);
+                tc::mma_commit(&k_empty[st]);
+                if (j1 - j0 == 1) tc::mma_commit(q_empty);
+                for (int j = j0; j < j1 && ok; j++) {
+                    ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                    int st_next = st + 1;
+                    uint32_t ph_next = ph;
+                    if (st_next == S) {
+                        st_next = 0;
+                        ph_next ^= 1;
+                    }
+                    // the last tile that takes this stage, and the next one's
+                    const int last = j < hi[1] ? 1 : 0, last_next = j + 1 < hi[1] ? 1 : 0;
+                    bool k_ready = false;
+                    for (int x = 0; x < 2 && ok; x++) {
+                        if (j >= hi[x]) continue;
+                        const uint32_t c = n[x] + (j - j0);
+                        // the first 64 keys' P V runs while the softmax warps
+                        // still compute the other half of P
+                        ok = tc::mbar_wait(&p_half[x], c & 1, abort_flag, err_word, kErrWaitFull) &&
+                             (j > j0 || tc::mbar_wait(&o_free[x], (segs[x] & 1) ^ 1, abort_flag,
+                                                      err_word, kErrWaitAccum));
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_pv(x, st, j == j0, 0);
+                        ok = tc::mbar_wait(&p_full[x], c & 1, abort_flag, err_word, kErrWaitFull);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_pv(x, st, false, 4);
+                        tc::mma_commit(&pv_done[x]);
+                        if (x == last) tc::mma_commit(&v_empty[st]);
+                        if (j + 1 < hi[x]) {
+                            if (!k_ready) {
+                                ok = tc::mbar_wait(&k_full[st_next], ph_next, abort_flag, err_word,
+                                                   kErrWaitFull);
+                                if (!ok) break;
+                                tc::tc_fence_after();
+                                k_ready = true;
+                            }
+                            issue_s(x, st_next);
+                            if (x == last_next) {
+                                tc::mma_commit(&k_empty[st_next]);
+                                if (j + 1 == j1 - 1) tc::mma_commit(q_empty);
+                            }
+                        }
+                    }
+                    st = st_next;
+                    ph = ph_next;
+                }
+                for (int x = 0; x < 2; x++)
+                    if (hi[x] > j0) {
+                        n[x] += hi[x] - j0;
+                        segs[x]++;
+                    }
+                seg++;
+            } while (ok && w.next(a, item_tok));
+            if (issued) {
+                tc::mma_commit(drain);
+                const uint64_t t0 = tc::globaltimer();
+                while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            }
+        }
+      }
+    } else {
+        // ------------------------------------------------------- softmax x
+        tc::setmaxnreg_inc<kRegsSoftmax>();
+        const int x = (warp - 4) >> 2;
+        const int q = warp & 3;
+        const int row = q * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+        const uint32_t s_addr = tmem_base + lane_base + x * 128;
+        const uint32_t o_addr = tmem_base + lane_base + 256 + x * 128;
+        Walk *wp = reinterpret_cast<Walk *>(smem + L::kWalk) + (warp - 4);
+        uint32_t n = 0;
+        int g0 = 0;               // key tiles of the CTA's earlier segments (the value ring)
+        bool more = any;
+        if (any && lane == 0) *wp = plan.start;
+        __syncwarp();
+        while (more) {
+            int t0, ntok, hi, hi_a;
+            tile_span(a, *wp, 0, t0, ntok, hi_a);
+            tile_span(a, *wp, x, t0, ntok, hi);
+            const int j0 = wp->j0, kv_len = wp->kv_len;
+            const int tok_row = row / a.group;
+            const int lim = min(kv_len, seen_by(a.s, kv_len, wp->q_len, t0 + tok_row));
+            const int lim0 = min(kv_len, seen_by(a.s, kv_len, wp->q_len, t0));   // the tile's fewest
+            float m_ref = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = j0; j < hi; j++) {
+                const uint32_t c = n + (j - j0);
+                ok = tc::mbar_wait(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc::tc_fence_after();
+                const int key0 = j * kKeys;
+                // the whole score row into registers: four loads, one wait
+                uint32_t sr[4][32];
+#pragma unroll
+                for (int cc = 0; cc < 4; cc++) tc::tmem_ld_32x32b_x32(s_addr + cc * 32, sr[cc]);
+                tc::tmem_ld_wait(sr[0]);
+                tc::reg_fence(sr[1]);
+                tc::reg_fence(sr[2]);
+                tc::reg_fence(sr[3]);
+                if (key0 + kKeys > lim0) {
+                    const int rest = lim - key0;
+#pragma unroll
+                    for (int cc = 0; cc < 4; cc++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (cc * 32 + e >= rest) sr[cc][e] = __float_as_uint(-INFINITY);
+                }
+                // row max over the 128 raw scores (scale folded later)
+                float mx[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) mx[u] = -INFINITY;
+#pragma unroll
+                for (int cc = 0; cc < 4; cc++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        mx[i & 7] = max3(mx[i & 7], __uint_as_float(sr[cc][2 * i]),
+                                         __uint_as_float(sr[cc][2 * i + 1]));
+                const float mt = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]),
+                                      fmaxf(mx[6], mx[7])) *
+                                 a.scale_log2;
+                const float m_new = fmaxf(m_ref, mt);
+                if (j == j0) {
+                    m_ref = m_new;
+                } else {
+                    // Lazy rescale: the reference max moves only when the row
+                    // max rose by more than 8 (P stays below 2^8 otherwise).
+                    const bool need = m_new > m_ref + 8.0f;
+                    if (__any_sync(0xffffffffu, need)) {
+                        ok = tc::mbar_wait(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
+                                           kErrWaitAccum);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        tc::tc_fence_after();
+                        const float corr = need ? tc::ex2(m_ref - m_new) : 1.0f;
+#pragma unroll 1
+                        for (int cc = 0; cc < D / 32; cc++) {
+                            uint32_t o[32];
+                            tc::tmem_ld_32x32b_x32(o_addr + cc * 32, o);
+                            tc::tmem_ld_wait(o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                            tc::tmem_st_32x32b_x32(o_addr + cc * 32, o);
+                        }
+                        tc::tmem_st_wait();
+                        if (need) {
+                            l *= corr;
+                            m_ref = m_new;
+                        }
+                    }
+                }
+                if (key0 + kKeys > kv_len && (x == 0 || j >= hi_a)) {
+                    // values behind the last cached token (the first tile to
+                    // take this stage clears them; its first half of P is taken
+                // when all four warps have handed it over)
+                    const int gk = g0 + (j - j0);
+                    ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, kv_len - key0);
+                    tc::fence_proxy_async_smem();
+                }
+                // P = 2^(s*scale*log2e - m_ref) from the registers, as 16-bit
+                // pairs over S columns 16cc..16cc+15; the row sum in four
+                // packed pairs.  A row that sees nothing yet has no reference.
+                uint64_t acc2[4] = {0, 0, 0, 0};
+                const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
+                const uint64_t sl2 = pair(a.scale_log2, a.scale_log2), nm2 = pair(nm, nm);
+#pragma unroll
+                for (int cc = 0; cc < 4; cc++) {
+                    if (cc == 2) {
+                        // keys 0..63 of P are in TMEM: hand them to the MMA warp
+                        tc::tmem_st_wait();
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&p_half[x]);
+                    }
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        float a0, a1;
+                        unpair(fma_pair(pair(__uint_as_float(sr[cc][2 * e]),
+                                             __uint_as_float(sr[cc][2 * e + 1])),
+                                        sl2, nm2),
+                               a0, a1);
+                        const float p0 = tc::ex2(a0), p1 = tc::ex2(a1);
+                        acc2[e & 3] = add_pair(acc2[e & 3], pair(p0, p1));
+                        pk[e] = pack2<T>(p0, p1);
+                    }
+                    tc::tmem_st_32x32b_x16(s_addr + cc * 16, pk);
+                }
+                tc::tmem_st_wait();
+                {
+                    float s0, s1, s2, s3, s4, s5, s6, s7;
+                    unpair(acc2[0], s0, s1);
+                    unpair(acc2[1], s2, s3);
+                    unpair(acc2[2], s4, s5);
+                    unpair(acc2[3], s6, s7);
+                    l += ((s0 + s1) + (s2 + s3)) + ((s4 + s5) + (s6 + s7));
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&p_full[x]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            // ---- end of the segment
+            const bool whole = j0 == 0 && wp->j1 == wp->nt;
+            const bool live = tok_row < ntok && row < a.tok * a.group;
+            const size_t prow = ((size_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0)) * kPartRows + x * 128 + row;
+            const int64_t orow = (int64_t)(wp->first + t0 + tok_row) * a.heads + wp->h * a.group +
+                                 row % a.group;
+            if (hi > j0) {
+                n += hi - j0;
+                ok = tc::mbar_wait(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc::tc_fence_after();
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+                for (int cc = 0; cc < D / 32; cc++) {
+                    uint32_t o[32];
+                    tc::tmem_ld_32x32b_x32(o_addr + cc * 32, o);
+                    tc::tmem_ld_wait(o);
+                    if (!live) continue;
+                    if (whole) {
+                        uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + orow * D +
+                                                               cc * 32);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                v[i] = pack2<T>(__uint_as_float(o[8 * e + 2 * i]) * inv,
+                                                __uint_as_float(o[8 * e + 2 * i + 1]) * inv);
+                            dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
+                        }
+                    } else {
+                        uint4 *dst = reinterpret_cast<uint4 *>(a.part_o + prow * D + cc * 32);
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&o_free[x]);
+            }
+            if (live) {
+                if (!whole) {
+                    reinterpret_cast<float2 *>(a.part_ml)[prow] = make_float2(m_ref, l);
+                } else if (a.lse) {
+                    a.lse[orow] = l == 0.0f ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+            g0 += wp->j1 - j0;
+            __syncwarp();
+            if (lane == 0) {
+                const Walk last = *wp;
+                more = wp->next(a, item_tok);
+                if (!more && warp == 4) note_parts(a, plan, last, item_tok);
+            }
+            more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+            __syncwarp();
+        }
+    }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tc::tmem_dealloc(tmem_base, 512);
+    }
+}
+
+template <typename T, int D>
+int launch_pre(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+               const PagedTc &a) {
+    using L = PreSmem<D>;
+    static_assert(L::kTotal <= 232448, "shared memory of one CTA");
+    static bool attr_done[64] = {};
+    if (!attr_done[d->ordinal & 63]) {
+        auto kern = paged_pre_kernel<T, D>;
+        if (int rc = check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                L::kTotal),
+                           "cudaFuncSetAttribute(paged_pre)"))
+            return rc;
+        // setmaxnreg.inc draws on the registers of the launch: a build with
+        // fewer would leave it waiting, so refuse it
+        cudaFuncAttributes fa;
+        if (int rc = check(cudaFuncGetAttributes(&fa, kern), "cudaFuncGetAttributes(paged_pre)"))
+            return rc;
+        if (fa.numRegs * 384 < kRegsPool)
+            return fail(HEXCUDA_ERR_CUDA, "paged_pre_kernel built with %d registers, %d needed",
+                        fa.numRegs, (kRegsPool + 383) / 384);
+        attr_done[d->ordinal & 63] = true;
+    }
+    paged_pre_kernel<T, D><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, mv, a);
+    return HEXCUDA_OK;
+}
+
+}  // namespace
+
+int launch_paged_pre(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                     PagedTc &a, int dtype, int dim) {
+    if (dtype == HEXCUDA_F16)
+        return dim == 128 ? launch_pre<__half, 128>(d, mq, mk, mv, a)
+                          : launch_pre<__half, 64>(d, mq, mk, mv, a);
+    return dim == 128 ? launch_pre<__nv_bfloat16, 128>(d, mq, mk, mv, a)
+                      : launch_pre<__nv_bfloat16, 64>(d, mq, mk, mv, a);
+}
+
+}  // namespace hx
