@@ -10,7 +10,7 @@
 // two additions then come in either order).
 #include <math.h>
 
-#include "paged.cuh"
+#include "paged_tc.cuh"
 
 namespace hx {
 namespace {
@@ -73,6 +73,13 @@ HX_EXPORT int hexcuda_cache_scores(int dev, int dtype, const void *q, const floa
     if (!d) return HEXCUDA_ERR_NODEV;
     PagedSeqs s{block_table, kv_lens, q_offs, batch, total_q, num_pages, page_size,
                 max_pages, causal, d->err_word};
+    if (paged_tc_fits(q, k_pages, nullptr, nullptr, heads, kv_heads, head_dim, num_pages, page_size)) {
+        launch_begin(d);
+        if (int rc = launch_scores_tc(d, s, dtype, q, lse, k_pages, scores, max_q, heads, kv_heads,
+                                      head_dim, scale))
+            return rc;
+        return launch_end(d, "cache_scores");
+    }
     launch_begin(d);
     const int tiles = (int)(((int64_t)max_pages * page_size + 127) / 128);
     const int64_t items = (int64_t)batch * kv_heads * tiles;

@@ -240,4 +240,9 @@ int launch_paged_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const
 int launch_paged_pre(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
                      PagedTc &a, int dtype, int dim);
 
+// The weights of cache_scores (scores_tc.cu), for what paged_tc_fits.
+int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const float *lse,
+                     const void *k, float *scores, int max_q, int heads, int kv_heads, int dim,
+                     float scale);
+
 }  // namespace hx

@@ -1,0 +1,533 @@
+// scores_tc.cu -- collected attention weight (cache_scores.cu) on the tensor
+// cores.
+//
+// A column sum of the softmax matrix is a row sum when the keys are on the M
+// side: S^T [128 keys x R rows] = K Q^T, one thread per key, which adds
+// 2^(scale*log2e * s - lse*log2e) over the columns.  The key tile stays in
+// shared memory while the query tiles that see it pass by, so a key's sum is
+// made by one CTA, in a fixed order, and added to the cache once.
+//
+// A work item is (sequence, key head, tile of 128 keys); it costs one unit per
+// query tile that sees it (R = 16 or 32 rows when a key head has that few,
+// else 128; tok = R / group tokens a tile).  Items go to the CTAs whole, in
+// order, CTA c taking those that start in units c T / C .. (c + 1) T / C - 1.
+//
+// Per CTA (one per SM), 384 threads: warp 0 TMA (page fragments of the key
+// tile, one lane each; query tiles), warp 1 tensor memory and MMA issue, warp 2
+// the rows' lse * log2e (plus infinity where a row counts for nothing), two
+// warpgroups that take the units in turn, four score tiles in tensor memory.
+// With few rows the kernel is bound by HBM (each key once); with many by the
+// exponentials, one per score.
+//
+// Every wait is bounded; see mbar_wait.
+#include <math.h>
+
+#include "paged_tc.cuh"
+
+namespace hx {
+namespace {
+
+struct ScoresTc {
+    PagedSeqs s;
+    int heads, kv_heads, group, tok, frag, map_rows;
+    float scale_log2;
+    const float *lse;
+    float *scores;
+};
+
+template <int D, int R>
+struct ScSmem {
+    static constexpr int kSubs = D / 64;
+    static constexpr int kTile = kSubs * kSubTile;
+    static constexpr int kKStages = (R == 128 ? 2 : 6) * (128 / D);
+    static constexpr int kQStages = 4;
+    static constexpr int kQTile = kSubs * R * 128;
+    static constexpr int kK = 0;
+    static constexpr int kQ = kK + kKStages * kTile;
+    static constexpr int kLse = kQ + kQStages * kQTile;      // [4][R]
+    static constexpr int kX = kLse + 4 * R * 4;              // [128]: one warpgroup's sums
+    static constexpr int kPlan = kX + 128 * 4;
+    static constexpr int kBar = kPlan + 512;
+    // q_full, q_empty, l_full, l_empty, s_full, s_empty [4], x_full, x_empty,
+    // drain, k_full, k_empty [stages]
+    static constexpr int kNumBars = 27 + 2 * kKStages;
+    static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
+};
+
+// The CTA's items in order.  Every role walks its own copy.
+struct KeyWalk {
+    int b, h, kt, first, q_len, kv_len;
+    long long pos, end;      // first unit of the item, end of the run
+
+    __device__ __forceinline__ int row_tiles(const ScoresTc &a) const {
+        return (q_len + a.tok - 1) / a.tok;
+    }
+    // the first query tile that sees a key of tile kt
+    __device__ __forceinline__ int first_tile(const ScoresTc &a) const {
+        if (!a.s.causal) return 0;
+        const int t = kt * kKeys - (kv_len - q_len);
+        return t > 0 ? t / a.tok : 0;
+    }
+    __device__ __forceinline__ int cost(const ScoresTc &a) const {
+        return row_tiles(a) - first_tile(a);
+    }
+    __device__ __forceinline__ bool next(const ScoresTc &a) {
+        pos += cost(a);
+        if (pos >= end) return false;
+        if (++kt * kKeys >= kv_len) {
+            kt = 0;
+            if (++h == a.kv_heads) {
+                h = 0;
+                do {
+                    if (++b >= a.s.batch) return false;
+                    quiet_seq(a.s, b, first, q_len, kv_len);
+                } while (q_len == 0 || kv_len == 0);
+            }
+        }
+        return true;
+    }
+};
+
+struct KeyPlan {
+    long long sums[12];
+    KeyWalk start;
+    int any;
+};
+static_assert(sizeof(KeyPlan) <= 512, "KeyPlan");
+
+// Units of one key head of a sequence, and of those the ones of its first
+// `plain` tiles, which every query tile sees.
+__device__ __forceinline__ long long head_units(const ScoresTc &a, KeyWalk &w, int &plain) {
+    plain = 0;
+    if (w.q_len == 0 || w.kv_len == 0) return 0;
+    const int tiles = (w.kv_len + kKeys - 1) / kKeys;
+    plain = tiles;
+    if (a.s.causal) {
+        const long long c = (long long)w.kv_len - w.q_len + a.tok;
+        plain = c <= 0 ? 0 : (int)min((long long)tiles, (c + kKeys - 1) / kKeys);
+    }
+    long long n = (long long)plain * w.row_tiles(a);
+    for (w.kt = plain; w.kt < tiles; w.kt++) n += w.cost(a);
+    return n;
+}
+
+// Whole block: this CTA's first item in sh.start; false when it has none.
+__device__ __forceinline__ bool plan_keys(const ScoresTc &a, KeyPlan &sh) {
+    constexpr int kThreads = 384;
+    const int per = (a.s.batch + kThreads - 1) / kThreads;
+    const int b0 = min(a.s.batch, (int)threadIdx.x * per), b1 = min(a.s.batch, b0 + per);
+    long long mine = 0;
+    KeyWalk w;
+    int plain;
+    for (int b = b0; b < b1; b++) {
+        w.q_len = seq_q_len(a.s, b, w.first);
+        w.kv_len = seq_kv_len(a.s, b);
+        mine += head_units(a, w, plain) * a.kv_heads;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) sh.sums[warp] = upto;
+    if (threadIdx.x == 0) sh.any = 0;
+    __syncthreads();
+    long long total = 0;
+    for (int i = 0; i < kThreads / 32; i++) {
+        if (i < warp) upto += sh.sums[i];
+        total += sh.sums[i];
+    }
+    const long long lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1LL) * total / gridDim.x;
+    if (lo < hi && upto - mine <= lo && lo < upto) {
+        long long at = lo - (upto - mine);
+        for (int b = b0; b < b1; b++) {
+            quiet_seq(a.s, b, w.first, w.q_len, w.kv_len);
+            const long long n = head_units(a, w, plain);
+            if (at >= n * a.kv_heads) {
+                at -= n * a.kv_heads;
+                continue;
+            }
+            w.b = b;
+            w.h = (int)(at / n);
+            at -= w.h * n;
+            const int rt = w.row_tiles(a);
+            if (at < (long long)plain * rt) {
+                w.kt = (int)(at / rt);
+                at -= (long long)w.kt * rt;
+            } else {
+                at -= (long long)plain * rt;
+                for (w.kt = plain; at >= w.cost(a); w.kt++) at -= w.cost(a);
+            }
+            w.pos = lo - at;
+            w.end = hi;
+            // an item that an earlier CTA's run cuts is that CTA's
+            sh.any = at == 0 || w.next(a);
+            sh.start = w;
+            break;
+        }
+    }
+    __syncthreads();
+    return sh.any != 0;
+}
+
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(384, 1)
+    scores_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const ScoresTc a) {
+    using L = ScSmem<D, R>;
+    constexpr int kSubs = L::kSubs, KS = L::kKStages, QS = L::kQStages;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *q_full = bars, *q_empty = bars + 4, *l_full = bars + 8, *l_empty = bars + 12;
+    uint64_t *s_full = bars + 16, *s_empty = bars + 20, *x_full = bars + 24, *x_empty = bars + 25;
+    uint64_t *drain = bars + 26, *k_full = bars + 27, *k_empty = k_full + KS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    KeyPlan &plan = *reinterpret_cast<KeyPlan *>(smem + L::kPlan);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err_word = a.s.err_word;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4; i++) {
+            tc::mbar_init(&q_full[i], 1);
+            tc::mbar_init(&q_empty[i], 1);
+            tc::mbar_init(&l_full[i], 1);
+            tc::mbar_init(&l_empty[i], 4);
+            tc::mbar_init(&s_full[i], 1);
+            tc::mbar_init(&s_empty[i], 4);
+        }
+        tc::mbar_init(x_full, 4);
+        tc::mbar_init(x_empty, 4);
+        tc::mbar_init(drain, 1);
+        for (int i = 0; i < KS; i++) {
+            tc::mbar_init(&k_full[i], 1);
+            tc::mbar_init(&k_empty[i], 1);
+        }
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+        tc::tma_prefetch_desc(&tmQ);
+        tc::tma_prefetch_desc(&tmK);
+    }
+    constexpr uint32_t kCols = 4 * R;
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, kCols);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    const bool any = plan_keys(a, plan);
+    tc::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (!any) {
+        // nothing to do but free the tensor memory
+    } else if (warp == 0) {
+        // --------------------------------------------------------------- TMA
+        KeyWalk w = plan.start;
+        int st = 0;
+        uint32_t ph = 0, u = 0, armed = 0, k_ph = 0;
+        bool ok = true;
+        auto key_row = [&](const KeyWalk &v) {
+            const int t = v.kt * kKeys + lane * a.frag;
+            if (lane * a.frag >= kKeys || t >= v.kv_len) return -1;
+            const int i = t / a.s.page_size;
+            const int page = seq_page(a.s, v.b, i);
+            return page < 0 ? a.map_rows
+                            : (page * a.kv_heads + v.h) * a.s.page_size + (t - i * a.s.page_size);
+        };
+        int row = key_row(w);
+        do {
+            const int count = frag_count(row);
+            ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0)
+                tc::mbar_arrive_expect_tx(&k_full[st], (uint32_t)(count * a.frag * 128 * kSubs));
+            __syncwarp();
+            if (row >= 0)
+                for (int c = 0; c < kSubs; c++)
+                    tc::tma_load_2d(smem + L::kK + st * L::kTile + c * kSubTile + lane * a.frag * 128,
+                                    &tmK, &k_full[st], c * 64, row);
+            __syncwarp();
+            armed |= 1u << st;
+            k_ph = (k_ph & ~(1u << st)) | (ph << st);
+            if (++st == KS) {
+                st = 0;
+                ph ^= 1;
+            }
+            const int h = w.h, first = w.first, t_end = w.row_tiles(a);
+            const int t_begin = w.first_tile(a);
+            const bool more = w.next(a);
+            row = more ? key_row(w) : -1;       // the next item's pages, while the queries pass
+            for (int t = t_begin; t < t_end; t++, u++) {
+                const int qs = u % QS;
+                ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
+                    for (int c = 0; c < kSubs; c++)
+                        tc::tma_load_3d(smem + L::kQ + qs * L::kQTile + c * R * 128, &tmQ, &q_full[qs],
+                                        c * 64, h * a.group, first + t * a.tok);
+                }
+            }
+            if (!ok || !more) break;
+        } while (true);
+        if (lane == 0) {
+            // drain our own loads (a no-op when every load was consumed)
+            const uint64_t t0 = tc::globaltimer();
+            auto drain_wait = [&](uint64_t *bar, uint32_t par) {
+                while (!tc::mbar_try_wait(bar, par) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            };
+            for (uint32_t i = u > QS ? u - QS : 0; i < u; i++) drain_wait(&q_full[i % QS], (i / QS) & 1);
+            for (int i = 0; i < KS; i++)
+                if (armed >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ----------------------------------------------------------- MMA
+            constexpr uint32_t idesc = tc::idesc_f16_f32(kKeys, R, false, false, kBf16);
+            const uint32_t sK = tc::smem_u32(smem + L::kK), sQ = tc::smem_u32(smem + L::kQ);
+            KeyWalk w = plan.start;
+            int st = 0;
+            uint32_t ph = 0, u = 0;
+            bool ok = true;
+            do {
+                ok = tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                const int n = w.cost(a);
+                for (int t = 0; t < n && ok; t++, u++) {
+                    const int qs = u % QS;
+                    ok = tc::mbar_wait(&q_full[qs], (u / QS) & 1, abort_flag, err_word, kErrWaitFull) &&
+                         tc::mbar_wait(&s_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word,
+                                       kErrWaitAccum);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t kb = sK + st * L::kTile, qb = sQ + qs * L::kQTile;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++)
+                        tc::mma_ss<tc::MmaKind::F16>(
+                            tmem_base + (u & 3) * R,
+                            tc::sdesc_kmajor_sw128(kb + (k >> 2) * kSubTile + (k & 3) * 32),
+                            tc::sdesc_kmajor_sw128(qb + (k >> 2) * (R * 128) + (k & 3) * 32), idesc,
+                            k > 0 ? 1u : 0u);
+                    tc::mma_commit(&q_empty[qs]);
+                    tc::mma_commit(&s_full[u & 3]);
+                }
+                if (!ok) break;
+                tc::mma_commit(&k_empty[st]);
+                if (++st == KS) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            } while (w.next(a));
+            if (u > 0) {
+                tc::mma_commit(drain);
+                const uint64_t t0 = tc::globaltimer();
+                while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
+            }
+        }
+    } else if (warp == 2) {
+        // ------------------------------------------------- the rows' lse * log2e
+        KeyWalk w = plan.start;
+        float *sl = reinterpret_cast<float *>(smem + L::kLse);
+        uint32_t u = 0;
+        bool ok = true;
+        do {
+            const int t_end = w.row_tiles(a);
+            for (int t = w.first_tile(a); t < t_end && ok; t++, u++) {
+                const int nrows = min(a.tok, w.q_len - t * a.tok) * a.group;
+                float z[(R + 31) / 32];
+#pragma unroll
+                for (int i = 0; i < (R + 31) / 32; i++) {
+                    const int n = lane + 32 * i;
+                    z[i] = INFINITY;
+                    if (n < nrows) {
+                        const int64_t at = (int64_t)(w.first + t * a.tok + n / a.group) * a.heads +
+                                           w.h * a.group + n % a.group;
+                        const float v = a.lse[at];
+                        if (v != -INFINITY) z[i] = v * 1.4426950408889634f;
+                    }
+                }
+                ok = tc::mbar_wait(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < (R + 31) / 32; i++)
+                    if (lane + 32 * i < R) sl[(u & 3) * R + lane + 32 * i] = z[i];
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&l_full[u & 3]);
+            }
+        } while (ok && w.next(a));
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------- weights
+        const int wg = (warp - 4) >> 2, key = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const float *sl = reinterpret_cast<const float *>(smem + L::kLse);
+        float *xs = reinterpret_cast<float *>(smem + L::kX);
+        KeyWalk w = plan.start;
+        uint32_t u = 0, shared_items = 0;
+        bool ok = true;
+        do {
+            const int t_begin = w.first_tile(a), t_end = w.row_tiles(a), n = t_end - t_begin;
+            const int kk = w.kt * kKeys + key;
+            const int before = a.s.causal ? kk - (w.kv_len - w.q_len) : 0;   // tokens that do not see kk
+            float sum = 0.0f;
+            for (int t = t_begin; t < t_end && ok; t++, u++) {
+                if ((int)(u & 1) != wg) continue;
+                const int buf = u & 3;
+                ok = tc::mbar_wait(&s_full[buf], (u >> 2) & 1, abort_flag, err_word, kErrWaitAccum) &&
+                     tc::mbar_wait(&l_full[buf], (u >> 2) & 1, abort_flag, err_word, kErrWaitFull);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::tc_fence_after();
+                // rows lo <= n < hi of the tile count for this key
+                const int hi = min(a.tok, w.q_len - t * a.tok) * a.group;
+                const int lo = max(0, min(a.tok, before - t * a.tok)) * a.group;
+                const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < R);
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                auto add = [&](const auto &r, int c0, int count) {
+#pragma unroll
+                    for (int e = 0; e < count; e += 4) {
+                        const float4 z = *reinterpret_cast<const float4 *>(sl + buf * R + c0 + e);
+                        float p[4];
+                        p[0] = tc::ex2(fmaf(__uint_as_float(r[e]), a.scale_log2, -z.x));
+                        p[1] = tc::ex2(fmaf(__uint_as_float(r[e + 1]), a.scale_log2, -z.y));
+                        p[2] = tc::ex2(fmaf(__uint_as_float(r[e + 2]), a.scale_log2, -z.z));
+                        p[3] = tc::ex2(fmaf(__uint_as_float(r[e + 3]), a.scale_log2, -z.w));
+                        if (cut) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (c0 + e + i < lo || c0 + e + i >= hi) p[i] = 0.0f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[i] += p[i];
+                    }
+                };
+                const uint32_t s_addr = tmem_base + lane_base + buf * R;
+                if constexpr (R == 16) {
+                    uint32_t r[16];
+                    tc::tmem_ld_32x32b_x16(s_addr, r);
+                    tc::tmem_ld_wait(r);
+                    add(r, 0, 16);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < R; c += 64) {
+                        uint32_t r0[32], r1[32];
+                        tc::tmem_ld_32x32b_x32(s_addr + c, r0);
+                        if (R > 32) tc::tmem_ld_32x32b_x32(s_addr + c + 32, r1);
+                        tc::tmem_ld_wait(r0);
+                        if (R > 32) tc::reg_fence(r1);
+                        add(r0, c, 32);
+                        if (R > 32) add(r1, c + 32, 32);
+                    }
+                }
+                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(&s_empty[buf]);
+                    tc::mbar_arrive(&l_empty[buf]);
+                }
+            }
+            if (!ok) break;
+            // an item of several units: the warpgroup without the last one
+            // hands its sums to the other
+            const bool owner = (int)((u - 1) & 1) == wg;
+            if (n > 1) {
+                if (!owner) {
+                    ok = tc::mbar_wait(x_empty, (shared_items & 1) ^ 1, abort_flag, err_word, kErrWaitOther);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    xs[key] = sum;
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(x_full);
+                } else {
+                    ok = tc::mbar_wait(x_full, shared_items & 1, abort_flag, err_word, kErrWaitOther);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    sum += xs[key];
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(x_empty);
+                }
+                shared_items++;
+            }
+            if (owner && kk < w.kv_len) {
+                const int i = kk / a.s.page_size;
+                const int page = a.s.table[(int64_t)w.b * a.s.max_pages + i];
+                if (page >= 0 && page < a.s.num_pages)
+                    atomicAdd(&a.scores[((int64_t)page * a.kv_heads + w.h) * a.s.page_size + kk -
+                                        i * a.s.page_size],
+                              sum);
+            }
+        } while (w.next(a));
+    }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tc::tmem_dealloc(tmem_base, kCols);
+    }
+}
+
+template <typename T, int D, int R>
+int launch(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a) {
+    using L = ScSmem<D, R>;
+    static_assert(L::kTotal <= 232448, "shared memory of one CTA");
+    static bool attr_done[64] = {};
+    if (!attr_done[d->ordinal & 63]) {
+        if (int rc = check(cudaFuncSetAttribute(scores_tc_kernel<T, D, R>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                L::kTotal),
+                           "cudaFuncSetAttribute(scores_tc)"))
+            return rc;
+        attr_done[d->ordinal & 63] = true;
+    }
+    scores_tc_kernel<T, D, R><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, a);
+    return HEXCUDA_OK;
+}
+
+template <typename T, int D>
+int launch_rows(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a, int rows) {
+    if (rows == 16) return launch<T, D, 16>(d, mq, mk, a);
+    if (rows == 32) return launch<T, D, 32>(d, mq, mk, a);
+    return launch<T, D, 128>(d, mq, mk, a);
+}
+
+}  // namespace
+
+int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const float *lse,
+                     const void *k, float *scores, int max_q, int heads, int kv_heads, int dim,
+                     float scale) {
+    ScoresTc a;
+    a.s = s;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.group = heads / kv_heads;
+    const int64_t need = (int64_t)(max_q < 1 ? 1 : max_q) * a.group;
+    const int rows = need <= 16 ? 16 : need <= 32 ? 32 : 128;
+    a.tok = rows / a.group;
+    const int low = s.page_size & -s.page_size;
+    a.frag = low < kKeys ? low : kKeys;
+    a.map_rows = s.num_pages * kv_heads * s.page_size;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.lse = lse;
+    a.scores = scores;
+    CUtensorMap mq, mk;
+    if (int rc = make_query_map(&mq, q, s.total_q, heads, dim, a.group, a.tok)) return rc;
+    if (int rc = make_page_map(&mk, k, a.map_rows, dim, a.frag)) return rc;
+    note_mech(kMechTcgen05 | kMechTma);
+    if (dtype == HEXCUDA_F16)
+        return dim == 128 ? launch_rows<__half, 128>(d, mq, mk, a, rows)
+                          : launch_rows<__half, 64>(d, mq, mk, a, rows);
+    return dim == 128 ? launch_rows<__nv_bfloat16, 128>(d, mq, mk, a, rows)
+                      : launch_rows<__nv_bfloat16, 64>(d, mq, mk, a, rows);
+}
+
+}  // namespace hx
