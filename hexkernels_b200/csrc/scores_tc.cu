@@ -7,17 +7,19 @@
 // shared memory while the query tiles that see it pass by, so a key's sum is
 // made by one CTA, in a fixed order, and added to the cache once.
 //
-// A work item is (sequence, key head, tile of 128 keys); it costs one unit per
-// query tile that sees it (R = 16 or 32 rows when a key head has that few,
-// else 128; tok = R / group tokens a tile).  Items go to the CTAs whole, in
-// order, CTA c taking those that start in units c T / C .. (c + 1) T / C - 1.
+// A work item is (sequence, key head, 256 keys); it costs one unit per query
+// tile that sees it (R = 16 or 32 rows when a key head has that few, else 128;
+// tok = R / group tokens a tile).  Items go to the CTAs whole, in order, CTA c
+// taking those that start in units c T / C .. (c + 1) T / C - 1.
 //
-// Per CTA (one per SM), 384 threads: warp 0 TMA (page fragments of the key
-// tile, one lane each; query tiles), warp 1 tensor memory and MMA issue, warp 2
-// the rows' lse * log2e (plus infinity where a row counts for nothing), two
-// warpgroups that take the units in turn, four score tiles in tensor memory.
-// With few rows the kernel is bound by HBM (each key once); with many by the
-// exponentials, one per score.
+// Per CTA (one per SM), 384 threads: warp 0 TMA of key tiles (page fragments,
+// one lane each), warp 3 TMA of query tiles, warp 1 tensor memory and MMA
+// issue, warp 2 the rows' lse * log2e (plus infinity where a row counts for
+// nothing), then a warpgroup for each half of the keys, each with two score
+// tiles in tensor memory.  256 keys to a query tile, because the query tiles
+// come from L2 again and again: with 128 keys they asked for more than L2
+// gives.  With few rows the kernel is bound by HBM (each key once); with many
+// by the exponentials, one per score.
 //
 // Every wait is bounded; see mbar_wait.
 #include <math.h>
@@ -38,21 +40,22 @@ struct ScoresTc {
 template <int D, int R>
 struct ScSmem {
     static constexpr int kSubs = D / 64;
-    static constexpr int kTile = kSubs * kSubTile;
-    static constexpr int kKStages = (R == 128 ? 2 : 6) * (128 / D);
-    static constexpr int kQStages = 4;
+    static constexpr int kTile = kSubs * kSubTile;           // 128 keys
+    static constexpr int kKStages = (R == 128 ? 2 : 3) * (128 / D);
+    static constexpr int kQStages = R == 16 ? 4 : 2;
     static constexpr int kQTile = kSubs * R * 128;
     static constexpr int kK = 0;
-    static constexpr int kQ = kK + kKStages * kTile;
+    static constexpr int kQ = kK + kKStages * 2 * kTile;
     static constexpr int kLse = kQ + kQStages * kQTile;      // [4][R]
-    static constexpr int kX = kLse + 4 * R * 4;              // [128]: one warpgroup's sums
-    static constexpr int kPlan = kX + 128 * 4;
+    static constexpr int kPlan = kLse + 4 * R * 4;
     static constexpr int kBar = kPlan + 512;
-    // q_full, q_empty, l_full, l_empty, s_full, s_empty [4], x_full, x_empty,
-    // drain, k_full, k_empty [stages]
-    static constexpr int kNumBars = 27 + 2 * kKStages;
+    // l_full, l_empty [4], s_full, s_empty [half][2], drain, q_full, q_empty,
+    // k_full, k_empty [stages]
+    static constexpr int kNumBars = 17 + 2 * kQStages + 2 * kKStages;
     static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
 };
+
+constexpr int kItemKeys = 2 * kKeys;
 
 // The CTA's items in order.  Every role walks its own copy.
 struct KeyWalk {
@@ -62,19 +65,23 @@ struct KeyWalk {
     __device__ __forceinline__ int row_tiles(const ScoresTc &a) const {
         return (q_len + a.tok - 1) / a.tok;
     }
-    // the first query tile that sees a key of tile kt
-    __device__ __forceinline__ int first_tile(const ScoresTc &a) const {
+    // the first query tile that sees a key of the item's half x
+    __device__ __forceinline__ int first_tile(const ScoresTc &a, int x) const {
         if (!a.s.causal) return 0;
-        const int t = kt * kKeys - (kv_len - q_len);
+        const int t = kt * kItemKeys + x * kKeys - (kv_len - q_len);
         return t > 0 ? t / a.tok : 0;
     }
+    // the same for half 1, or behind the last when no key lies in it
+    __device__ __forceinline__ int first_tile_1(const ScoresTc &a) const {
+        return kt * kItemKeys + kKeys < kv_len ? first_tile(a, 1) : row_tiles(a);
+    }
     __device__ __forceinline__ int cost(const ScoresTc &a) const {
-        return row_tiles(a) - first_tile(a);
+        return row_tiles(a) - first_tile(a, 0);
     }
     __device__ __forceinline__ bool next(const ScoresTc &a) {
         pos += cost(a);
         if (pos >= end) return false;
-        if (++kt * kKeys >= kv_len) {
+        if (++kt * kItemKeys >= kv_len) {
             kt = 0;
             if (++h == a.kv_heads) {
                 h = 0;
@@ -100,11 +107,11 @@ static_assert(sizeof(KeyPlan) <= 512, "KeyPlan");
 __device__ __forceinline__ long long head_units(const ScoresTc &a, KeyWalk &w, int &plain) {
     plain = 0;
     if (w.q_len == 0 || w.kv_len == 0) return 0;
-    const int tiles = (w.kv_len + kKeys - 1) / kKeys;
+    const int tiles = (w.kv_len + kItemKeys - 1) / kItemKeys;
     plain = tiles;
     if (a.s.causal) {
         const long long c = (long long)w.kv_len - w.q_len + a.tok;
-        plain = c <= 0 ? 0 : (int)min((long long)tiles, (c + kKeys - 1) / kKeys);
+        plain = c <= 0 ? 0 : (int)min((long long)tiles, (c + kItemKeys - 1) / kItemKeys);
     }
     long long n = (long long)plain * w.row_tiles(a);
     for (w.kt = plain; w.kt < tiles; w.kt++) n += w.cost(a);
@@ -171,6 +178,49 @@ __device__ __forceinline__ bool plan_keys(const ScoresTc &a, KeyPlan &sh) {
     return sh.any != 0;
 }
 
+// Sum over the rows lo <= r < hi of one score tile (this lane's key) of
+// 2^(s * scale_log2 - z[r]); CUT: some lane's rows are not all R.
+template <int R, bool CUT>
+__device__ __forceinline__ float add_weights(uint32_t s_addr, const float *z, float scale_log2, int lo,
+                                             int hi, float (&acc)[4]) {
+    auto add = [&](const auto &r, int c0, auto count) {
+#pragma unroll
+        for (int e = 0; e < decltype(count)::value; e += 4) {
+            const float4 zz = *reinterpret_cast<const float4 *>(z + c0 + e);
+            const float zv[4] = {zz.x, zz.y, zz.z, zz.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float p = tc::ex2(fmaf(__uint_as_float(r[e + i]), scale_log2, -zv[i]));
+                if (CUT && (c0 + e + i < lo || c0 + e + i >= hi)) p = 0.0f;
+                acc[i] += p;
+            }
+        }
+    };
+    if constexpr (R == 16) {
+        uint32_t r[16];
+        tc::tmem_ld_32x32b_x16(s_addr, r);
+        tc::tmem_ld_wait(r);
+        add(r, 0, std::integral_constant<int, 16>());
+    } else if constexpr (R == 32) {
+        uint32_t r[32];
+        tc::tmem_ld_32x32b_x32(s_addr, r);
+        tc::tmem_ld_wait(r);
+        add(r, 0, std::integral_constant<int, 32>());
+    } else {
+#pragma unroll
+        for (int c = 0; c < R; c += 64) {
+            uint32_t r0[32], r1[32];
+            tc::tmem_ld_32x32b_x32(s_addr + c, r0);
+            tc::tmem_ld_32x32b_x32(s_addr + c + 32, r1);
+            tc::tmem_ld_wait(r0);
+            tc::reg_fence(r1);
+            add(r0, c, std::integral_constant<int, 32>());
+            add(r1, c + 32, std::integral_constant<int, 32>());
+        }
+    }
+    return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(384, 1)
     scores_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -182,9 +232,9 @@ __global__ void __launch_bounds__(384, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *q_full = bars, *q_empty = bars + 4, *l_full = bars + 8, *l_empty = bars + 12;
-    uint64_t *s_full = bars + 16, *s_empty = bars + 20, *x_full = bars + 24, *x_empty = bars + 25;
-    uint64_t *drain = bars + 26, *k_full = bars + 27, *k_empty = k_full + KS;
+    uint64_t *l_full = bars, *l_empty = bars + 4, *s_full = bars + 8, *s_empty = bars + 12;
+    uint64_t *drain = bars + 16, *q_full = bars + 17, *q_empty = q_full + QS;
+    uint64_t *k_full = q_empty + QS, *k_empty = k_full + KS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     KeyPlan &plan = *reinterpret_cast<KeyPlan *>(smem + L::kPlan);
@@ -193,16 +243,16 @@ __global__ void __launch_bounds__(384, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; i++) {
-            tc::mbar_init(&q_full[i], 1);
-            tc::mbar_init(&q_empty[i], 1);
             tc::mbar_init(&l_full[i], 1);
-            tc::mbar_init(&l_empty[i], 4);
+            tc::mbar_init(&l_empty[i], 8);
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&s_empty[i], 4);
         }
-        tc::mbar_init(x_full, 4);
-        tc::mbar_init(x_empty, 4);
         tc::mbar_init(drain, 1);
+        for (int i = 0; i < QS; i++) {
+            tc::mbar_init(&q_full[i], 1);
+            tc::mbar_init(&q_empty[i], 1);
+        }
         for (int i = 0; i < KS; i++) {
             tc::mbar_init(&k_full[i], 1);
             tc::mbar_init(&k_empty[i], 1);
@@ -225,32 +275,50 @@ __global__ void __launch_bounds__(384, 1)
     if (!any) {
         // nothing to do but free the tensor memory
     } else if (warp == 0) {
-        // --------------------------------------------------------------- TMA
+        // ---------------------------------------------------------- TMA, keys
         KeyWalk w = plan.start;
         int st = 0;
-        uint32_t ph = 0, u = 0, armed = 0, k_ph = 0;
+        uint32_t ph = 0, armed = 0, k_ph = 0;
         bool ok = true;
-        auto key_row = [&](const KeyWalk &v) {
-            const int t = v.kt * kKeys + lane * a.frag;
-            if (lane * a.frag >= kKeys || t >= v.kv_len) return -1;
-            const int i = t / a.s.page_size;
-            const int page = seq_page(a.s, v.b, i);
-            return page < 0 ? a.map_rows
-                            : (page * a.kv_heads + v.h) * a.s.page_size + (t - i * a.s.page_size);
+        // lane's fragment of an item: its first token and, as the table has
+        // it, its page; the load is not waited for until the item's turn
+        const int span = lane * a.frag;
+        auto token = [&](const KeyWalk &v) {
+            const int t = v.kt * kItemKeys + span;
+            return span < kItemKeys && t < v.kv_len ? t : -1;
         };
-        int row = key_row(w);
+        auto page_of = [&](const KeyWalk &v, int t) {
+            return t < 0 ? -1 : a.s.table[(int64_t)v.b * a.s.max_pages + t / a.s.page_size];
+        };
+        int tok = token(w), page = page_of(w, tok);
+        bool more;
         do {
-            const int count = frag_count(row);
+            const int t = tok, p = page, h = w.h;
+            more = w.next(a);
+            if (more) {
+                tok = token(w);
+                page = page_of(w, tok);
+            }
             ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            int row = -1;
+            if (t >= 0) {
+                row = a.map_rows;
+                if (p >= 0 && p < a.s.num_pages)
+                    row = (p * a.kv_heads + h) * a.s.page_size + t % a.s.page_size;
+                else
+                    flag_index(err_word);
+            }
+            const int count = frag_count(row);
             if (lane == 0)
                 tc::mbar_arrive_expect_tx(&k_full[st], (uint32_t)(count * a.frag * 128 * kSubs));
             __syncwarp();
-            if (row >= 0)
+            if (row >= 0) {
+                uint8_t *dst = smem + L::kK + (st * 2 + span / kKeys) * L::kTile + span % kKeys * 128;
                 for (int c = 0; c < kSubs; c++)
-                    tc::tma_load_2d(smem + L::kK + st * L::kTile + c * kSubTile + lane * a.frag * 128,
-                                    &tmK, &k_full[st], c * 64, row);
+                    tc::tma_load_2d(dst + c * kSubTile, &tmK, &k_full[st], c * 64, row);
+            }
             __syncwarp();
             armed |= 1u << st;
             k_ph = (k_ph & ~(1u << st)) | (ph << st);
@@ -258,34 +326,40 @@ __global__ void __launch_bounds__(384, 1)
                 st = 0;
                 ph ^= 1;
             }
-            const int h = w.h, first = w.first, t_end = w.row_tiles(a);
-            const int t_begin = w.first_tile(a);
-            const bool more = w.next(a);
-            row = more ? key_row(w) : -1;       // the next item's pages, while the queries pass
-            for (int t = t_begin; t < t_end; t++, u++) {
-                const int qs = u % QS;
-                ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) {
-                    tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
-                    for (int c = 0; c < kSubs; c++)
-                        tc::tma_load_3d(smem + L::kQ + qs * L::kQTile + c * R * 128, &tmQ, &q_full[qs],
-                                        c * 64, h * a.group, first + t * a.tok);
-                }
-            }
-            if (!ok || !more) break;
-        } while (true);
+        } while (more);
         if (lane == 0) {
             // drain our own loads (a no-op when every load was consumed)
             const uint64_t t0 = tc::globaltimer();
-            auto drain_wait = [&](uint64_t *bar, uint32_t par) {
-                while (!tc::mbar_try_wait(bar, par) && tc::globaltimer() - t0 < kWaitBudgetNs) {
-                }
-            };
-            for (uint32_t i = u > QS ? u - QS : 0; i < u; i++) drain_wait(&q_full[i % QS], (i / QS) & 1);
             for (int i = 0; i < KS; i++)
-                if (armed >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
+                if (armed >> i & 1)
+                    while (!tc::mbar_try_wait(&k_full[i], k_ph >> i & 1) &&
+                           tc::globaltimer() - t0 < kWaitBudgetNs) {
+                    }
+        }
+    } else if (warp == 3) {
+        // ------------------------------------------------------- TMA, queries
+        if (lane == 0) {
+            KeyWalk w = plan.start;
+            uint32_t u = 0;
+            bool ok = true;
+            do {
+                const int t_end = w.row_tiles(a);
+                for (int t = w.first_tile(a, 0); t < t_end; t++, u++) {
+                    const int qs = u % QS;
+                    ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word,
+                                       kErrWaitEmpty);
+                    if (!ok) break;
+                    tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
+                    for (int c = 0; c < kSubs; c++)
+                        tc::tma_load_3d(smem + L::kQ + qs * L::kQTile + c * R * 128, &tmQ, &q_full[qs],
+                                        c * 64, w.h * a.group, w.first + t * a.tok);
+                }
+            } while (ok && w.next(a));
+            const uint64_t t0 = tc::globaltimer();
+            for (uint32_t i = u > QS ? u - QS : 0; i < u; i++)
+                while (!tc::mbar_try_wait(&q_full[i % QS], (i / QS) & 1) &&
+                       tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -294,28 +368,34 @@ __global__ void __launch_bounds__(384, 1)
             const uint32_t sK = tc::smem_u32(smem + L::kK), sQ = tc::smem_u32(smem + L::kQ);
             KeyWalk w = plan.start;
             int st = 0;
-            uint32_t ph = 0, u = 0;
+            uint32_t ph = 0, u = 0, n[2] = {0, 0};       // units; score tiles of each half
             bool ok = true;
             do {
                 ok = tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
-                const int n = w.cost(a);
-                for (int t = 0; t < n && ok; t++, u++) {
+                const int t_end = w.row_tiles(a), t1 = w.first_tile_1(a);
+                for (int t = w.first_tile(a, 0); t < t_end && ok; t++, u++) {
                     const int qs = u % QS;
-                    ok = tc::mbar_wait(&q_full[qs], (u / QS) & 1, abort_flag, err_word, kErrWaitFull) &&
-                         tc::mbar_wait(&s_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word,
-                                       kErrWaitAccum);
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    const uint32_t kb = sK + st * L::kTile, qb = sQ + qs * L::kQTile;
+                    ok = tc::mbar_wait(&q_full[qs], (u / QS) & 1, abort_flag, err_word, kErrWaitFull);
+                    const uint32_t qb = sQ + qs * L::kQTile;
+                    for (int x = 0; x < 2 && ok; x++) {
+                        if (x == 1 && t < t1) continue;
+                        const int buf = x * 2 + (n[x] & 1);
+                        ok = tc::mbar_wait(&s_empty[buf], ((n[x] >> 1) & 1) ^ 1, abort_flag, err_word,
+                                           kErrWaitAccum);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        const uint32_t kb = sK + (st * 2 + x) * L::kTile;
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++)
-                        tc::mma_ss<tc::MmaKind::F16>(
-                            tmem_base + (u & 3) * R,
-                            tc::sdesc_kmajor_sw128(kb + (k >> 2) * kSubTile + (k & 3) * 32),
-                            tc::sdesc_kmajor_sw128(qb + (k >> 2) * (R * 128) + (k & 3) * 32), idesc,
-                            k > 0 ? 1u : 0u);
-                    tc::mma_commit(&q_empty[qs]);
-                    tc::mma_commit(&s_full[u & 3]);
+                        for (int k = 0; k < D / 16; k++)
+                            tc::mma_ss<tc::MmaKind::F16>(
+                                tmem_base + buf * R,
+                                tc::sdesc_kmajor_sw128(kb + (k >> 2) * kSubTile + (k & 3) * 32),
+                                tc::sdesc_kmajor_sw128(qb + (k >> 2) * (R * 128) + (k & 3) * 32),
+                                idesc, k > 0 ? 1u : 0u);
+                        tc::mma_commit(&s_full[buf]);
+                        n[x]++;
+                    }
+                    if (ok) tc::mma_commit(&q_empty[qs]);
                 }
                 if (!ok) break;
                 tc::mma_commit(&k_empty[st]);
@@ -324,7 +404,7 @@ __global__ void __launch_bounds__(384, 1)
                     ph ^= 1;
                 }
             } while (w.next(a));
-            if (u > 0) {
+            if (n[0] > 0) {
                 tc::mma_commit(drain);
                 const uint64_t t0 = tc::globaltimer();
                 while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
@@ -333,130 +413,94 @@ __global__ void __launch_bounds__(384, 1)
         }
     } else if (warp == 2) {
         // ------------------------------------------------- the rows' lse * log2e
+        constexpr int kPer = (R + 31) / 32;
         KeyWalk w = plan.start;
         float *sl = reinterpret_cast<float *>(smem + L::kLse);
         uint32_t u = 0;
+        // lane's rows of a tile: token and head
+        int row_tok[kPer], row_at[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            row_tok[i] = (lane + 32 * i) / a.group;
+            row_at[i] = row_tok[i] * a.heads + (lane + 32 * i) % a.group;
+            if (lane + 32 * i >= a.tok * a.group) row_tok[i] = 0x7fffffff;   // no row
+        }
+        auto load = [&](int t, float (&z)[kPer]) {
+            const float *base = a.lse + ((int64_t)(w.first + t * a.tok) * a.heads + w.h * a.group);
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                z[i] = row_tok[i] < w.q_len - t * a.tok ? base[row_at[i]] : -INFINITY;
+        };
+        float z[kPer], zn[kPer];
+        int t = w.first_tile(a, 0);
+        load(t, z);
+        bool more = true;
+        while (more) {
+            // the next unit's values, while this one's place is waited for
+            if (++t >= w.row_tiles(a)) {
+                more = w.next(a);
+                if (more) t = w.first_tile(a, 0);
+            }
+            if (more) load(t, zn);
+            bool ok = tc::mbar_wait(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+                if (lane + 32 * i < R)
+                    sl[(u & 3) * R + lane + 32 * i] =
+                        z[i] == -INFINITY ? INFINITY : z[i] * 1.4426950408889634f;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&l_full[u & 3]);
+            u++;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) z[i] = zn[i];
+        }
+    } else {
+        // ------------------------------------------------------------- weights
+        const int x = (warp - 4) >> 2, key = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const float *sl = reinterpret_cast<const float *>(smem + L::kLse);
+        KeyWalk w = plan.start;
+        uint32_t u = 0, n = 0;
         bool ok = true;
         do {
             const int t_end = w.row_tiles(a);
-            for (int t = w.first_tile(a); t < t_end && ok; t++, u++) {
-                const int nrows = min(a.tok, w.q_len - t * a.tok) * a.group;
-                float z[(R + 31) / 32];
-#pragma unroll
-                for (int i = 0; i < (R + 31) / 32; i++) {
-                    const int n = lane + 32 * i;
-                    z[i] = INFINITY;
-                    if (n < nrows) {
-                        const int64_t at = (int64_t)(w.first + t * a.tok + n / a.group) * a.heads +
-                                           w.h * a.group + n % a.group;
-                        const float v = a.lse[at];
-                        if (v != -INFINITY) z[i] = v * 1.4426950408889634f;
-                    }
-                }
-                ok = tc::mbar_wait(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < (R + 31) / 32; i++)
-                    if (lane + 32 * i < R) sl[(u & 3) * R + lane + 32 * i] = z[i];
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&l_full[u & 3]);
-            }
-        } while (ok && w.next(a));
-    } else if (warp >= 4) {
-        // ------------------------------------------------------------- weights
-        const int wg = (warp - 4) >> 2, key = (warp & 3) * 32 + lane;
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const float *sl = reinterpret_cast<const float *>(smem + L::kLse);
-        float *xs = reinterpret_cast<float *>(smem + L::kX);
-        KeyWalk w = plan.start;
-        uint32_t u = 0, shared_items = 0;
-        bool ok = true;
-        do {
-            const int t_begin = w.first_tile(a), t_end = w.row_tiles(a), n = t_end - t_begin;
-            const int kk = w.kt * kKeys + key;
+            const int t_mine = x == 0 ? w.first_tile(a, 0) : w.first_tile_1(a);
+            const int kk = w.kt * kItemKeys + x * kKeys + key;
             const int before = a.s.causal ? kk - (w.kv_len - w.q_len) : 0;   // tokens that do not see kk
             float sum = 0.0f;
-            for (int t = t_begin; t < t_end && ok; t++, u++) {
-                if ((int)(u & 1) != wg) continue;
-                const int buf = u & 3;
-                ok = tc::mbar_wait(&s_full[buf], (u >> 2) & 1, abort_flag, err_word, kErrWaitAccum) &&
-                     tc::mbar_wait(&l_full[buf], (u >> 2) & 1, abort_flag, err_word, kErrWaitFull);
+            for (int t = w.first_tile(a, 0); t < t_end; t++, u++) {
+                const int lb = u & 3;
+                // (also a half that skips the unit waits for its lse values: it
+                // must not hand back a place that is not filled yet)
+                ok = tc::mbar_wait(&l_full[lb], (u >> 2) & 1, abort_flag, err_word, kErrWaitFull);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                tc::tc_fence_after();
-                // rows lo <= n < hi of the tile count for this key
-                const int hi = min(a.tok, w.q_len - t * a.tok) * a.group;
-                const int lo = max(0, min(a.tok, before - t * a.tok)) * a.group;
-                const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < R);
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                auto add = [&](const auto &r, int c0, int count) {
-#pragma unroll
-                    for (int e = 0; e < count; e += 4) {
-                        const float4 z = *reinterpret_cast<const float4 *>(sl + buf * R + c0 + e);
-                        float p[4];
-                        p[0] = tc::ex2(fmaf(__uint_as_float(r[e]), a.scale_log2, -z.x));
-                        p[1] = tc::ex2(fmaf(__uint_as_float(r[e + 1]), a.scale_log2, -z.y));
-                        p[2] = tc::ex2(fmaf(__uint_as_float(r[e + 2]), a.scale_log2, -z.z));
-                        p[3] = tc::ex2(fmaf(__uint_as_float(r[e + 3]), a.scale_log2, -z.w));
-                        if (cut) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (c0 + e + i < lo || c0 + e + i >= hi) p[i] = 0.0f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[i] += p[i];
-                    }
-                };
-                const uint32_t s_addr = tmem_base + lane_base + buf * R;
-                if constexpr (R == 16) {
-                    uint32_t r[16];
-                    tc::tmem_ld_32x32b_x16(s_addr, r);
-                    tc::tmem_ld_wait(r);
-                    add(r, 0, 16);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < R; c += 64) {
-                        uint32_t r0[32], r1[32];
-                        tc::tmem_ld_32x32b_x32(s_addr + c, r0);
-                        if (R > 32) tc::tmem_ld_32x32b_x32(s_addr + c + 32, r1);
-                        tc::tmem_ld_wait(r0);
-                        if (R > 32) tc::reg_fence(r1);
-                        add(r0, c, 32);
-                        if (R > 32) add(r1, c + 32, 32);
-                    }
+                if (t >= t_mine) {
+                    const int buf = x * 2 + (n & 1);
+                    ok = tc::mbar_wait(&s_full[buf], (n >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    // rows lo <= r < hi of the tile count for this key
+                    const int hi = min(a.tok, w.q_len - t * a.tok) * a.group;
+                    const int lo = max(0, min(a.tok, before - t * a.tok)) * a.group;
+                    const uint32_t s_addr = tmem_base + lane_base + buf * R;
+                    const float *zl = sl + lb * R;
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (__any_sync(0xffffffffu, lo > 0 || hi < R))
+                        sum += add_weights<R, true>(s_addr, zl, a.scale_log2, lo, hi, acc);
+                    else
+                        sum += add_weights<R, false>(s_addr, zl, a.scale_log2, 0, R, acc);
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s_empty[buf]);
+                    n++;
                 }
-                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    tc::mbar_arrive(&s_empty[buf]);
-                    tc::mbar_arrive(&l_empty[buf]);
-                }
+                if (lane == 0) tc::mbar_arrive(&l_empty[lb]);
             }
             if (!ok) break;
-            // an item of several units: the warpgroup without the last one
-            // hands its sums to the other
-            const bool owner = (int)((u - 1) & 1) == wg;
-            if (n > 1) {
-                if (!owner) {
-                    ok = tc::mbar_wait(x_empty, (shared_items & 1) ^ 1, abort_flag, err_word, kErrWaitOther);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    xs[key] = sum;
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(x_full);
-                } else {
-                    ok = tc::mbar_wait(x_full, shared_items & 1, abort_flag, err_word, kErrWaitOther);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    sum += xs[key];
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(x_empty);
-                }
-                shared_items++;
-            }
-            if (owner && kk < w.kv_len) {
+            if (kk < w.kv_len) {
                 const int i = kk / a.s.page_size;
                 const int page = a.s.table[(int64_t)w.b * a.s.max_pages + i];
                 if (page >= 0 && page < a.s.num_pages)
