@@ -4,12 +4,16 @@
 // What stays keeps its order and moves to the front of the sequence's pages
 // (or of other pages); which tokens stayed is written to `kept`.
 //
-// Two launches: the choice (one CTA per sequence and key head, a radix select
-// on the scores' bits and a prefix sum in index order, so ties go to the
-// lowest index), then the move of K, V and score rows.
+// Two launches: the choice (a radix select on the scores' bits, then the places
+// in index order, so ties go to the lowest index), then the move of K, V and
+// score rows.  Both are bound by what they read and write once, and for few
+// sequences by latency.
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged.cuh"
+#include "tc_common.cuh"
 
 namespace hx {
 namespace {
@@ -48,165 +52,305 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 
 constexpr int kSelThreads = 1024;
+constexpr int kBins = 2048;             // 11 bits of a key a pass (the last pass has 10)
+constexpr int kSmemKeys = 49152;        // keys of a CTA that fit shared memory
+constexpr int kMaxCluster = 8;
 
-__device__ __forceinline__ uint32_t score_key(const Evict &a, int b, int h, int j) {
-    const int page = evict_page(a, a.table, a.max_pages, b, j / a.page_size);
-    if (page < 0) return 0u;
-    return order_key(
-        a.scores[((int64_t)page * a.kv_heads + h) * a.page_size + j % a.page_size]);
+// shared memory of one CTA of the cluster that works on a (sequence, key head)
+struct Select {
+    int hist[2][kBins];
+    int warp_sum[32], warp_eq[32];
+    int counts[2];                      // keys above the threshold, equal to it
+    int bin, left;
+};
+
+// Same variable in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int peer_int(const int *p, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];"
+                 : "=r"(v)
+                 : "r"(tc::mapa_shared(tc::smem_u32(p), rank))
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return n;
 }
 
-// Exclusive prefix sum over the block of two packed counts (16 bits each fit
-// 1024 threads); returns this thread's, and the block's total in `total`.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t x = v;
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-        uint32_t y = warp_sums[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) y += z;
-        }
-        warp_sums[lane] = y;
-    }
-    __syncthreads();
-    total = warp_sums[31];
-    return x - v + (warp > 0 ? warp_sums[warp - 1] : 0u);
-}
-
+// The choice.  A cluster of CTAs works on one sequence and key head, each on a
+// contiguous range of places whose keys it keeps in shared memory (SMEM; read
+// again from the cache otherwise).  Three passes over 11, 11 and 10 bits find
+// the want-th highest key: each CTA counts its keys that share the bits found
+// so far by their next bits, every CTA adds up the cluster's counts (over
+// distributed shared memory) and finds the bin where the count from the top
+// reaches what is wanted.  Then the places are written in ascending order,
+// each warp on a contiguous run, with ballots for the ranks in it.
+template <bool SMEM>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a) {
-    __shared__ int hist[256];
-    __shared__ uint32_t warp_sums[32];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_left;
-    const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
+    __shared__ Select sh;
+    extern __shared__ uint32_t keys[];
+    const uint32_t ranks = cluster_size(), rank = tc::cluster_ctarank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int bh = blockIdx.x / ranks;
+    const int b = bh / a.kv_heads, h = bh % a.kv_heads;
     const int n = evict_len(a, b);
-    int *kept = a.kept + (int64_t)blockIdx.x * a.budget;
+    const int all = kSelThreads * (int)ranks, me = (int)rank * kSelThreads + (int)threadIdx.x;
+    int *kept = a.kept + (int64_t)bh * a.budget;
     const int m = min(n, a.budget);
-    for (int j = m + threadIdx.x; j < a.budget; j += kSelThreads) kept[j] = -1;
-    if (n <= a.budget) {
-        for (int j = threadIdx.x; j < n; j += kSelThreads) kept[j] = j;
+    for (int j = m + me; j < a.budget; j += all) kept[j] = -1;
+    if (n <= a.budget) {            // (the whole cluster)
+        for (int j = me; j < n; j += all) kept[j] = j;
         return;
     }
     // the sinks and the recent ones stay whatever their weight
     const int lo = a.sink, hi = n - a.recent;
     const int want = a.budget - a.sink - a.recent;
-    for (int j = threadIdx.x; j < a.sink; j += kSelThreads) kept[j] = j;
-    for (int j = threadIdx.x; j < a.recent; j += kSelThreads)
-        kept[a.budget - a.recent + j] = hi + j;
+    for (int j = me; j < a.sink; j += all) kept[j] = j;
+    for (int j = me; j < a.recent; j += all) kept[a.budget - a.recent + j] = hi + j;
     if (want == 0) return;
-    // the want-th highest key, byte by byte from the top
+    // this CTA's places: [first, first + count), a multiple of 32 but for the last
+    const int per = ((hi - lo + (int)ranks - 1) / (int)ranks + 31) & ~31;
+    const int first = lo + (int)rank * per;
+    const int count = max(0, min(per, hi - first));
+    auto read_key = [&](int i) -> uint32_t {
+        const int j = first + i, pi = j / a.page_size;
+        const int page = evict_page(a, a.table, a.max_pages, b, pi);
+        if (page < 0) return 0u;
+        return order_key(
+            a.scores[((int64_t)page * a.kv_heads + h) * a.page_size + (j - pi * a.page_size)]);
+    };
+    if (SMEM)
+        for (int i = threadIdx.x; i < count; i += kSelThreads) keys[i] = read_key(i);
+    auto key_at = [&](int i) { return SMEM ? keys[i] : read_key(i); };
     uint32_t prefix = 0, mask = 0;
     int left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        int *hist = sh.hist[pass & 1];
+        for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        for (int j = lo + threadIdx.x; j < hi; j += kSelThreads) {
-            const uint32_t key = score_key(a, b, h, j);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+        for (int i0 = warp * 32; i0 < count; i0 += kSelThreads) {
+            const int i = i0 + lane;
+            uint32_t key = 0;
+            bool in = false;
+            if (i < count) {
+                key = key_at(i);
+                in = (key & mask) == prefix;
+            }
+            const int bin = in ? (int)(key >> shift & ((1u << bits) - 1)) : -1;
+            // (equal scores are common; a warp of one bin adds once)
+            const int bin0 = __shfl_sync(0xffffffffu, bin, 0);
+            if (__all_sync(0xffffffffu, bin == bin0)) {
+                if (lane == 0 && in) atomicAdd(&hist[bin], 32);
+            } else if (in) {
+                atomicAdd(&hist[bin], 1);
+            }
+        }
+        tc::cluster_sync_all();
+        // thread t has bins kBins - 1 - 2t and the one below, counted from the top
+        const int top = kBins - 1 - 2 * (int)threadIdx.x;
+        int h0 = 0, h1 = 0;
+        for (uint32_t r = 0; r < ranks; r++) {
+            h0 += peer_int(&hist[top], r);
+            h1 += peer_int(&hist[top - 1], r);
+        }
+        int upto = h0 + h1;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) sh.warp_sum[warp] = upto;
+        __syncthreads();
+        if (warp == 0) {
+            int v = sh.warp_sum[lane];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += y;
+            }
+            sh.warp_eq[lane] = v;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int bin = 255, rest = left;
-            while (bin > 0 && hist[bin] < rest) rest -= hist[bin--];
-            s_prefix = prefix | (uint32_t)bin << shift;
-            s_left = rest;
+        if (warp > 0) upto += sh.warp_eq[warp - 1];
+        const int before = upto - h0 - h1;
+        if (before < left && left <= upto) {
+            const bool second = left > before + h0;
+            sh.bin = second ? top - 1 : top;
+            sh.left = left - before - (second ? h0 : 0);
         }
         __syncthreads();
-        prefix = s_prefix;
-        left = s_left;
-        mask |= 255u << shift;
-        __syncthreads();
+        prefix |= (uint32_t)sh.bin << shift;
+        left = sh.left;
+        mask |= ((1u << bits) - 1) << shift;
+        // (the next pass counts in the other histogram: peers may still read this one)
     }
-    // in index order: every key above it, and the first `left` equal to it
+    // ranks: keys above the threshold and equal to it in the places before a warp's run
+    const int run = ((count + 31) / 32 + 31) / 32 * 32;         // 32 warps, whole ballots
+    const int i_lo = min(count, warp * run), i_hi = min(count, i_lo + run);
     int above = 0, equal = 0;
-    for (int j0 = lo; j0 < hi; j0 += kSelThreads) {
-        const int j = j0 + threadIdx.x;
-        uint32_t flags = 0;
-        if (j < hi) {
-            const uint32_t key = score_key(a, b, h, j);
-            flags = key > prefix ? 1u : key == prefix ? 0x10000u : 0u;
-        }
-        uint32_t total;
-        const uint32_t before = block_scan(flags, warp_sums, total);
-        const int eq = equal + (int)(before >> 16);
-        const int at = above + (int)(before & 0xffffu) + min(eq, left);
-        if (flags == 1u || (flags != 0 && eq < left)) kept[a.sink + at] = j;
-        above += (int)(total & 0xffffu);
-        equal += (int)(total >> 16);
+    for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
+        const bool in = i0 + lane < i_hi;
+        const uint32_t key = in ? key_at(i0 + lane) : 0u;
+        above += __popc(__ballot_sync(0xffffffffu, in && key > prefix));
+        equal += __popc(__ballot_sync(0xffffffffu, in && key == prefix));
     }
+    if (lane == 0) {
+        sh.warp_sum[warp] = above;
+        sh.warp_eq[warp] = equal;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int x = sh.warp_sum[lane], y = sh.warp_eq[lane];
+        const int x0 = x, y0 = y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) {
+                x += p;
+                y += q;
+            }
+        }
+        sh.warp_sum[lane] = x - x0;
+        sh.warp_eq[lane] = y - y0;
+        if (lane == 31) {
+            sh.counts[0] = x;
+            sh.counts[1] = y;
+        }
+    }
+    tc::cluster_sync_all();
+    above = sh.warp_sum[warp];
+    equal = sh.warp_eq[warp];
+    for (uint32_t r = 0; r < rank; r++) {
+        above += peer_int(&sh.counts[0], r);
+        equal += peer_int(&sh.counts[1], r);
+    }
+    // every key above the threshold, and the first `left` equal to it
+    const uint32_t below = (1u << lane) - 1;
+    for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
+        const bool in = i0 + lane < i_hi;
+        const uint32_t key = in ? key_at(i0 + lane) : 0u;
+        const uint32_t gt = __ballot_sync(0xffffffffu, in && key > prefix);
+        const uint32_t eq = __ballot_sync(0xffffffffu, in && key == prefix);
+        const int e = equal + __popc(eq & below);
+        const int at = above + __popc(gt & below) + min(e, left);
+        if ((gt >> lane & 1) || ((eq >> lane & 1) && e < left))
+            kept[a.sink + at] = first + i0 + lane;
+        above += __popc(gt);
+        equal += __popc(eq);
+    }
+    tc::cluster_sync_all();         // no CTA leaves while a peer may read its counts
 }
 
-// One CTA per sequence, key head, tensor (K, V, scores) and column slice.  Kept
-// token i comes from place kept[i] >= i, so the rows are moved in ascending
-// chunks: a chunk's rows are all read before any of them is written, and no
-// later chunk reads what an earlier one wrote, also when the target pages are
-// the source's.
+// The move of K, V and score rows.  Kept token i comes from place kept[i] >= i.
+//
+// In place (the target's first page is the source's): a CTA moves one column
+// slice of K or V (or the scores) of one sequence and key head in ascending
+// chunks.  A chunk's rows are all read before any of them is written, and no
+// later chunk reads what an earlier one wrote.  To other pages: the same CTAs
+// take row ranges instead.
+constexpr int kMoveThreads = 512;
+
 template <typename W>
-__global__ void __launch_bounds__(256) evict_move_kernel(const Evict a, int row_words, int slices) {
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Evict a, int row_words,
+                                                                  int slices) {
+    constexpr int U = 4;
     const int parts = 2 * slices + 1;
     const int part = blockIdx.x % parts;
     const int bh = blockIdx.x / parts;
     const int b = bh / a.kv_heads, h = bh % a.kv_heads;
     const int n = min(evict_len(a, b), a.budget);
     const int *kept = a.kept + (int64_t)bh * a.budget;
+    if (part == 2 * slices && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[b] = n;
+    if (n == 0) return;
+    const bool in_place = a.table[(int64_t)b * a.max_pages] == a.dst_table[(int64_t)b * a.dst_max_pages];
     auto source = [&](int i) -> int64_t {
-        const int j = kept[i];
-        const int page = evict_page(a, a.table, a.max_pages, b, j / a.page_size);
-        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + j % a.page_size;
+        const int j = kept[i], pi = j / a.page_size;
+        const int page = evict_page(a, a.table, a.max_pages, b, pi);
+        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + (j - pi * a.page_size);
     };
     auto target = [&](int i) -> int64_t {
-        const int page = evict_page(a, a.dst_table, a.dst_max_pages, b, i / a.page_size);
-        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + i % a.page_size;
+        const int pi = i / a.page_size;
+        const int page = evict_page(a, a.dst_table, a.dst_max_pages, b, pi);
+        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + (i - pi * a.page_size);
     };
-    if (part == 2 * slices) {
-        if (h == 0 && threadIdx.x == 0) a.new_lens[b] = n;
-        for (int i0 = 0; i0 < n; i0 += 256) {
-            const int i = i0 + threadIdx.x;
-            int64_t from = -1, to = -1;
-            float x = 0.0f;
-            if (i < n) {
-                from = source(i);
-                to = target(i);
-                if (from >= 0) x = a.scores[from];
-            }
-            __syncthreads();
-            if (from >= 0 && to >= 0 && from != to) a.scores[to] = x;
-        }
-        return;
+    // rows [i_lo, i_hi) of columns [col0, col0 + words)
+    const bool is_score = part == 2 * slices;
+    const int pieces = (is_score ? 1 : slices) * (int)gridDim.y;
+    const int piece = (is_score ? 0 : part % slices * (int)gridDim.y) + (int)blockIdx.y;
+    int i_lo = 0, i_hi = n, words = is_score ? 1 : row_words / slices;
+    int col0 = is_score ? 0 : part % slices * words;
+    if (in_place) {
+        if (blockIdx.y != 0) return;
+    } else {
+        i_lo = (int)((int64_t)n * piece / pieces);
+        i_hi = (int)((int64_t)n * (piece + 1) / pieces);
+        words = is_score ? 1 : row_words;
+        col0 = 0;
     }
-    W *pages = reinterpret_cast<W *>(part < slices ? a.k_pages : a.v_pages);
-    const int words = row_words / slices, col0 = part % slices * words;
-    const int64_t total = (int64_t)n * words;
-    constexpr int U = 4;
-    for (int64_t w0 = 0; w0 < total; w0 += 256 * U) {
-        W x[U];
-        int64_t at[U];
+    // threads of a row: the power of two from `words` on, so that no division is left
+    int shift = 0;
+    while ((1 << shift) < words) shift++;
+    const int c = threadIdx.x & ((1 << shift) - 1);
+    const int rows = kMoveThreads >> shift;
+    for (int i0 = i_lo; i0 < i_hi; i0 += rows * U) {
+        int64_t from[U], to[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t w = w0 + u * 256 + threadIdx.x;
-            at[u] = -1;
-            if (w < total) {
-                const int i = (int)(w / words), c = col0 + (int)(w % words);
-                const int64_t from = source(i), to = target(i);
-                if (from >= 0 && to >= 0 && from != to) {
-                    x[u] = pages[from * row_words + c];
-                    at[u] = to * row_words + c;
-                }
+            const int i = i0 + u * rows + (threadIdx.x >> shift);
+            from[u] = to[u] = -1;
+            if (i < i_hi && c < words) {
+                from[u] = source(i);
+                to[u] = target(i);
+                if (from[u] < 0 || from[u] == to[u]) to[u] = -1;
             }
         }
-        __syncthreads();
+        if (is_score) {
+            float x[U];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (at[u] >= 0) pages[at[u]] = x[u];
+            for (int u = 0; u < U; u++)
+                if (to[u] >= 0) x[u] = a.scores[from[u]];
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (to[u] >= 0) a.scores[to[u]] = x[u];
+        } else {
+            W *pages = reinterpret_cast<W *>(part < slices ? a.k_pages : a.v_pages);
+            W x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (to[u] >= 0) x[u] = pages[from[u] * row_words + col0 + c];
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (to[u] >= 0) pages[to[u] * row_words + col0 + c] = x[u];
+        }
     }
+}
+
+template <bool SMEM>
+int launch_select(Dev *d, const Evict &a, int ranks, size_t smem) {
+    static size_t allowed[64] = {};
+    if (smem > 24576 && smem > allowed[d->ordinal & 63]) {
+        if (int rc = check(cudaFuncSetAttribute(evict_select_kernel<SMEM>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                kSmemKeys * 4),
+                           "cudaFuncSetAttribute(evict_select)"))
+            return rc;
+        allowed[d->ordinal & 63] = kSmemKeys * 4;
+    }
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.batch * a.kv_heads * ranks));
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = d->stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return check(cudaLaunchKernelEx(&cfg, evict_select_kernel<SMEM>, a), "launch evict_select");
 }
 
 }  // namespace
@@ -247,14 +391,27 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
             budget, sink, recent, d->err_word};
     launch_begin(d);
     const int bh = batch * kv_heads;
-    evict_select_kernel<<<bh, kSelThreads, 0, d->stream>>>(a);
+    // CTAs a sequence and key head: as many as keep the device busy, while each
+    // has some thousands of places left
+    const int64_t longest = (int64_t)max_pages * page_size;
+    int ranks = 1;
+    while (ranks < kMaxCluster && (bh * 2 * ranks <= d->sms || longest > (int64_t)ranks * kSmemKeys) &&
+           longest > (int64_t)ranks * 4096)
+        ranks *= 2;
+    const int64_t per = ((longest + ranks - 1) / ranks + 31) / 32 * 32;
+    if (int rc = per <= kSmemKeys ? launch_select<true>(d, a, ranks, (size_t)per * 4)
+                                  : launch_select<false>(d, a, ranks, 0))
+        return rc;
     const bool vec = head_dim % 8 == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15u) == 0;
-    if (vec) {
-        const int slices = head_dim % 64 == 0 ? head_dim / 32 : 1;
-        evict_move_kernel<uint4><<<bh * (2 * slices + 1), 256, 0, d->stream>>>(a, head_dim / 8,
-                                                                               slices);
-    } else {
-        evict_move_kernel<uint16_t><<<bh * 3, 256, 0, d->stream>>>(a, head_dim, 1);
-    }
+    // column slices of 64 bytes, as far as CTAs are missing
+    int slices = 1;
+    while (vec && head_dim % (64 * slices) == 0 && bh * 2 * slices < 2 * d->sms && slices < 4) slices *= 2;
+    // to other pages: 256 rows a CTA
+    const int chunks = (int)std::min<int64_t>(((int64_t)budget + 256 * slices - 1) / (256 * slices), 65535);
+    const dim3 grid((unsigned)(bh * (2 * slices + 1)), (unsigned)chunks);
+    if (vec)
+        evict_move_kernel<uint4><<<grid, kMoveThreads, 0, d->stream>>>(a, head_dim / 8, slices);
+    else
+        evict_move_kernel<uint16_t><<<grid, kMoveThreads, 0, d->stream>>>(a, head_dim, 1);
     return launch_end(d, name, 2);
 }

@@ -72,6 +72,127 @@ __device__ __forceinline__ T *row_target(const NormRope &a, int t, int r, int64_
     return pages + ((page * a.kv_heads + r) * a.page_size + off) * a.dim;
 }
 
+// Four values as 32-bit floats, and back.
+template <typename T>
+__device__ __forceinline__ void widen(uint2 w, float (&x)[4]) {
+    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+    x[0] = a.x;
+    x[1] = a.y;
+    x[2] = b.x;
+    x[3] = b.y;
+}
+template <typename T>
+__device__ __forceinline__ uint2 narrow(const float (&x)[4]) {
+    return make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+}
+
+// Head sizes that are multiples of 8, 8-byte aligned rows: LPR lanes a row (8
+// values a lane), 256 / LPR rows at a time, every thread in the same columns
+// of all its rows, so that a token's cosines and sines and the gains are read
+// once.  A lane's 8 values are two pieces of 4 chosen so that a pair never
+// leaves the lane: columns 4c.. and rot/2 + 4c.. when halves turn together,
+// 8c.. and 8c + 4.. otherwise; in both the lane's four pairs are 4c .. 4c + 3.
+// `ysplit` blocks share a token when tokens are few.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRope a, int ysplit) {
+    constexpr int kRows = 256 / LPR, U = 4;
+    const int c = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const int per_token = a.heads + a.kv_heads * (a.v ? 2 : 1);
+    const bool in_row = c * 8 < a.dim, turns = c * 8 < a.rot;
+    const int o0 = turns && a.halves ? 4 * c : 8 * c;
+    const int o1 = turns && a.halves ? a.rot / 2 + 4 * c : 8 * c + 4;
+    auto gain_of = [&](const void *g, float (&x)[4], float (&y)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = y[i] = 1.0f;
+        if (g && a.norm && in_row) {
+            widen<T>(*reinterpret_cast<const uint2 *>((const T *)g + o0), x);
+            widen<T>(*reinterpret_cast<const uint2 *>((const T *)g + o1), y);
+        }
+    };
+    float gq0[4], gq1[4], gk0[4], gk1[4];
+    gain_of(a.q_gain, gq0, gq1);
+    gain_of(a.k_gain, gk0, gk1);
+    const float inv_dim = 1.0f / (float)a.dim;
+    const int64_t items = (int64_t)a.tokens * ysplit;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int t = (int)(item / ysplit);
+        int pos, off;
+        int64_t page;
+        if (!token_place(a, t, pos, page, off)) continue;
+        float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (turns) {
+            cs = *reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * (a.rot / 2) + 4 * c);
+            sn = *reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * (a.rot / 2) + 4 * c);
+        }
+        const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+        const int step = kRows * ysplit;
+        // (rows of one warp may end at different passes; all lanes stay for the shuffles)
+        for (int r0 = (int)(item % ysplit) * kRows; r0 < per_token; r0 += U * step) {
+            uint2 w0[U], w1[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int r = r0 + u * step + slot;
+                w0[u] = w1[u] = make_uint2(0, 0);
+                if (r < per_token && in_row) {
+                    const T *src = row_source<T>(a, t, r);
+                    w0[u] = *reinterpret_cast<const uint2 *>(src + o0);
+                    w1[u] = *reinterpret_cast<const uint2 *>(src + o1);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int r = r0 + u * step + slot;
+                if (r0 + u * step >= per_token) break;
+                float x[4], y[4];
+                widen<T>(w0[u], x);
+                widen<T>(w1[u], y);
+                float inv = 1.0f;
+                if (a.norm) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    inv = rsqrtf(sum * inv_dim + a.eps);
+                }
+                if (r >= per_token || !in_row) continue;
+                T *dst = row_target<T>(a, t, r, page, off);
+                if (r < a.heads + a.kv_heads) {
+                    const bool is_q = r < a.heads;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        x[i] *= inv * (is_q ? gq0[i] : gk0[i]);
+                        y[i] *= inv * (is_q ? gq1[i] : gk1[i]);
+                    }
+                    if (a.halves) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float p = x[i], q = y[i];
+                            x[i] = p * cv[i] - q * sv[i];
+                            y[i] = p * sv[i] + q * cv[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const float p = x[i], q = x[i + 1], e = y[i], f = y[i + 1];
+                            x[i] = p * cv[i / 2] - q * sv[i / 2];
+                            x[i + 1] = p * sv[i / 2] + q * cv[i / 2];
+                            y[i] = e * cv[2 + i / 2] - f * sv[2 + i / 2];
+                            y[i + 1] = e * sv[2 + i / 2] + f * cv[2 + i / 2];
+                        }
+                    }
+                    w0[u] = narrow<T>(x);
+                    w1[u] = narrow<T>(y);
+                    if (a.scores && !is_q && c == 0)
+                        a.scores[(page * a.kv_heads + (r - a.heads)) * a.page_size + off] = 0.0f;
+                }
+                *reinterpret_cast<uint2 *>(dst + o0) = w0[u];
+                *reinterpret_cast<uint2 *>(dst + o1) = w1[u];
+            }
+        }
+    }
+}
+
 // Any head size up to 256, any alignment: one warp per row, the row in shared
 // memory for its partner columns.
 template <typename T>
@@ -121,6 +242,42 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRope a) {
         if (a.scores && r >= a.heads && lane == 0)
             a.scores[(page * a.kv_heads + (r - a.heads)) * a.page_size + off] = 0.0f;
         __syncwarp();
+    }
+}
+
+// Whether the tensors and strides allow the 8- and 16-byte accesses above.
+bool wide_rows(const NormRope &a) {
+    const uintptr_t p8 = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out |
+                         (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.q_gain |
+                         (uintptr_t)a.k_gain;
+    const uintptr_t p16 = (uintptr_t)a.cos_t | (uintptr_t)a.sin_t;
+    const int64_t strides = (a.heads ? a.q_stride : 0) | (a.kv_heads ? a.k_stride : 0) |
+                            (a.v ? a.v_stride : 0);
+    return a.dim % 8 == 0 && a.rot % 8 == 0 && strides % 4 == 0 && p8 % 8 == 0 &&
+           (a.rot == 0 || p16 % 16 == 0);
+}
+
+template <typename T, int LPR>
+void launch_wide(Dev *d, const NormRope &a) {
+    constexpr auto kern = norm_rope_kernel<T, LPR>;
+    const int rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
+    const int passes = (rows + 256 / LPR - 1) / (256 / LPR);
+    // few tokens: a block per pass, so that a token's rows go out at once
+    const int ysplit = a.tokens < 4 * d->sms ? passes : 1;
+    kern<<<resident_blocks<kern>(d, (int64_t)a.tokens * ysplit * 256), 256, 0, d->stream>>>(a, ysplit);
+}
+template <typename T>
+void launch_rows(Dev *d, const NormRope &a) {
+    if (!wide_rows(a)) {
+        constexpr auto kern = norm_rope_any_kernel<T>;
+        const int64_t rows = (int64_t)a.tokens * (a.heads + a.kv_heads * (a.v ? 2 : 1));
+        kern<<<resident_blocks<kern>(d, rows * 32), 256, 0, d->stream>>>(a);
+    } else if (a.dim <= 64) {
+        launch_wide<T, 8>(d, a);
+    } else if (a.dim <= 128) {
+        launch_wide<T, 16>(d, a);
+    } else {
+        launch_wide<T, 32>(d, a);
     }
 }
 
@@ -193,13 +350,9 @@ HX_EXPORT int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_
     a.eps = eps;
     a.err_word = d->err_word;
     launch_begin(d);
-    const int64_t rows = (int64_t)tokens * (heads + kv_heads * (a.v ? 2 : 1));
-    if (dtype == HEXCUDA_F16) {
-        constexpr auto kern = norm_rope_any_kernel<__half>;
-        kern<<<resident_blocks<kern>(d, rows * 32), 256, 0, d->stream>>>(a);
-    } else {
-        constexpr auto kern = norm_rope_any_kernel<__nv_bfloat16>;
-        kern<<<resident_blocks<kern>(d, rows * 32), 256, 0, d->stream>>>(a);
-    }
+    if (dtype == HEXCUDA_F16)
+        launch_rows<__half>(d, a);
+    else
+        launch_rows<__nv_bfloat16>(d, a);
     return launch_end(d, name);
 }
