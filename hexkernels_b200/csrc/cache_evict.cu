@@ -121,8 +121,37 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
         return order_key(
             a.scores[((int64_t)page * a.kv_heads + h) * a.page_size + (j - pi * a.page_size)]);
     };
-    if (SMEM)
-        for (int i = threadIdx.x; i < count; i += kSelThreads) keys[i] = read_key(i);
+    if (SMEM) {
+        // eight keys a thread at a time: all their pages, then all their scores
+        constexpr int U = 8;
+        for (int i0 = threadIdx.x; i0 < count; i0 += U * kSelThreads) {
+            int page[U];
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + u * kSelThreads;
+                page[u] = i < count
+                              ? a.table[(int64_t)b * a.max_pages + (first + i) / a.page_size]
+                              : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + u * kSelThreads;
+                x[u] = 0.0f;
+                if (i < count && page[u] >= 0 && page[u] < a.num_pages)
+                    x[u] = a.scores[((int64_t)page[u] * a.kv_heads + h) * a.page_size +
+                                    (first + i) % a.page_size];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + u * kSelThreads;
+                if (i >= count) break;
+                const bool bad = page[u] < 0 || page[u] >= a.num_pages;
+                if (bad) flag_index(a.err_word);
+                keys[i] = bad ? 0u : order_key(x[u]);
+            }
+        }
+    }
     auto key_at = [&](int i) { return SMEM ? keys[i] : read_key(i); };
     uint32_t prefix = 0, mask = 0;
     int left = want;
@@ -243,88 +272,98 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
 }
 
 // The move of K, V and score rows.  Kept token i comes from place kept[i] >= i.
+// A CTA works on one sequence and key head in chunks of 256 kept tokens: each
+// thread looks up the rows of one token (places, pages) for all, then the rows
+// are copied, all loads of a chunk in flight together.
 //
 // In place (the target's first page is the source's): a CTA moves one column
-// slice of K or V (or the scores) of one sequence and key head in ascending
-// chunks.  A chunk's rows are all read before any of them is written, and no
-// later chunk reads what an earlier one wrote.  To other pages: the same CTAs
-// take row ranges instead.
-constexpr int kMoveThreads = 512;
+// slice of K or V (or the scores), chunk after ascending chunk.  A chunk's rows
+// are all read before any of them is written, and no later chunk reads what an
+// earlier one wrote.  To other pages: each CTA takes chunks of its own.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 256;
 
 template <typename W>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Evict a, int row_words,
                                                                   int slices) {
-    constexpr int U = 4;
+    constexpr int U = 8;
+    __shared__ int64_t from[2][kMoveRows], to[2][kMoveRows];
     const int parts = 2 * slices + 1;
     const int part = blockIdx.x % parts;
     const int bh = blockIdx.x / parts;
     const int b = bh / a.kv_heads, h = bh % a.kv_heads;
     const int n = min(evict_len(a, b), a.budget);
     const int *kept = a.kept + (int64_t)bh * a.budget;
-    if (part == 2 * slices && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[b] = n;
+    const bool is_score = part == 2 * slices;
+    if (is_score && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[b] = n;
     if (n == 0) return;
     const bool in_place = a.table[(int64_t)b * a.max_pages] == a.dst_table[(int64_t)b * a.dst_max_pages];
-    auto source = [&](int i) -> int64_t {
-        const int j = kept[i], pi = j / a.page_size;
-        const int page = evict_page(a, a.table, a.max_pages, b, pi);
-        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + (j - pi * a.page_size);
+    if (in_place && blockIdx.y != 0) return;
+    // this thread's token of the chunk at i0: the rows of the cache it leaves and
+    // goes to, -1 when there is nothing to move
+    auto look_up = [&](int i0, int buf) {
+        const int i = i0 + threadIdx.x;
+        int64_t f = -1, t = -1;
+        if (i < n) {
+            const int j = kept[i], pj = j / a.page_size, pi = i / a.page_size;
+            const int source = evict_page(a, a.table, a.max_pages, b, pj);
+            const int target = evict_page(a, a.dst_table, a.dst_max_pages, b, pi);
+            if (source >= 0 && target >= 0) {
+                f = ((int64_t)source * a.kv_heads + h) * a.page_size + (j - pj * a.page_size);
+                t = ((int64_t)target * a.kv_heads + h) * a.page_size + (i - pi * a.page_size);
+                if (f == t) t = -1;
+            }
+        }
+        from[buf][threadIdx.x] = f;
+        to[buf][threadIdx.x] = t;
     };
-    auto target = [&](int i) -> int64_t {
-        const int pi = i / a.page_size;
-        const int page = evict_page(a, a.dst_table, a.dst_max_pages, b, pi);
-        return page < 0 ? -1 : ((int64_t)page * a.kv_heads + h) * a.page_size + (i - pi * a.page_size);
-    };
-    // rows [i_lo, i_hi) of columns [col0, col0 + words)
-    const bool is_score = part == 2 * slices;
-    const int pieces = (is_score ? 1 : slices) * (int)gridDim.y;
-    const int piece = (is_score ? 0 : part % slices * (int)gridDim.y) + (int)blockIdx.y;
-    int i_lo = 0, i_hi = n, words = is_score ? 1 : row_words / slices;
-    int col0 = is_score ? 0 : part % slices * words;
-    if (in_place) {
-        if (blockIdx.y != 0) return;
-    } else {
-        i_lo = (int)((int64_t)n * piece / pieces);
-        i_hi = (int)((int64_t)n * (piece + 1) / pieces);
-        words = is_score ? 1 : row_words;
-        col0 = 0;
-    }
+    // in place: every chunk of one slice; else every `stride`-th chunk, whole rows
+    const int pieces = is_score ? 1 : slices;
+    const int words = is_score ? 1 : in_place ? row_words / slices : row_words;
+    const int col0 = in_place && !is_score ? part % slices * words : 0;
+    const int stride = in_place ? 1 : pieces * (int)gridDim.y;
+    const int chunk0 = in_place ? 0 : (is_score ? 0 : part % slices * (int)gridDim.y) + (int)blockIdx.y;
+    const int chunks = (n + kMoveRows - 1) / kMoveRows;
+    if (chunk0 >= chunks) return;
     // threads of a row: the power of two from `words` on, so that no division is left
     int shift = 0;
     while ((1 << shift) < words) shift++;
-    const int c = threadIdx.x & ((1 << shift) - 1);
+    const int c = threadIdx.x & ((1 << shift) - 1), row0 = threadIdx.x >> shift;
     const int rows = kMoveThreads >> shift;
-    for (int i0 = i_lo; i0 < i_hi; i0 += rows * U) {
-        int64_t from[U], to[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + u * rows + (threadIdx.x >> shift);
-            from[u] = to[u] = -1;
-            if (i < i_hi && c < words) {
-                from[u] = source(i);
-                to[u] = target(i);
-                if (from[u] < 0 || from[u] == to[u]) to[u] = -1;
-            }
-        }
+    W *pages = reinterpret_cast<W *>(part < slices ? a.k_pages : a.v_pages);
+    int buf = 0;
+    look_up(chunk0 * kMoveRows, buf);
+    __syncthreads();
+    for (int chunk = chunk0; chunk < chunks; chunk += stride, buf ^= 1) {
         if (is_score) {
-            float x[U];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (to[u] >= 0) x[u] = a.scores[from[u]];
+            float x = 0.0f;
+            const int64_t t = to[buf][threadIdx.x];
+            if (t >= 0) x = a.scores[from[buf][threadIdx.x]];
+            if (chunk + stride < chunks) look_up((chunk + stride) * kMoveRows, buf ^ 1);
             __syncthreads();
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (to[u] >= 0) a.scores[to[u]] = x[u];
-        } else {
-            W *pages = reinterpret_cast<W *>(part < slices ? a.k_pages : a.v_pages);
+            if (t >= 0) a.scores[t] = x;
+            continue;
+        }
+        // rows of a chunk that its threads can hold in registers at once
+        for (int r0 = 0; r0 < kMoveRows; r0 += rows * U) {
             W x[U];
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (to[u] >= 0) x[u] = pages[from[u] * row_words + col0 + c];
+            for (int u = 0; u < U; u++) {
+                const int r = r0 + u * rows + row0;
+                if (r < kMoveRows && c < words && to[buf][r] >= 0)
+                    x[u] = pages[from[buf][r] * row_words + col0 + c];
+            }
+            if (r0 == 0 && chunk + stride < chunks)
+                look_up((chunk + stride) * kMoveRows, buf ^ 1);
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (to[u] >= 0) pages[to[u] * row_words + col0 + c] = x[u];
+            for (int u = 0; u < U; u++) {
+                const int r = r0 + u * rows + row0;
+                if (r < kMoveRows && c < words && to[buf][r] >= 0)
+                    pages[to[buf][r] * row_words + col0 + c] = x[u];
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -406,8 +445,9 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
     // column slices of 64 bytes, as far as CTAs are missing
     int slices = 1;
     while (vec && head_dim % (64 * slices) == 0 && bh * 2 * slices < 2 * d->sms && slices < 4) slices *= 2;
-    // to other pages: 256 rows a CTA
-    const int chunks = (int)std::min<int64_t>(((int64_t)budget + 256 * slices - 1) / (256 * slices), 65535);
+    // to other pages: a chunk of tokens a CTA
+    const int per_cta = kMoveRows * slices;
+    const int chunks = (int)std::min<int64_t>(((int64_t)budget + per_cta - 1) / per_cta, 65535);
     const dim3 grid((unsigned)(bh * (2 * slices + 1)), (unsigned)chunks);
     if (vec)
         evict_move_kernel<uint4><<<grid, kMoveThreads, 0, d->stream>>>(a, head_dim / 8, slices);

@@ -8,17 +8,18 @@
 //     S^T [128 keys x N rows] = K Q^T      A = K as it lies in the pages
 //     O^T [D x N rows]       += V^T P^T    A = V as it lies (MN-major)
 // with N = 16 or 32 query rows (tokens x heads of one key head).  A softmax
-// thread owns one key: it reads its N scores from tensor memory, subtracts the
-// row's reference maximum, takes 2^x, adds to its own N partial sums and
-// writes P^T (N contiguous 16-bit values, the MN-major B operand) to shared
-// memory.  Maxima over keys are only needed when some score exceeds its row's
+// thread owns one key and half of the rows: it reads its N / 2 scores from
+// tensor memory, subtracts the rows' reference maxima, takes 2^x, adds to its
+// own partial sums and writes its half of P^T's row (N contiguous 16-bit values
+// a key, the MN-major B operand) to shared memory.  Maxima over keys are only needed when some score exceeds its row's
 // reference by 2^8 (or at an item's first tile); a vote per tile finds that
 // out, then the reference moves and O^T is rescaled.  Row sums are reduced
 // over the threads once per item.
 //
-// Per CTA (one per SM): warp 0 TMA, one lane per page fragment; warp 1 tensor
-// memory and MMA issue, S^T of the next tile before P V of this one; warps 4-7
-// softmax.  Key and value tiles of 128 tokens go through rings of 3 stages
+// Per CTA (one per SM), 384 threads: warps 0 and 3 TMA of keys and of values,
+// one lane per page fragment; warp 1 tensor memory and MMA issue, S^T of the
+// next tile before P V of this one; two softmax warpgroups, one for each half
+// of the rows, which know nothing of one another.  Key and value tiles of 128 tokens go through rings of 3 stages
 // (dim 128; 6 at dim 64), 192 KB of loads in flight per SM.
 //
 // Every wait is bounded; see mbar_wait.
@@ -39,7 +40,7 @@ struct DecSmem {
     static constexpr int kV = kK + kStages * kTile;
     static constexpr int kQ = kV + kStages * kTile;        // 2 buffers
     static constexpr int kP = kQ + 2 * kQTile;             // 2 buffers of 128 x N
-    static constexpr int kRed = kP + 2 * kKeys * N * 2;    // [4][N] maxima or sums, [N] results
+    static constexpr int kRed = kP + 2 * kKeys * N * 2;    // [4][N] maxima or sums, [N] 1 / sum
     static constexpr int kPlan = kRed + 5 * N * 4;
     static constexpr int kBar = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;
     // q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2],
@@ -48,28 +49,30 @@ struct DecSmem {
     static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
 };
 
-// Or of a condition over the softmax warps (named barrier 1).
-__device__ __forceinline__ bool vote_or(bool p) {
+// Or of a condition over the 128 threads of a softmax warpgroup (its named
+// barrier).
+__device__ __forceinline__ bool vote_or(int barrier, bool p) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, 128, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"((uint32_t)p)
+        : "r"(barrier), "r"((uint32_t)p)
         : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() {
-    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+__device__ __forceinline__ void softmax_sync(int barrier) {
+    asm volatile("barrier.cta.sync %0, 128;" ::"r"(barrier) : "memory");
 }
 
-// N per-lane values reduced over the warp; lane l gets column l * N / 32.
-template <int N, bool MAX>
-__device__ __forceinline__ float reduce_columns(float (&v)[N], int lane) {
+// C per-lane values (8 or 16) reduced over the warp; lane l gets column l * C / 32.
+template <int C, bool MAX>
+__device__ __forceinline__ float reduce_columns(float (&v)[C], int lane) {
+    int o = 16;
 #pragma unroll
-    for (int n = N / 2, o = 16; n > 0; n >>= 1, o >>= 1) {
+    for (int n = C / 2; n > 0; n >>= 1, o >>= 1) {
         const bool up = (lane & o) != 0;
 #pragma unroll
         for (int i = 0; i < n; i++) {
@@ -78,32 +81,32 @@ __device__ __forceinline__ float reduce_columns(float (&v)[N], int lane) {
             v[i] = MAX ? fmaxf(keep, got) : keep + got;
         }
     }
-    if constexpr (N == 16) {
-        const float got = __shfl_xor_sync(0xffffffffu, v[0], 1);
+    for (; o > 0; o >>= 1) {
+        const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
         v[0] = MAX ? fmaxf(v[0], got) : v[0] + got;
     }
     return v[0];
 }
 
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[8]) {
+    tc::tmem_ld_32x32b_x8(taddr, r);
+    tc::tmem_ld_wait(r);
+}
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[16]) {
     tc::tmem_ld_32x32b_x16(taddr, r);
     tc::tmem_ld_wait(r);
 }
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[32]) {
-    tc::tmem_ld_32x32b_x32(taddr, r);
-    tc::tmem_ld_wait(r);
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[8]) {
+    tc::tmem_st_32x32b_x8(taddr, r);
+    tc::tmem_st_wait();
 }
 __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[16]) {
     tc::tmem_st_32x32b_x16(taddr, r);
     tc::tmem_st_wait();
 }
-__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r)[32]) {
-    tc::tmem_st_32x32b_x32(taddr, r);
-    tc::tmem_st_wait();
-}
 
 template <typename T, int D, int N>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(384, 1)
     paged_dec_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const PagedTc a) {
     using L = DecSmem<D, N>;
@@ -128,11 +131,11 @@ __global__ void __launch_bounds__(256, 1)
             tc::mbar_init(&q_full[i], 1);
             tc::mbar_init(&q_empty[i], 1);
             tc::mbar_init(&s_full[i], 1);
-            tc::mbar_init(&s_empty[i], 4);
-            tc::mbar_init(&p_full[i], 4);
+            tc::mbar_init(&s_empty[i], 8);
+            tc::mbar_init(&p_full[i], 8);
             tc::mbar_init(&pv_done[i], 1);
         }
-        tc::mbar_init(o_free, 4);
+        tc::mbar_init(o_free, 8);
         tc::mbar_init(drain, 1);
         for (int i = 0; i < S; i++) {
             tc::mbar_init(&k_full[i], 1);
@@ -152,63 +155,65 @@ __global__ void __launch_bounds__(256, 1)
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    const bool any = plan_run<256>(a, a.tok, plan);
+    const bool any = plan_run<384>(a, a.tok, plan);
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_o = tmem_base + 2 * N;
 
     if (!any) {
         // nothing to do but free the tensor memory
-    } else if (warp == 0) {
-        // --------------------------------------------------------------- TMA
+    } else if (warp == 0 || warp == 3) {
+        // ------------------------------------------ TMA: keys (and Q), values
+        // (two warps, because a page of 16 tokens makes 32 loads of a tile, and
+        // the loads that one warp can start were the bound)
+        const bool keys = warp == 0;
+        uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+        const CUtensorMap *map = keys ? &tmK : &tmV;
+        uint8_t *ring = smem + (keys ? L::kK : L::kV);
         Walk w = plan.start;
         int seg = 0, st = 0;
-        uint32_t ph = 0, armed = 0, armed_q = 0;      // stages and phases last loaded
-        uint32_t k_ph = 0, v_ph = 0, q_ph = 0, armed_v = 0;
-        bool ok = true;
-        int row = frag_row(a, w, w.j0, lane);
-        do {
-            const int qb = seg & 1;
-            ok = tc::mbar_wait(&q_empty[qb], ((seg >> 1) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+        uint32_t ph = 0, armed_q = 0, armed = 0, q_ph = 0, last_ph = 0;     // last loads
+        bool ok = true, more = true;
+        int j = w.j0;
+        Frag f = frag_of(a, w, j, lane);
+        while (more) {
+            const Frag f_now = f;
+            const int h = w.h;
+            const bool first = j == w.j0;
+            const int q_row = w.first + w.rt * a.tok;
+            // the tile after this one, and its pages
+            if (++j == w.j1) {
+                more = w.next(a, a.tok);
+                j = w.j0;
+            }
+            if (more) f = frag_of(a, w, j, lane);
+            if (first && keys) {
+                const int qb = seg & 1;
+                ok = tc::mbar_wait(&q_empty[qb], ((seg >> 1) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(a.tok * a.group * 128 * kSubs));
+                    for (int c = 0; c < kSubs; c++)
+                        tc::tma_load_3d(smem + L::kQ + qb * L::kQTile + c * N * 128, &tmQ, &q_full[qb],
+                                        c * 64, h * a.group, q_row);
+                }
+                armed_q |= 1u << qb;
+                q_ph = (q_ph & ~(1u << qb)) | (((uint32_t)(seg >> 1) & 1u) << qb);
+                seg++;
+            }
+            ok = tc::mbar_wait(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            if (lane == 0) {
-                tc::mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(a.tok * a.group * 128 * kSubs));
-                for (int c = 0; c < kSubs; c++)
-                    tc::tma_load_3d(smem + L::kQ + qb * L::kQTile + c * N * 128, &tmQ, &q_full[qb],
-                                    c * 64, w.h * a.group, w.first + w.rt * a.tok);
+            const int row = frag_row(a, f_now, h), count = frag_count(row);
+            load_frags<kSubs>(a, ring + st * L::kTile, map, &full[st], row, count, lane);
+            armed |= 1u << st;
+            last_ph = (last_ph & ~(1u << st)) | (ph << st);
+            if (++st == S) {
+                st = 0;
+                ph ^= 1;
             }
-            armed_q |= 1u << qb;
-            q_ph = (q_ph & ~(1u << qb)) | (((uint32_t)(seg >> 1) & 1u) << qb);
-            const int j1 = w.j1;
-            Walk cur = w;
-            for (int j = cur.j0; j < j1; j++) {
-                const int count = frag_count(row);
-                ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
-                armed |= 1u << st;
-                k_ph = (k_ph & ~(1u << st)) | (ph << st);
-                // the next tile's pages, while the value stage drains
-                int row_next = -1;
-                if (j + 1 < j1) row_next = frag_row(a, cur, j + 1, lane);
-                ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
-                armed_v |= 1u << st;
-                v_ph = (v_ph & ~(1u << st)) | (ph << st);
-                row = row_next;
-                if (++st == S) {
-                    st = 0;
-                    ph ^= 1;
-                }
-            }
-            seg++;
-            if (!ok || !w.next(a, a.tok)) break;
-            row = frag_row(a, w, w.j0, lane);
-        } while (true);
+        }
         if (lane == 0) {
             // drain our own loads (a no-op when every load was consumed)
             const uint64_t t0 = tc::globaltimer();
@@ -218,10 +223,8 @@ __global__ void __launch_bounds__(256, 1)
             };
             for (int i = 0; i < 2; i++)
                 if (armed_q >> i & 1) drain_wait(&q_full[i], q_ph >> i & 1);
-            for (int i = 0; i < S; i++) {
-                if (armed >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
-                if (armed_v >> i & 1) drain_wait(&v_full[i], v_ph >> i & 1);
-            }
+            for (int i = 0; i < S; i++)
+                if (armed >> i & 1) drain_wait(&full[i], last_ph >> i & 1);
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -302,10 +305,15 @@ __global__ void __launch_bounds__(256, 1)
         }
     } else if (warp >= 4) {
         // ----------------------------------------------------------- softmax
-        const int key = threadIdx.x - 128, qw = warp & 3;
+        // rows n0 .. n0 + C - 1 of the tile, barrier 1 + x
+        constexpr int C = N / 2;
+        const int x = (warp - 4) >> 2, n0 = x * C, bar = 1 + x;
+        const int qw = warp & 3, key = qw * 32 + lane;
         const uint32_t lane_base = (uint32_t)(qw * 32) << 16;
         float *red = reinterpret_cast<float *>(smem + L::kRed);     // [4][N]
         float *res = red + 4 * N;                                   // [N]
+        const bool col_lane = lane % (32 / C) == 0;                 // holds a reduced column
+        const int col = n0 + lane / (32 / C);
         Walk w = plan.start;
         int st = 0;
         uint32_t ph = 0, g = 0;
@@ -315,9 +323,9 @@ __global__ void __launch_bounds__(256, 1)
             const int t0 = w.rt * a.tok, ntok = min(a.tok, w.q_len - t0);
             const int nrows = ntok * a.group;
             const int seen0 = min(w.kv_len, seen_by(a.s, w.kv_len, w.q_len, t0));   // fewest keys
-            float m[N], l[N];
+            float m[C], l[C];
 #pragma unroll
-            for (int n = 0; n < N; n++) {
+            for (int n = 0; n < C; n++) {
                 m[n] = -INFINITY;
                 l[n] = 0.0f;
             }
@@ -325,12 +333,12 @@ __global__ void __launch_bounds__(256, 1)
                 const int buf = g & 1;
                 bool ok = tc::mbar_wait(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
                 tc::tc_fence_after();
-                float x[N];
+                float v[C];
                 if (ok) {
-                    uint32_t r[N];
-                    load_columns(tmem_base + buf * N + lane_base, r);
+                    uint32_t r[C];
+                    load_columns(tmem_base + buf * N + n0 + lane_base, r);
 #pragma unroll
-                    for (int n = 0; n < N; n++) x[n] = __uint_as_float(r[n]) * a.scale_log2;
+                    for (int n = 0; n < C; n++) v[n] = __uint_as_float(r[n]) * a.scale_log2;
                 }
                 tc::tc_fence_before();
                 __syncwarp();
@@ -338,10 +346,10 @@ __global__ void __launch_bounds__(256, 1)
                 const int kk = j * kKeys + key;
                 if (j * kKeys + kKeys > seen0) {
                     // the rows of token t see the keys before seen_by(t)
-                    int t = t0, i = 0;
+                    int t = t0 + n0 / a.group, i = n0 % a.group;
 #pragma unroll
-                    for (int n = 0; n < N; n++) {
-                        if (kk >= min(w.kv_len, seen_by(a.s, w.kv_len, w.q_len, t))) x[n] = -INFINITY;
+                    for (int n = 0; n < C; n++) {
+                        if (kk >= min(w.kv_len, seen_by(a.s, w.kv_len, w.q_len, t))) v[n] = -INFINITY;
                         if (++i == a.group) {
                             i = 0;
                             t++;
@@ -350,27 +358,28 @@ __global__ void __launch_bounds__(256, 1)
                 }
                 bool high = j == w.j0;
 #pragma unroll
-                for (int n = 0; n < N; n++) high |= x[n] > m[n] + 8.0f;
-                if (vote_or(high || !ok)) {
-                    float top[N];
+                for (int n = 0; n < C; n++) high |= v[n] > m[n] + 8.0f;
+                if (vote_or(bar, high || !ok)) {
+                    float top[C];
 #pragma unroll
-                    for (int n = 0; n < N; n++) top[n] = x[n];
-                    const float mine = reduce_columns<N, true>(top, lane);
-                    if (N == 32 || (lane & 1) == 0) red[qw * N + (N == 32 ? lane : lane >> 1)] = mine;
+                    for (int n = 0; n < C; n++) top[n] = v[n];
+                    const float mine = reduce_columns<C, true>(top, lane);
+                    if (col_lane) red[qw * N + col] = mine;
                     // (the tile before this one has its P V done: O is stable)
                     if (ok && j > w.j0)
                         ok = tc::mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
                                            kErrWaitAccum);
-                    if (vote_or(!ok)) {
+                    if (vote_or(bar, !ok)) {
                         run = false;
                         break;
                     }
                     tc::tc_fence_after();
-                    float corr[N];
+                    float corr[C];
                     bool moved = false;
 #pragma unroll
-                    for (int n = 0; n < N; n++) {
-                        const float t4 = fmaxf(fmaxf(red[n], red[N + n]), fmaxf(red[2 * N + n], red[3 * N + n]));
+                    for (int n = 0; n < C; n++) {
+                        const float *p = red + n0 + n;
+                        const float t4 = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
                         corr[n] = 1.0f;
                         if (t4 > m[n] + 8.0f || (j == w.j0 && t4 > m[n])) {
                             corr[n] = tc::ex2(m[n] - t4);
@@ -380,20 +389,20 @@ __global__ void __launch_bounds__(256, 1)
                         }
                     }
                     if (moved && j > w.j0) {
-                        uint32_t o[N];
-                        load_columns(tmem_o + lane_base, o);
+                        uint32_t o[C];
+                        load_columns(tmem_o + n0 + lane_base, o);
 #pragma unroll
-                        for (int n = 0; n < N; n++)
+                        for (int n = 0; n < C; n++)
                             o[n] = __float_as_uint(__uint_as_float(o[n]) * corr[n]);
-                        store_columns(tmem_o + lane_base, o);
+                        store_columns(tmem_o + n0 + lane_base, o);
                     }
                 }
-                // P^T of this key: N weights relative to the references
-                uint32_t pk[N / 2];
+                // P^T of this key: weights relative to the references
+                uint32_t pk[C / 2];
 #pragma unroll
-                for (int n = 0; n < N; n += 2) {
-                    const float p0 = tc::ex2(x[n] - (m[n] == -INFINITY ? 0.0f : m[n]));
-                    const float p1 = tc::ex2(x[n + 1] - (m[n + 1] == -INFINITY ? 0.0f : m[n + 1]));
+                for (int n = 0; n < C; n += 2) {
+                    const float p0 = tc::ex2(v[n] - (m[n] == -INFINITY ? 0.0f : m[n]));
+                    const float p1 = tc::ex2(v[n + 1] - (m[n + 1] == -INFINITY ? 0.0f : m[n + 1]));
                     l[n] += p0;
                     l[n + 1] += p1;
                     pk[n / 2] = pack2<T>(p0, p1);
@@ -403,7 +412,7 @@ __global__ void __launch_bounds__(256, 1)
                     ok = tc::mbar_wait(&pv_done[buf], ((g - 2) >> 1) & 1, abort_flag, err_word,
                                        kErrWaitAccum);
                 const int valid = w.kv_len - j * kKeys;
-                if (valid < kKeys) {
+                if (x == 0 && valid < kKeys) {
                     if (ok) ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
                     if (ok) clear_rows<kSubs>(smem + L::kV + st * L::kTile, key, valid);
                 }
@@ -412,8 +421,9 @@ __global__ void __launch_bounds__(256, 1)
                                                             key * N * 2);
                     const int sw = N == 16 ? (key >> 2) & 1 : (key >> 1) & 3;
 #pragma unroll
-                    for (int c = 0; c < N / 8; c++)
-                        prow[c ^ sw] = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                    for (int c = 0; c < C / 8; c++)
+                        prow[(n0 / 8 + c) ^ sw] =
+                            make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
                 }
                 tc::fence_proxy_async_smem();
                 tc::tc_fence_before();
@@ -428,59 +438,60 @@ __global__ void __launch_bounds__(256, 1)
             // ---- end of the segment: row sums over the keys, O^T / l
             bool ok = tc::mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
                                     kErrWaitAccum);
-            float mine = reduce_columns<N, false>(l, lane);
-            if (N == 32 || (lane & 1) == 0) red[qw * N + (N == 32 ? lane : lane >> 1)] = mine;
-            if (vote_or(!ok)) break;
+            const float mine = reduce_columns<C, false>(l, lane);
+            if (col_lane) red[qw * N + col] = mine;
+            if (vote_or(bar, !ok)) break;
             tc::tc_fence_after();
             const bool whole = w.j0 == 0 && w.j1 == w.nt;
             const int slot = blockIdx.x * 2 + (w.j0 == 0 ? 1 : 0);
-            if (key < N) {
-                const float sum = (red[key] + red[N + key]) + (red[2 * N + key] + red[3 * N + key]);
+            if (key < C) {
+                const int n = n0 + key;
+                const float sum = (red[n] + red[N + n]) + (red[2 * N + n] + red[3 * N + n]);
                 float top = 0.0f;
 #pragma unroll
-                for (int n = 0; n < N; n++) top = key == n ? m[n] : top;
-                res[key] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (key < nrows) {
+                for (int i = 0; i < C; i++) top = key == i ? m[i] : top;
+                res[n] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (n < nrows) {
                     if (!whole) {
-                        float *ml = a.part_ml + ((size_t)slot * kPartRows + key) * 2;
+                        float *ml = a.part_ml + ((size_t)slot * kPartRows + n) * 2;
                         ml[0] = top;
                         ml[1] = sum;
                     } else if (a.lse) {
-                        const int64_t r = (int64_t)(w.first + t0 + key / a.group) * a.heads +
-                                          w.h * a.group + key % a.group;
+                        const int64_t r = (int64_t)(w.first + t0 + n / a.group) * a.heads +
+                                          w.h * a.group + n % a.group;
                         a.lse[r] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
                     }
                 }
             }
-            softmax_sync();
-            uint32_t o[N];
-            load_columns(tmem_o + lane_base, o);
+            softmax_sync(bar);
+            uint32_t o[C];
+            load_columns(tmem_o + n0 + lane_base, o);
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(o_free);
             if (key < D) {
                 if (whole) {
-                    int t = 0, i = 0;
+                    int t = n0 / a.group, i = n0 % a.group;
 #pragma unroll
-                    for (int n = 0; n < N; n++) {
-                        if (n < nrows)
+                    for (int n = 0; n < C; n++) {
+                        if (n0 + n < nrows)
                             out[((int64_t)(w.first + t0 + t) * a.heads + w.h * a.group + i) * D + key] =
-                                from_f32<T>(__uint_as_float(o[n]) * res[n]);
+                                from_f32<T>(__uint_as_float(o[n]) * res[n0 + n]);
                         if (++i == a.group) {
                             i = 0;
                             t++;
                         }
                     }
                 } else {
-                    float *po = a.part_o + (size_t)slot * kPartRows * D + key;
+                    float *po = a.part_o + ((size_t)slot * kPartRows + n0) * D + key;
 #pragma unroll
-                    for (int n = 0; n < N; n++)
-                        if (n < nrows) po[n * D] = __uint_as_float(o[n]);
+                    for (int n = 0; n < C; n++)
+                        if (n0 + n < nrows) po[n * D] = __uint_as_float(o[n]);
                 }
             }
             Walk last = w;
             if (!w.next(a, a.tok)) {
-                if (key == 0) note_parts(a, plan, last, a.tok);
+                if (x == 0 && key == 0) note_parts(a, plan, last, a.tok);
                 break;
             }
         } while (true);
@@ -509,7 +520,7 @@ int launch_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUten
             return rc;
         attr_done[d->ordinal & 63] = true;
     }
-    paged_dec_kernel<T, D, N><<<d->sms, 256, L::kTotal, d->stream>>>(mq, mk, mv, a);
+    paged_dec_kernel<T, D, N><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, mv, a);
     return HEXCUDA_OK;
 }
 

@@ -148,50 +148,57 @@ __global__ void __launch_bounds__(384, 1)
         Walk w = plan.start;
         int seg = 0, st = 0;
         uint32_t ph = 0, armed_k = 0, armed_v = 0, k_ph = 0, v_ph = 0;
-        bool ok = true;
-        int row = frag_row(a, w, w.j0, lane);
-        do {
-            int t0, ntok_a, ntok_b, hi;
-            tile_span(a, w, 1, t0, ntok_b, hi);
-            tile_span(a, w, 0, t0, ntok_a, hi);
-            ok = tc::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+        bool ok = true, more = true;
+        int j = w.j0;
+        Frag f = frag_of(a, w, j, lane);
+        while (more) {
+            // the tile after this one, and its pages
+            Walk ahead = w;
+            int j_next = j + 1;
+            if (j_next == w.j1) {
+                more = ahead.next(a, item_tok);
+                j_next = ahead.j0;
+            }
+            Frag f_next = f;
+            if (more) f_next = frag_of(a, ahead, j_next, lane);
+            if (j == w.j0) {
+                int t0, ntok_a, ntok_b, hi;
+                tile_span(a, w, 1, t0, ntok_b, hi);
+                tile_span(a, w, 0, t0, ntok_a, hi);
+                ok = tc::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    const int tiles = ntok_b > 0 ? 2 : 1;
+                    tc::mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * a.tok * a.group * 128 * kSubs));
+                    for (int x = 0; x < tiles; x++)
+                        for (int c = 0; c < kSubs; c++)
+                            tc::tma_load_3d(smem + L::kQ + x * L::kTile + c * kSubTile, &tmQ, q_full,
+                                            c * 64, w.h * a.group, w.first + t0 + x * a.tok);
+                }
+                seg++;
+            }
+            ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            if (lane == 0) {
-                const int tiles = ntok_b > 0 ? 2 : 1;
-                tc::mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * a.tok * a.group * 128 * kSubs));
-                for (int x = 0; x < tiles; x++)
-                    for (int c = 0; c < kSubs; c++)
-                        tc::tma_load_3d(smem + L::kQ + x * L::kTile + c * kSubTile, &tmQ, q_full,
-                                        c * 64, w.h * a.group, w.first + t0 + x * a.tok);
+            const int row = frag_row(a, f, w.h), count = frag_count(row);
+            load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
+            armed_k |= 1u << st;
+            k_ph = (k_ph & ~(1u << st)) | (ph << st);
+            ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
+            armed_v |= 1u << st;
+            v_ph = (v_ph & ~(1u << st)) | (ph << st);
+            if (++st == S) {
+                st = 0;
+                ph ^= 1;
             }
-            const int j1 = w.j1;
-            for (int j = w.j0; j < j1; j++) {
-                const int count = frag_count(row);
-                ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
-                armed_k |= 1u << st;
-                k_ph = (k_ph & ~(1u << st)) | (ph << st);
-                // the next tile's pages, while the value stage drains
-                const int row_next = j + 1 < j1 ? frag_row(a, w, j + 1, lane) : -1;
-                ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
-                armed_v |= 1u << st;
-                v_ph = (v_ph & ~(1u << st)) | (ph << st);
-                row = row_next;
-                if (++st == S) {
-                    st = 0;
-                    ph ^= 1;
-                }
-            }
-            seg++;
-            if (!ok || !w.next(a, item_tok)) break;
-            row = frag_row(a, w, w.j0, lane);
-        } while (true);
+            w = ahead;
+            j = j_next;
+            f = f_next;
+        }
         if (lane == 0) {
             // drain our own loads (a no-op when every load was consumed)
             const uint64_t t0 = tc::globaltimer();
@@ -199,8 +206,6 @@ __global__ void __launch_bounds__(384, 1)
                 while (!tc::mbar_try_wait(bar, par) && tc::globaltimer() - t0 < kWaitBudgetNs) {
                 }
             };
-            // (the last segment whose Q was loaded: seg - 1, or seg when its
-            // key loop was left early, which seg++ has counted too)
             if (seg > 0) drain_wait(q_full, (seg - 1) & 1);
             for (int i = 0; i < S; i++) {
                 if (armed_k >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);

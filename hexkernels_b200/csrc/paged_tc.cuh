@@ -185,14 +185,26 @@ __device__ __forceinline__ void note_parts(const PagedTc &a, const PlanShared &s
 
 // ---- one warp: the page loads of a key tile ----
 
-// Lane f's fragment of tile j: the row of the cache where it starts, or -1
-// when no cached token lies in it.
-__device__ __forceinline__ int frag_row(const PagedTc &a, const Walk &w, int j, int lane) {
+// Lane f's fragment of tile j of the walk's sequence: its first token (-1 when
+// no cached token lies in it) and its page as the table has it.  The page is
+// fetched a tile ahead and only looked at in frag_row, so that the warp does
+// not wait for it.
+struct Frag {
+    int token, page;
+};
+__device__ __forceinline__ Frag frag_of(const PagedTc &a, const Walk &w, int j, int lane) {
     const int t = j * kKeys + lane * a.frag;
-    if (lane * a.frag >= kKeys || t >= w.kv_len) return -1;
-    const int i = t / a.s.page_size;
-    const int page = seq_page(a.s, w.b, i);
-    return page < 0 ? a.map_rows : (page * a.kv_heads + w.h) * a.s.page_size + (t - i * a.s.page_size);
+    if (lane * a.frag >= kKeys || t >= w.kv_len) return Frag{-1, 0};
+    return Frag{t, a.s.table[(int64_t)w.b * a.s.max_pages + t / a.s.page_size]};
+}
+// The row of the cache where the fragment starts: one behind the last (the
+// load then gives zeros) when the table names no page.
+__device__ __forceinline__ int frag_row(const PagedTc &a, const Frag &f, int h) {
+    if (f.token < 0) return -1;
+    if (f.page >= 0 && f.page < a.s.num_pages)
+        return (f.page * a.kv_heads + h) * a.s.page_size + f.token % a.s.page_size;
+    flag_index(a.s.err_word);
+    return a.map_rows;
 }
 // Fragments that hold cached tokens (the lanes with a row).
 __device__ __forceinline__ int frag_count(int row) {

@@ -31,15 +31,13 @@ struct NormRope {
     int *err_word;
 };
 
-// Position and slot of a token; false for a token that is skipped (padding,
-// or an index out of range, which is flagged).
-__device__ __forceinline__ bool token_place(const NormRope &a, int t, int &pos, int64_t &page,
+// Where a token of this position and slot goes; false for one that is skipped
+// (padding, or an index out of range, which is flagged).
+__device__ __forceinline__ bool token_place(const NormRope &a, int pos, int slot, int64_t &page,
                                             int &off) {
-    pos = a.rot > 0 ? a.positions[t] : 0;
     page = 0;
     off = 0;
     if (a.slots) {
-        const int slot = a.slots[t];
         if (slot < 0) return false;
         page = slot / a.page_size;
         off = slot % a.page_size;
@@ -94,38 +92,48 @@ __device__ __forceinline__ uint2 narrow(const float (&x)[4]) {
 // 8c.. and 8c + 4.. otherwise; in both the lane's four pairs are 4c .. 4c + 3.
 // `ysplit` blocks share a token when tokens are few.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRope a, int ysplit) {
+__global__ void __launch_bounds__(256, 4) norm_rope_kernel(const NormRope a, int ysplit) {
     constexpr int kRows = 256 / LPR, U = 4;
     const int c = threadIdx.x % LPR, slot = threadIdx.x / LPR;
     const int per_token = a.heads + a.kv_heads * (a.v ? 2 : 1);
     const bool in_row = c * 8 < a.dim, turns = c * 8 < a.rot;
     const int o0 = turns && a.halves ? 4 * c : 8 * c;
     const int o1 = turns && a.halves ? a.rot / 2 + 4 * c : 8 * c + 4;
-    auto gain_of = [&](const void *g, float (&x)[4], float (&y)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = y[i] = 1.0f;
+    // the gains of this lane's columns, as they are stored
+    uint2 gq0, gq1, gk0, gk1;
+    const uint2 ones = make_uint2(pack2<T>(1.0f, 1.0f), pack2<T>(1.0f, 1.0f));
+    auto gain_of = [&](const void *g, uint2 &x, uint2 &y) {
+        x = y = ones;
         if (g && a.norm && in_row) {
-            widen<T>(*reinterpret_cast<const uint2 *>((const T *)g + o0), x);
-            widen<T>(*reinterpret_cast<const uint2 *>((const T *)g + o1), y);
+            x = *reinterpret_cast<const uint2 *>((const T *)g + o0);
+            y = *reinterpret_cast<const uint2 *>((const T *)g + o1);
         }
     };
-    float gq0[4], gq1[4], gk0[4], gk1[4];
     gain_of(a.q_gain, gq0, gq1);
     gain_of(a.k_gain, gk0, gk1);
     const float inv_dim = 1.0f / (float)a.dim;
     const int64_t items = (int64_t)a.tokens * ysplit;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int step = kRows * ysplit;
+    // a token's position and slot, fetched while the token before it is worked on
+    auto fetch = [&](int64_t item, int &pos, int &at) {
         const int t = (int)(item / ysplit);
-        int pos, off;
+        pos = a.rot > 0 ? a.positions[t] : 0;
+        at = a.slots ? a.slots[t] : 0;
+    };
+    int pos_next = 0, slot_next = 0;
+    if ((int64_t)blockIdx.x < items) fetch(blockIdx.x, pos_next, slot_next);
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int t = (int)(item / ysplit), pos = pos_next, at = slot_next;
+        if (item + gridDim.x < items) fetch(item + gridDim.x, pos_next, slot_next);
         int64_t page;
-        if (!token_place(a, t, pos, page, off)) continue;
+        int off;
+        if (!token_place(a, pos, at, page, off)) continue;
         float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (turns) {
             cs = *reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * (a.rot / 2) + 4 * c);
             sn = *reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * (a.rot / 2) + 4 * c);
         }
         const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
-        const int step = kRows * ysplit;
         // (rows of one warp may end at different passes; all lanes stay for the shuffles)
         for (int r0 = (int)(item % ysplit) * kRows; r0 < per_token; r0 += U * step) {
             uint2 w0[U], w1[U];
@@ -159,10 +167,13 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const NormRope a, int ys
                 T *dst = row_target<T>(a, t, r, page, off);
                 if (r < a.heads + a.kv_heads) {
                     const bool is_q = r < a.heads;
+                    float g0[4], g1[4];
+                    widen<T>(is_q ? gq0 : gk0, g0);
+                    widen<T>(is_q ? gq1 : gk1, g1);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        x[i] *= inv * (is_q ? gq0[i] : gk0[i]);
-                        y[i] *= inv * (is_q ? gq1[i] : gk1[i]);
+                        x[i] *= inv * g0[i];
+                        y[i] *= inv * g1[i];
                     }
                     if (a.halves) {
 #pragma unroll
@@ -204,9 +215,10 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRope a) {
     float *x = rows[warp];
     for (int64_t w = (int64_t)blockIdx.x * 8 + warp; w < n; w += (int64_t)gridDim.x * 8) {
         const int t = (int)(w / per_token), r = (int)(w % per_token);
-        int pos, off;
+        const int pos = a.rot > 0 ? a.positions[t] : 0;
+        int off;
         int64_t page;
-        if (!token_place(a, t, pos, page, off)) continue;
+        if (!token_place(a, pos, a.slots ? a.slots[t] : 0, page, off)) continue;
         const T *src = row_source<T>(a, t, r);
         T *dst = row_target<T>(a, t, r, page, off);
         if (r >= a.heads + a.kv_heads) {
