@@ -17,8 +17,9 @@
 // over the threads once per item.
 //
 // Per CTA (one per SM), 384 threads: warps 0 and 3 TMA of keys and of values,
-// one lane per page fragment; warp 1 tensor memory and MMA issue, S^T of the
-// next tile before P V of this one; two softmax warpgroups, one for each half
+// one lane per page fragment; warps 1 and 2 issue the MMAs of S^T and of O^T
+// (two warps, because one thread's waits and issues, some 90 cycles each, added
+// up to more than the tile's loads); two softmax warpgroups, one for each half
 // of the rows, which know nothing of one another.  Key and value tiles of 128 tokens go through rings of 3 stages
 // (dim 128; 6 at dim 64), 192 KB of loads in flight per SM.
 //
@@ -44,8 +45,8 @@ struct DecSmem {
     static constexpr int kPlan = kRed + 5 * N * 4;
     static constexpr int kBar = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;
     // q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2],
-    // o_free, drain, k_full, k_empty, v_full, v_empty [stages]
-    static constexpr int kNumBars = 14 + 4 * kStages;
+    // o_free, drain[2], k_full, k_empty, v_full, v_empty [stages]
+    static constexpr int kNumBars = 15 + 4 * kStages;
     static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
 };
 
@@ -105,6 +106,14 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&r
     tc::tmem_st_wait();
 }
 
+// Waits (bounded) for every MMA that this thread has issued.
+__device__ __forceinline__ void mma_drain(uint64_t *bar) {
+    tc::mma_commit(bar);
+    const uint64_t t0 = tc::globaltimer();
+    while (!tc::mbar_try_wait(bar, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+    }
+}
+
 template <typename T, int D, int N>
 __global__ void __launch_bounds__(384, 1)
     paged_dec_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -118,7 +127,7 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_empty = bars + 6;
     uint64_t *p_full = bars + 8, *pv_done = bars + 10, *o_free = bars + 12, *drain = bars + 13;
-    uint64_t *k_full = bars + 14, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+    uint64_t *k_full = bars + 15, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
@@ -136,7 +145,8 @@ __global__ void __launch_bounds__(384, 1)
             tc::mbar_init(&pv_done[i], 1);
         }
         tc::mbar_init(o_free, 8);
-        tc::mbar_init(drain, 1);
+        tc::mbar_init(&drain[0], 1);
+        tc::mbar_init(&drain[1], 1);
         for (int i = 0; i < S; i++) {
             tc::mbar_init(&k_full[i], 1);
             tc::mbar_init(&k_empty[i], 1);
@@ -228,38 +238,13 @@ __global__ void __launch_bounds__(384, 1)
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            // ----------------------------------------------------------- MMA
-            constexpr uint32_t idesc_s = tc::idesc_f16_f32(kKeys, N, false, false, kBf16);
-            constexpr uint32_t idesc_o = tc::idesc_f16_f32(128, N, true, true, kBf16);
-            const uint32_t sK = tc::smem_u32(smem + L::kK), sV = tc::smem_u32(smem + L::kV);
-            const uint32_t sQ = tc::smem_u32(smem + L::kQ), sP = tc::smem_u32(smem + L::kP);
+            // -------------------------------------------------- MMA, S^T = K Q^T
+            constexpr uint32_t idesc = tc::idesc_f16_f32(kKeys, N, false, false, kBf16);
+            const uint32_t sK = tc::smem_u32(smem + L::kK), sQ = tc::smem_u32(smem + L::kQ);
             Walk w = plan.start;
             int seg = 0, st = 0;
             uint32_t ph = 0, g = 0;
-            bool ok = true, issued = false;
-            // the tile whose P V is still to be issued
-            bool pending = false, pend_first = false;
-            int pend_st = 0, pend_seg = 0;
-            uint32_t pend_ph = 0;
-            auto issue_pv = [&](uint32_t gp) {
-                const int buf = gp & 1;
-                ok = tc::mbar_wait(&v_full[pend_st], pend_ph, abort_flag, err_word, kErrWaitFull) &&
-                     tc::mbar_wait(&p_full[buf], (gp >> 1) & 1, abort_flag, err_word, kErrWaitFull) &&
-                     (!pend_first || tc::mbar_wait(o_free, (pend_seg & 1) ^ 1, abort_flag, err_word,
-                                                   kErrWaitAccum));
-                if (!ok) return;
-                tc::tc_fence_after();
-                const uint32_t vb = sV + pend_st * L::kTile, pb = sP + buf * (kKeys * N * 2);
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; k++)
-                    // (dim 64: the second 64 of the 128 rows repeat the first, unread)
-                    tc::mma_ss<tc::MmaKind::F16>(
-                        tmem_o, tc::sdesc_mnmajor_sw128(vb + k * 2048, D == 128 ? kSubTile : 0, 1024),
-                        tc::sdesc_mnmajor_narrow<N * 2>(pb + k * 16 * N * 2), idesc_o,
-                        (!pend_first || k > 0) ? 1u : 0u);
-                tc::mma_commit(&v_empty[pend_st]);
-                tc::mma_commit(&pv_done[buf]);
-            };
+            bool ok = true;
             do {
                 const int qb = seg & 1;
                 ok = tc::mbar_wait(&q_full[qb], (seg >> 1) & 1, abort_flag, err_word, kErrWaitFull);
@@ -276,18 +261,11 @@ __global__ void __launch_bounds__(384, 1)
                         tc::mma_ss<tc::MmaKind::F16>(
                             tmem_base + buf * N,
                             tc::sdesc_kmajor_sw128(kb + (k >> 2) * kSubTile + (k & 3) * 32),
-                            tc::sdesc_kmajor_sw128(qt + (k >> 2) * (N * 128) + (k & 3) * 32), idesc_s,
+                            tc::sdesc_kmajor_sw128(qt + (k >> 2) * (N * 128) + (k & 3) * 32), idesc,
                             k > 0 ? 1u : 0u);
-                    issued = true;
                     tc::mma_commit(&k_empty[st]);
                     tc::mma_commit(&s_full[buf]);
                     if (j == w.j1 - 1) tc::mma_commit(&q_empty[qb]);
-                    if (pending) issue_pv(g - 1);
-                    pending = true;
-                    pend_first = j == w.j0;
-                    pend_st = st;
-                    pend_ph = ph;
-                    pend_seg = seg;
                     if (++st == S) {
                         st = 0;
                         ph ^= 1;
@@ -295,13 +273,45 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 seg++;
             } while (ok && w.next(a, a.tok));
-            if (ok && pending) issue_pv(g - 1);
-            if (issued) {
-                tc::mma_commit(drain);
-                const uint64_t t0 = tc::globaltimer();
-                while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+            mma_drain(&drain[0]);
+        }
+    } else if (warp == 2) {
+        if (lane == 0) {
+            // ------------------------------------------------ MMA, O^T += V^T P^T
+            constexpr uint32_t idesc = tc::idesc_f16_f32(128, N, true, true, kBf16);
+            const uint32_t sV = tc::smem_u32(smem + L::kV), sP = tc::smem_u32(smem + L::kP);
+            Walk w = plan.start;
+            int seg = 0, st = 0;
+            uint32_t ph = 0, g = 0;
+            bool ok = true;
+            do {
+                for (int j = w.j0; j < w.j1 && ok; j++, g++) {
+                    const int buf = g & 1;
+                    const bool first = j == w.j0;
+                    ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
+                         (!first || tc::mbar_wait(o_free, (seg & 1) ^ 1, abort_flag, err_word,
+                                                  kErrWaitAccum)) &&
+                         tc::mbar_wait(&p_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitFull);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t vb = sV + st * L::kTile, pb = sP + buf * (kKeys * N * 2);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; k++)
+                        // (dim 64: the second 64 of the 128 rows repeat the first, unread)
+                        tc::mma_ss<tc::MmaKind::F16>(
+                            tmem_o, tc::sdesc_mnmajor_sw128(vb + k * 2048, D == 128 ? kSubTile : 0, 1024),
+                            tc::sdesc_mnmajor_narrow<N * 2>(pb + k * 16 * N * 2), idesc,
+                            (!first || k > 0) ? 1u : 0u);
+                    tc::mma_commit(&v_empty[st]);
+                    tc::mma_commit(&pv_done[buf]);
+                    if (++st == S) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
-            }
+                seg++;
+            } while (ok && w.next(a, a.tok));
+            mma_drain(&drain[1]);
         }
     } else if (warp >= 4) {
         // ----------------------------------------------------------- softmax
