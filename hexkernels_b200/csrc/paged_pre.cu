@@ -7,19 +7,26 @@
 // heads that share a key head also share its key and value loads (rows past
 // tok * group are computed and dropped).  One softmax warpgroup per tile, one
 // query row per thread, so the tensor pipe works for one tile while the other
-// tile's warpgroup takes its exponentials; the order of the MMAs, the
-// two-halves hand-over of P and the lazy reference maximum are those of the
-// dense ping-pong kernel (attn_tc.cu).  New here are the loads (a key tile is
-// gathered page by page, one lane of the TMA warp per fragment), the ragged
-// batch (paged_tc.cuh: every CTA gets the same number of key tiles; an item
-// that is cut leaves partial results), and the values behind the last cached
-// token, which are zeroed before they meet a weight of zero.
+// tile's warpgroup takes its exponentials; P is handed over in two halves and
+// the reference maximum is lazy, as in the dense ping-pong kernel (attn_tc.cu).
+// An item of one tile (at most 128 rows) would leave one warpgroup idle: there
+// both take the key tiles in turn, each with a reference, a sum and an output
+// of its own, and the first joins the two outputs, which lie side by side in
+// tensor memory.
 //
-// Per CTA (one per SM), 384 threads in three warpgroups: warp 0 TMA, warp 1
-// tensor memory and MMA issue; warpgroups 1 and 2 softmax of tiles a and b.
-// TMEM: S_a [0,128), S_b [128,256), O_a [256,..), O_b [384,..); P_x over S_x.
+// A key tile is gathered page by page, one lane of a TMA warp per fragment.
+// Values behind the last cached token are zeroed before they meet a weight of
+// zero.  The batch is split evenly over the CTAs (paged_tc.cuh).
 //
-// Every wait is bounded; see mbar_wait.
+// Per CTA (one per SM), 384 threads in three warpgroups: warps 0 and 3 TMA of
+// keys (and queries) and of values, warps 1 and 2 the MMAs of tiles a and b
+// (one warp for both left the tensor pipe idle for the 90 cycles of each of its
+// waits), warpgroups 1 and 2 softmax of tiles a and b.
+// TMEM: S_a [0,128), S_b [128,256), then O_a, O_b.  Dim 128: P_x over S_x, so
+// S of the next key tile follows P V of this one.  Dim 64 has room for P beside
+// S, so S of the next key tile is ready when the softmax asks for it.
+//
+// Every wait is bounded; see wait_phase.
 #include <math.h>
 
 #include "paged_tc.cuh"
@@ -44,10 +51,12 @@ struct PreSmem {
     static constexpr int kV = kK + kStages * kTile;
     static constexpr int kPlan = kV + kStages * kTile;
     static constexpr int kWalk = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;   // a Walk per softmax warp
-    static constexpr int kBar = (kWalk + 8 * (int)sizeof(Walk) + 15) / 16 * 16;
-    // q_full, q_empty, s_full[2], p_full[2], p_half[2], pv_done[2], o_free[2],
-    // drain, k_full, k_empty, v_full, v_empty [stages]
-    static constexpr int kNumBars = 13 + 4 * kStages;
+    static constexpr int kMl = (kWalk + 8 * (int)sizeof(Walk) + 15) / 16 * 16;       // [128][2]: tile b's, to be joined
+    static constexpr int kTurn = kMl + 128 * 8;            // [2][4] key tiles that a softmax warp is done with
+    static constexpr int kBar = kTurn + 32;
+    // q_full, q_empty, s_full[2], s_empty[2], p_full[2], p_half[2], pv_done[2],
+    // o_free[2], joined, drain[2], k_full, k_empty, v_full, v_empty [stages]
+    static constexpr int kNumBars = 17 + 4 * kStages;
     static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
 };
 
@@ -75,13 +84,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Tile x of segment w: its first token, its tokens, and the end of its key
-// tiles in the segment (j0 when it has none).
-__device__ __forceinline__ void tile_span(const PagedTc &a, const Walk &w, int x, int &t0, int &ntok,
-                                          int &hi) {
-    t0 = (2 * w.rt + x) * a.tok;
-    ntok = min(a.tok, w.q_len - t0);
-    hi = ntok > 0 ? max(w.j0, min(w.j1, tiles_to(a.s, w.kv_len, w.q_len, t0 + a.tok))) : w.j0;
+// What tile x does in segment w: its first token and number of tokens, and its
+// key tiles start, start + step, .. < end.  `alt`: the item has one tile, whose
+// key tiles the two sides take in turn.
+struct Span {
+    int t0, ntok, start, end, step;
+    bool alt;
+    __device__ __forceinline__ int count() const {
+        return start < end ? (end - start + step - 1) / step : 0;
+    }
+};
+__device__ __forceinline__ Span span_of(const PagedTc &a, const Walk &w, int x) {
+    Span s;
+    s.alt = w.q_len <= (2 * w.rt + 1) * a.tok;
+    s.t0 = (2 * w.rt + (s.alt ? 0 : x)) * a.tok;
+    s.ntok = min(a.tok, w.q_len - s.t0);
+    s.start = w.j0 + (s.alt ? x : 0);
+    s.step = s.alt ? 2 : 1;
+    s.end = s.alt ? w.j1 : min(w.j1, tiles_to(a.s, w.kv_len, w.q_len, s.t0 + a.tok));
+    return s;
 }
 
 template <typename T, int D>
@@ -95,9 +116,10 @@ __global__ void __launch_bounds__(384, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4;
-    uint64_t *p_half = bars + 6, *pv_done = bars + 8, *o_free = bars + 10, *drain = bars + 12;
-    uint64_t *k_full = bars + 13, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4;
+    uint64_t *p_full = bars + 6, *p_half = bars + 8, *pv_done = bars + 10, *o_free = bars + 12;
+    uint64_t *joined = bars + 14, *drain = bars + 15;
+    uint64_t *k_full = bars + 17, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
@@ -107,23 +129,29 @@ __global__ void __launch_bounds__(384, 1)
     tc::launch_dependents();
 
     if (threadIdx.x == 0) {
+        // (both sides hand every query, key and value tile back, also one that
+        // they do not use: a side that skipped some could not tell a later
+        // phase of the same parity from the one it waits for)
         tc::mbar_init(q_full, 1);
-        tc::mbar_init(q_empty, 1);
+        tc::mbar_init(q_empty, 2);
         for (int x = 0; x < 2; x++) {
             tc::mbar_init(&s_full[x], 1);
+            tc::mbar_init(&s_empty[x], 4);
             tc::mbar_init(&p_full[x], 4);
             tc::mbar_init(&p_half[x], 4);
             tc::mbar_init(&pv_done[x], 1);
             tc::mbar_init(&o_free[x], 4);
+            tc::mbar_init(&drain[x], 1);
         }
-        tc::mbar_init(drain, 1);
+        tc::mbar_init(joined, 4);
         for (int i = 0; i < S; i++) {
             tc::mbar_init(&k_full[i], 1);
-            tc::mbar_init(&k_empty[i], 1);
+            tc::mbar_init(&k_empty[i], 2);
             tc::mbar_init(&v_full[i], 1);
-            tc::mbar_init(&v_empty[i], 1);
+            tc::mbar_init(&v_empty[i], 2);
         }
         *abort_flag = 0;
+        for (int i = 0; i < 8; i++) reinterpret_cast<uint32_t *>(smem + L::kTurn)[i] = 0;
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmQ);
         tc::tma_prefetch_desc(&tmK);
@@ -137,67 +165,61 @@ __global__ void __launch_bounds__(384, 1)
     const bool any = plan_run<384>(a, item_tok, plan);
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    constexpr bool kOwnP = D == 64;         // P beside S, not over it
+    constexpr uint32_t kColO = 256, kColP = kOwnP ? 384 : 0, kStepP = kOwnP ? 64 : 128;
 
     if (warp < 4) {
       // warpgroup 0: one setmaxnreg for all four warps, then the roles
       tc::setmaxnreg_dec<kRegsCtl>();
       if (!any) {
         // nothing to do but free the tensor memory
-      } else if (warp == 0) {
-        // --------------------------------------------------------------- TMA
+      } else if (warp == 0 || warp == 3) {
+        // ------------------------------------- TMA: keys and queries, values
+        const bool keys = warp == 0;
+        uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+        const CUtensorMap *map = keys ? &tmK : &tmV;
+        uint8_t *ring = smem + (keys ? L::kK : L::kV);
         Walk w = plan.start;
         int seg = 0, st = 0;
-        uint32_t ph = 0, armed_k = 0, armed_v = 0, k_ph = 0, v_ph = 0;
+        uint32_t ph = 0, armed = 0, last_ph = 0;
         bool ok = true, more = true;
         int j = w.j0;
         Frag f = frag_of(a, w, j, lane);
         while (more) {
-            // the tile after this one, and its pages
-            Walk ahead = w;
-            int j_next = j + 1;
-            if (j_next == w.j1) {
-                more = ahead.next(a, item_tok);
-                j_next = ahead.j0;
-            }
-            Frag f_next = f;
-            if (more) f_next = frag_of(a, ahead, j_next, lane);
-            if (j == w.j0) {
-                int t0, ntok_a, ntok_b, hi;
-                tile_span(a, w, 1, t0, ntok_b, hi);
-                tile_span(a, w, 0, t0, ntok_a, hi);
-                ok = tc::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            if (j == w.j0 && keys) {
+                const Span sa = span_of(a, w, 0);
+                ok = wait_phase(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) {
-                    const int tiles = ntok_b > 0 ? 2 : 1;
+                    const int tiles = sa.alt ? 1 : 2;
                     tc::mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * a.tok * a.group * 128 * kSubs));
                     for (int x = 0; x < tiles; x++)
                         for (int c = 0; c < kSubs; c++)
                             tc::tma_load_3d(smem + L::kQ + x * L::kTile + c * kSubTile, &tmQ, q_full,
-                                            c * 64, w.h * a.group, w.first + t0 + x * a.tok);
+                                            c * 64, w.h * a.group, w.first + sa.t0 + x * a.tok);
                 }
                 seg++;
             }
-            ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            const Frag f_now = f;
+            const int h = w.h;
+            // the tile after this one, and its pages
+            if (++j == w.j1) {
+                more = w.next(a, item_tok);
+                j = w.j0;
+            }
+            if (more) f = frag_of(a, w, j, lane);
+            ok = wait_phase(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int row = frag_row(a, f, w.h), count = frag_count(row);
-            load_frags<kSubs>(a, smem + L::kK + st * L::kTile, &tmK, &k_full[st], row, count, lane);
-            armed_k |= 1u << st;
-            k_ph = (k_ph & ~(1u << st)) | (ph << st);
-            ok = tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            load_frags<kSubs>(a, smem + L::kV + st * L::kTile, &tmV, &v_full[st], row, count, lane);
-            armed_v |= 1u << st;
-            v_ph = (v_ph & ~(1u << st)) | (ph << st);
+            const int row = frag_row(a, f_now, h), count = frag_count(row);
+            load_frags<kSubs>(a, ring + st * L::kTile, map, &full[st], row, count, lane);
+            armed |= 1u << st;
+            last_ph = (last_ph & ~(1u << st)) | (ph << st);
             if (++st == S) {
                 st = 0;
                 ph ^= 1;
             }
-            w = ahead;
-            j = j_next;
-            f = f_next;
         }
         if (lane == 0) {
             // drain our own loads (a no-op when every load was consumed)
@@ -207,116 +229,114 @@ __global__ void __launch_bounds__(384, 1)
                 }
             };
             if (seg > 0) drain_wait(q_full, (seg - 1) & 1);
-            for (int i = 0; i < S; i++) {
-                if (armed_k >> i & 1) drain_wait(&k_full[i], k_ph >> i & 1);
-                if (armed_v >> i & 1) drain_wait(&v_full[i], v_ph >> i & 1);
-            }
+            for (int i = 0; i < S; i++)
+                if (armed >> i & 1) drain_wait(&full[i], last_ph >> i & 1);
         }
-      } else if (warp == 1) {
+      } else {
         if (lane == 0) {
-            // ----------------------------------------------------------- MMA
+            // ------------------------------------------------- MMA of tile x
+            const int x = warp - 1;
             constexpr uint32_t idesc_s = tc::idesc_f16_f32(128, kKeys, false, false, kBf16);
             constexpr uint32_t idesc_o = tc::idesc_f16_f32(128, D, true, false, kBf16);
             const uint32_t sQ = tc::smem_u32(smem + L::kQ);
             const uint32_t sK = tc::smem_u32(smem + L::kK);
             const uint32_t sV = tc::smem_u32(smem + L::kV);
+            const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + kColO + x * D;
+            const uint32_t t_p = tmem_base + kColP + x * kStepP;
             Walk w = plan.start;
-            int seg = 0, st = 0;
-            uint32_t ph = 0;
-            uint32_t n[2] = {0, 0}, segs[2] = {0, 0};    // key tiles and segments of each tile so far
-            bool issued = false, ok = true;
-            auto issue_s = [&](int x, int stage) {
-                const uint32_t kb = sK + stage * L::kTile, qb = sQ + x * L::kTile;
-#pragma unroll
-                for (int k = 0; k < D / 16; k++) {
-                    const uint32_t off = (k >> 2) * kSubTile + (k & 3) * 32;
-                    tc::mma_ss<tc::MmaKind::F16>(tmem_base + x * 128, tc::sdesc_kmajor_sw128(qb + off),
-                                                 tc::sdesc_kmajor_sw128(kb + off), idesc_s,
-                                                 k > 0 ? 1u : 0u);
-                }
-                tc::mma_commit(&s_full[x]);
-                issued = true;
+            int seg = 0, g0 = 0;                 // segments; key tiles of the earlier ones
+            int k_pos = 0, v_pos = 0;            // key and value tiles handed back
+            uint32_t n = 0, segs = 0;            // key tiles and segments of this side so far
+            bool ok = true;
+            auto wait_full = [&](uint64_t *full, int gk) {
+                return wait_phase(&full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
             };
-            // O_x += P_x V for the keys of K steps k0 .. k0+3 (64 keys)
-            auto issue_pv = [&](int x, int stage, bool first, int k0) {
-                const uint32_t vb = sV + stage * L::kTile;
-#pragma unroll
-                for (int k = k0; k < k0 + 4; k++)
-                    tc::mma_ts_f16(tmem_base + 256 + x * 128, tmem_base + x * 128 + k * 8,
-                                   tc::sdesc_mnmajor_sw128(vb + k * 2048, kSubTile, 1024), idesc_o,
-                                   (!first || k > 0) ? 1u : 0u);
+            // tiles that this side does not use
+            auto pass = [&](uint64_t *full, uint64_t *empty, int &pos, int upto) {
+                for (; pos < upto && ok; pos++) {
+                    ok = wait_full(full, pos);
+                    if (ok) tc::mbar_arrive(&empty[pos % S]);
+                }
             };
             do {
-                int t0, ntok, hi[2];
-                tile_span(a, w, 0, t0, ntok, hi[0]);
-                tile_span(a, w, 1, t0, ntok, hi[1]);
-                const int j0 = w.j0, j1 = w.j1;
-                ok = tc::mbar_wait(q_full, seg & 1, abort_flag, err_word, kErrWaitFull) &&
-                     tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
-                if (!ok) break;
-                tc::tc_fence_after();
-                for (int x = 0; x < 2; x++)
-                    if (hi[x] > j0) issue_s(x, st);
-                tc::mma_commit(&k_empty[st]);
-                if (j1 - j0 == 1) tc::mma_commit(q_empty);
-                for (int j = j0; j < j1 && ok; j++) {
-                    ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
-                    int st_next = st + 1;
-                    uint32_t ph_next = ph;
-                    if (st_next == S) {
-                        st_next = 0;
-                        ph_next ^= 1;
+                const Span s = span_of(a, w, x);
+                const uint32_t qb = sQ + (s.alt ? 0 : x * L::kTile);
+                const int g1 = g0 + (w.j1 - w.j0);
+                auto issue_s = [&](int j) {
+                    const int gk = g0 + (j - w.j0), st = gk % S;
+                    pass(k_full, k_empty, k_pos, gk);
+                    ok = ok && wait_full(k_full, gk);
+                    if (!ok) return;
+                    tc::tc_fence_after();
+                    const uint32_t kb = sK + st * L::kTile;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t off = (k >> 2) * kSubTile + (k & 3) * 32;
+                        tc::mma_ss<tc::MmaKind::F16>(t_s, tc::sdesc_kmajor_sw128(qb + off),
+                                                     tc::sdesc_kmajor_sw128(kb + off), idesc_s,
+                                                     k > 0 ? 1u : 0u);
                     }
-                    // the last tile that takes this stage, and the next one's
-                    const int last = j < hi[1] ? 1 : 0, last_next = j + 1 < hi[1] ? 1 : 0;
-                    bool k_ready = false;
-                    for (int x = 0; x < 2 && ok; x++) {
-                        if (j >= hi[x]) continue;
-                        const uint32_t c = n[x] + (j - j0);
-                        // the first 64 keys' P V runs while the softmax warps
-                        // still compute the other half of P
-                        ok = tc::mbar_wait(&p_half[x], c & 1, abort_flag, err_word, kErrWaitFull) &&
-                             (j > j0 || tc::mbar_wait(&o_free[x], (segs[x] & 1) ^ 1, abort_flag,
-                                                      err_word, kErrWaitAccum));
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        issue_pv(x, st, j == j0, 0);
-                        ok = tc::mbar_wait(&p_full[x], c & 1, abort_flag, err_word, kErrWaitFull);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        issue_pv(x, st, false, 4);
-                        tc::mma_commit(&pv_done[x]);
-                        if (x == last) tc::mma_commit(&v_empty[st]);
-                        if (j + 1 < hi[x]) {
-                            if (!k_ready) {
-                                ok = tc::mbar_wait(&k_full[st_next], ph_next, abort_flag, err_word,
-                                                   kErrWaitFull);
-                                if (!ok) break;
-                                tc::tc_fence_after();
-                                k_ready = true;
-                            }
-                            issue_s(x, st_next);
-                            if (x == last_next) {
-                                tc::mma_commit(&k_empty[st_next]);
-                                if (j + 1 == j1 - 1) tc::mma_commit(q_empty);
-                            }
+                    tc::mma_commit(&s_full[x]);
+                    tc::mma_commit(&k_empty[st]);
+                    k_pos = gk + 1;
+                    if (j + s.step >= s.end) tc::mma_commit(q_empty);
+                    // the other side's tile, so that its stage is not held up
+                    if (s.alt) pass(k_full, k_empty, k_pos, min(gk + 2, g1));
+                };
+                // O_x += P_x V for the keys of K steps k0 .. k0+3 (64 keys)
+                auto issue_pv = [&](int st, bool first, int k0) {
+                    const uint32_t vb = sV + st * L::kTile;
+#pragma unroll
+                    for (int k = k0; k < k0 + 4; k++)
+                        tc::mma_ts_f16(t_o, t_p + k * 8,
+                                       tc::sdesc_mnmajor_sw128(vb + k * 2048, kSubTile, 1024), idesc_o,
+                                       (!first || k > 0) ? 1u : 0u);
+                };
+                ok = wait_phase(q_full, seg & 1, abort_flag, err_word, kErrWaitFull);
+                if (s.start < s.end) {
+                    // (S_x of the last segment has been read: its softmax handed P over,
+                    // and with P beside S also S itself)
+                    if (ok && kOwnP && n > 0)
+                        ok = wait_phase(&s_empty[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    if (ok) issue_s(s.start);
+                    for (int j = s.start; j < s.end && ok; j += s.step, n++) {
+                        const int gk = g0 + (j - w.j0), st = gk % S;
+                        const bool first = j == s.start;
+                        if (kOwnP && j + s.step < s.end) {
+                            ok = wait_phase(&s_empty[x], n & 1, abort_flag, err_word, kErrWaitAccum);
+                            if (ok) issue_s(j + s.step);
                         }
+                        pass(v_full, v_empty, v_pos, gk);
+                        ok = ok && wait_full(v_full, gk) &&
+                             (!first || wait_phase(&o_free[x], (segs & 1) ^ 1, abort_flag, err_word,
+                                                      kErrWaitAccum)) &&
+                             // the first 64 keys' P V runs while the softmax warps
+                             // still compute the other half of P
+                             wait_phase(&p_half[x], n & 1, abort_flag, err_word, kErrWaitFull);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_pv(st, first, 0);
+                        ok = wait_phase(&p_full[x], n & 1, abort_flag, err_word, kErrWaitFull);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        issue_pv(st, false, 4);
+                        tc::mma_commit(&pv_done[x]);
+                        tc::mma_commit(&v_empty[st]);
+                        v_pos = gk + 1;
+                        if (!kOwnP && j + s.step < s.end) issue_s(j + s.step);
                     }
-                    st = st_next;
-                    ph = ph_next;
+                    segs++;
+                } else if (ok) {
+                    tc::mbar_arrive(q_empty);
                 }
-                for (int x = 0; x < 2; x++)
-                    if (hi[x] > j0) {
-                        n[x] += hi[x] - j0;
-                        segs[x]++;
-                    }
+                if (ok) pass(k_full, k_empty, k_pos, g1);
+                if (ok) pass(v_full, v_empty, v_pos, g1);
+                g0 = g1;
                 seg++;
             } while (ok && w.next(a, item_tok));
-            if (issued) {
-                tc::mma_commit(drain);
-                const uint64_t t0 = tc::globaltimer();
-                while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
-                }
+            tc::mma_commit(&drain[x]);
+            const uint64_t t0 = tc::globaltimer();
+            while (!tc::mbar_try_wait(&drain[x], 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
             }
         }
       }
@@ -328,26 +348,29 @@ __global__ void __launch_bounds__(384, 1)
         const int row = q * 32 + lane;
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_base + x * 128;
-        const uint32_t o_addr = tmem_base + lane_base + 256 + x * 128;
+        const uint32_t o_addr = tmem_base + lane_base + kColO + x * D;
+        const uint32_t p_addr = tmem_base + lane_base + kColP + x * kStepP;
+        volatile uint32_t *turn = reinterpret_cast<volatile uint32_t *>(smem + L::kTurn);
+        float2 *ml_b = reinterpret_cast<float2 *>(smem + L::kMl);
         Walk *wp = reinterpret_cast<Walk *>(smem + L::kWalk) + (warp - 4);
-        uint32_t n = 0;
+        uint32_t n = 0, n_other = 0, joins = 0;  // key tiles so far, of the other side; joined segments
         int g0 = 0;               // key tiles of the CTA's earlier segments (the value ring)
         bool more = any;
         if (any && lane == 0) *wp = plan.start;
         __syncwarp();
         while (more) {
-            int t0, ntok, hi, hi_a;
-            tile_span(a, *wp, 0, t0, ntok, hi_a);
-            tile_span(a, *wp, x, t0, ntok, hi);
+            const Span s = span_of(a, *wp, x);
             const int j0 = wp->j0, kv_len = wp->kv_len;
             const int tok_row = row / a.group;
-            const int lim = min(kv_len, seen_by(a.s, kv_len, wp->q_len, t0 + tok_row));
-            const int lim0 = min(kv_len, seen_by(a.s, kv_len, wp->q_len, t0));   // the tile's fewest
+            const int lim = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0 + tok_row));
+            const int lim0 = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0));   // the tile's fewest
+            const int count_other = span_of(a, *wp, x ^ 1).count();
+            const uint32_t n0 = n;
             float m_ref = -INFINITY, l = 0.0f;
             bool ok = true;
-            for (int j = j0; j < hi; j++) {
-                const uint32_t c = n + (j - j0);
-                ok = tc::mbar_wait(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
+            for (int j = s.start; j < s.end; j += s.step, n++) {
+                const uint32_t c = n;
+                ok = wait_phase(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
                 const int key0 = j * kKeys;
@@ -359,6 +382,11 @@ __global__ void __launch_bounds__(384, 1)
                 tc::reg_fence(sr[1]);
                 tc::reg_fence(sr[2]);
                 tc::reg_fence(sr[3]);
+                if (kOwnP) {
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s_empty[x]);
+                }
                 if (key0 + kKeys > lim0) {
                     const int rest = lim - key0;
 #pragma unroll
@@ -381,14 +409,14 @@ __global__ void __launch_bounds__(384, 1)
                                       fmaxf(mx[6], mx[7])) *
                                  a.scale_log2;
                 const float m_new = fmaxf(m_ref, mt);
-                if (j == j0) {
+                if (j == s.start) {
                     m_ref = m_new;
                 } else {
                     // Lazy rescale: the reference max moves only when the row
                     // max rose by more than 8 (P stays below 2^8 otherwise).
                     const bool need = m_new > m_ref + 8.0f;
                     if (__any_sync(0xffffffffu, need)) {
-                        ok = tc::mbar_wait(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
+                        ok = wait_phase(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
                                            kErrWaitAccum);
                         if (!__all_sync(0xffffffffu, ok)) break;
                         tc::tc_fence_after();
@@ -410,18 +438,41 @@ __global__ void __launch_bounds__(384, 1)
                         }
                     }
                 }
-                if (key0 + kKeys > kv_len && (x == 0 || j >= hi_a)) {
-                    // values behind the last cached token (the first tile to
-                    // take this stage clears them; its first half of P is taken
-                // when all four warps have handed it over)
+                if (kOwnP && c > 0) {
+                    // P's columns were last read by the P V of the tile before
+                    ok = wait_phase(&pv_done[x], (c - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    tc::tc_fence_after();
+                }
+                if (key0 + kKeys > kv_len) {
+                    // zeros in the values behind the last cached token, by each
+                    // side before it hands its P over (all four warps have then;
+                    // that the other side writes the same zeros does not matter)
                     const int gk = g0 + (j - j0);
-                    ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
+                    ok = wait_phase(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
                     if (!__all_sync(0xffffffffu, ok)) break;
                     clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, kv_len - key0);
                     tc::fence_proxy_async_smem();
                 }
+                // The sides take their exponentials in turn, a's i-th tile, b's i-th,
+                // a's next: while one has the MUFU unit the other has its MMAs, its
+                // loads and its maximum.  (A matter of time only: a wait that runs
+                // out goes on.)
+                {
+                    const int i = (int)(c - n0) - (x == 0 ? 1 : 0);
+                    if (i >= 0 && i < count_other) {
+                        const uint32_t target = n_other + i + 1;
+                        for (int polls = 0; polls < 2000; polls++) {
+                            const volatile uint32_t *v = turn + (x ^ 1) * 4;
+                            if ((int)(v[0] - target) >= 0 && (int)(v[1] - target) >= 0 &&
+                                (int)(v[2] - target) >= 0 && (int)(v[3] - target) >= 0)
+                                break;
+                        }
+                        __syncwarp();
+                    }
+                }
                 // P = 2^(s*scale*log2e - m_ref) from the registers, as 16-bit
-                // pairs over S columns 16cc..16cc+15; the row sum in four
+                // pairs in columns 16cc..16cc+15; the row sum in four
                 // packed pairs.  A row that sees nothing yet has no reference.
                 uint64_t acc2[4] = {0, 0, 0, 0};
                 const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
@@ -447,8 +498,9 @@ __global__ void __launch_bounds__(384, 1)
                         acc2[e & 3] = add_pair(acc2[e & 3], pair(p0, p1));
                         pk[e] = pack2<T>(p0, p1);
                     }
-                    tc::tmem_st_32x32b_x16(s_addr + cc * 16, pk);
+                    tc::tmem_st_32x32b_x16(p_addr + cc * 16, pk);
                 }
+                if (lane == 0) turn[x * 4 + q] = c + 1;
                 tc::tmem_st_wait();
                 {
                     float s0, s1, s2, s3, s4, s5, s6, s7;
@@ -464,22 +516,63 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (!__all_sync(0xffffffffu, ok)) break;
             // ---- end of the segment
-            const bool whole = j0 == 0 && wp->j1 == wp->nt;
-            const bool live = tok_row < ntok && row < a.tok * a.group;
-            const size_t prow = ((size_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0)) * kPartRows + x * 128 + row;
-            const int64_t orow = (int64_t)(wp->first + t0 + tok_row) * a.heads + wp->h * a.group +
-                                 row % a.group;
-            if (hi > j0) {
-                n += hi - j0;
-                ok = tc::mbar_wait(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+            const bool used = s.start < s.end;
+            if (used) {
+                ok = wait_phase(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            }
+            float m = m_ref, sum = l, w_own = 1.0f, w_b = 0.0f;
+            n_other += count_other;
+            bool write = true;
+            if (s.alt && wp->j1 - j0 > 1) {
+                if (x == 1) {
+                    // (the P V it waited for had waited for o_free: the last
+                    // segment's values have been read)
+                    ml_b[row] = make_float2(m_ref, l);
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(joined);
+                } else {
+                    ok = wait_phase(joined, joins & 1, abort_flag, err_word, kErrWaitOther) &&
+                         wait_phase(&pv_done[1], (n_other - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    tc::tc_fence_after();
+                    const float2 b = ml_b[row];
+                    m = fmaxf(m_ref, b.x);
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    w_own = tc::ex2(m_ref - ref);
+                    w_b = tc::ex2(b.x - ref);
+                    sum = l * w_own + b.y * w_b;
+                }
+                joins++;
+            }
+            if (s.alt && x == 1) write = false;
+            const bool whole = j0 == 0 && wp->j1 == wp->nt;
+            const bool live = tok_row < s.ntok && row < a.tok * a.group;
+            const size_t prow = ((size_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0)) * kPartRows + x * 128 + row;
+            const int64_t orow = (int64_t)(wp->first + s.t0 + tok_row) * a.heads + wp->h * a.group +
+                                 row % a.group;
+            if (write && used) {
+                const bool both = s.alt && wp->j1 - j0 > 1;
+                const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float f_own = w_own * inv, f_b = w_b * inv;
 #pragma unroll 1
                 for (int cc = 0; cc < D / 32; cc++) {
                     uint32_t o[32];
                     tc::tmem_ld_32x32b_x32(o_addr + cc * 32, o);
                     tc::tmem_ld_wait(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f_own);
+                    if (both) {
+                        uint32_t ob[32];
+                        tc::tmem_ld_32x32b_x32(o_addr + D + cc * 32, ob);
+                        tc::tmem_ld_wait(ob);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(ob[e]) * f_b);
+                    }
                     if (!live) continue;
                     if (whole) {
                         uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + orow * D +
@@ -489,8 +582,8 @@ __global__ void __launch_bounds__(384, 1)
                             uint32_t v[4];
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                v[i] = pack2<T>(__uint_as_float(o[8 * e + 2 * i]) * inv,
-                                                __uint_as_float(o[8 * e + 2 * i + 1]) * inv);
+                                v[i] = pack2<T>(__uint_as_float(o[8 * e + 2 * i]),
+                                                __uint_as_float(o[8 * e + 2 * i + 1]));
                             dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
                         }
                     } else {
@@ -502,13 +595,16 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&o_free[x]);
+                if (lane == 0) {
+                    tc::mbar_arrive(&o_free[x]);
+                    if (both) tc::mbar_arrive(&o_free[1]);
+                }
             }
-            if (live) {
+            if (live && write) {
                 if (!whole) {
-                    reinterpret_cast<float2 *>(a.part_ml)[prow] = make_float2(m_ref, l);
+                    reinterpret_cast<float2 *>(a.part_ml)[prow] = make_float2(m, sum);
                 } else if (a.lse) {
-                    a.lse[orow] = l == 0.0f ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
+                    a.lse[orow] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
                 }
             }
             g0 += wp->j1 - j0;
