@@ -23,7 +23,7 @@
 // of the rows, which know nothing of one another.  Key and value tiles of 128 tokens go through rings of 3 stages
 // (dim 128; 6 at dim 64), 192 KB of loads in flight per SM.
 //
-// Every wait is bounded; see wait_phase.
+// Every wait is bounded; see mbar_wait.
 #include <math.h>
 
 #include "paged_tc.cuh"
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(384, 1)
             if (more) f = frag_of(a, w, j, lane);
             if (first && keys) {
                 const int qb = seg & 1;
-                ok = wait_phase(&q_empty[qb], ((seg >> 1) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = tc::mbar_wait(&q_empty[qb], ((seg >> 1) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) {
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(384, 1)
                 q_ph = (q_ph & ~(1u << qb)) | (((uint32_t)(seg >> 1) & 1u) << qb);
                 seg++;
             }
-            ok = wait_phase(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = tc::mbar_wait(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int row = frag_row(a, f_now, h), count = frag_count(row);
@@ -247,11 +247,11 @@ __global__ void __launch_bounds__(384, 1)
             bool ok = true;
             do {
                 const int qb = seg & 1;
-                ok = wait_phase(&q_full[qb], (seg >> 1) & 1, abort_flag, err_word, kErrWaitFull);
+                ok = tc::mbar_wait(&q_full[qb], (seg >> 1) & 1, abort_flag, err_word, kErrWaitFull);
                 for (int j = w.j0; j < w.j1 && ok; j++, g++) {
                     const int buf = g & 1;
-                    ok = wait_phase(&k_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
-                         wait_phase(&s_empty[buf], ((g >> 1) & 1) ^ 1, abort_flag, err_word,
+                    ok = tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
+                         tc::mbar_wait(&s_empty[buf], ((g >> 1) & 1) ^ 1, abort_flag, err_word,
                                        kErrWaitAccum);
                     if (!ok) break;
                     tc::tc_fence_after();
@@ -288,10 +288,10 @@ __global__ void __launch_bounds__(384, 1)
                 for (int j = w.j0; j < w.j1 && ok; j++, g++) {
                     const int buf = g & 1;
                     const bool first = j == w.j0;
-                    ok = wait_phase(&v_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
-                         (!first || wait_phase(o_free, (seg & 1) ^ 1, abort_flag, err_word,
+                    ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull) &&
+                         (!first || tc::mbar_wait(o_free, (seg & 1) ^ 1, abort_flag, err_word,
                                                   kErrWaitAccum)) &&
-                         wait_phase(&p_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitFull);
+                         tc::mbar_wait(&p_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitFull);
                     if (!ok) break;
                     tc::tc_fence_after();
                     const uint32_t vb = sV + st * L::kTile, pb = sP + buf * (kKeys * N * 2);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(384, 1)
             }
             for (int j = w.j0; j < w.j1; j++, g++) {
                 const int buf = g & 1;
-                bool ok = wait_phase(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                bool ok = tc::mbar_wait(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
                 tc::tc_fence_after();
                 float v[C];
                 if (ok) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(384, 1)
                     if (col_lane) red[qw * N + col] = mine;
                     // (the tile before this one has its P V done: O is stable)
                     if (ok && j > w.j0)
-                        ok = wait_phase(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
+                        ok = tc::mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
                                            kErrWaitAccum);
                     if (vote_or(bar, !ok)) {
                         run = false;
@@ -419,11 +419,11 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 // its buffer was last read by the P V of tile g - 2
                 if (ok && g >= 2)
-                    ok = wait_phase(&pv_done[buf], ((g - 2) >> 1) & 1, abort_flag, err_word,
+                    ok = tc::mbar_wait(&pv_done[buf], ((g - 2) >> 1) & 1, abort_flag, err_word,
                                        kErrWaitAccum);
                 const int valid = w.kv_len - j * kKeys;
                 if (x == 0 && valid < kKeys) {
-                    if (ok) ok = wait_phase(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                    if (ok) ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
                     if (ok) clear_rows<kSubs>(smem + L::kV + st * L::kTile, key, valid);
                 }
                 if (ok) {
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (!run) break;
             // ---- end of the segment: row sums over the keys, O^T / l
-            bool ok = wait_phase(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
+            bool ok = tc::mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, err_word,
                                     kErrWaitAccum);
             const float mine = reduce_columns<C, false>(l, lane);
             if (col_lane) red[qw * N + col] = mine;

@@ -7,8 +7,9 @@
 // heads that share a key head also share its key and value loads (rows past
 // tok * group are computed and dropped).  One softmax warpgroup per tile, one
 // query row per thread, so the tensor pipe works for one tile while the other
-// tile's warpgroup takes its exponentials; P is handed over in two halves and
-// the reference maximum is lazy, as in the dense ping-pong kernel (attn_tc.cu).
+// tile's warpgroup takes its exponentials; the order of the MMAs, which keeps
+// the two sides half a step apart, the hand-over of P in two halves and the lazy
+// reference maximum are those of the dense ping-pong kernel (attn_tc.cu).
 // An item of one tile (at most 128 rows) would leave one warpgroup idle: there
 // both take the key tiles in turn, each with a reference, a sum and an output
 // of its own, and the first joins the two outputs, which lie side by side in
@@ -19,14 +20,11 @@
 // zero.  The batch is split evenly over the CTAs (paged_tc.cuh).
 //
 // Per CTA (one per SM), 384 threads in three warpgroups: warps 0 and 3 TMA of
-// keys (and queries) and of values, warps 1 and 2 the MMAs of tiles a and b
-// (one warp for both left the tensor pipe idle for the 90 cycles of each of its
-// waits), warpgroups 1 and 2 softmax of tiles a and b.
-// TMEM: S_a [0,128), S_b [128,256), then O_a, O_b.  Dim 128: P_x over S_x, so
-// S of the next key tile follows P V of this one.  Dim 64 has room for P beside
-// S, so S of the next key tile is ready when the softmax asks for it.
+// keys (and queries) and of values, warp 1 tensor memory and MMA issue,
+// warpgroups 1 and 2 softmax of tiles a and b.
+// TMEM: S_a [0,128), S_b [128,256), O_a [256,..), O_b behind it; P_x over S_x.
 //
-// Every wait is bounded; see wait_phase.
+// Every wait is bounded; see mbar_wait.
 #include <math.h>
 
 #include "paged_tc.cuh"
@@ -52,11 +50,10 @@ struct PreSmem {
     static constexpr int kPlan = kV + kStages * kTile;
     static constexpr int kWalk = (kPlan + (int)sizeof(PlanShared) + 15) / 16 * 16;   // a Walk per softmax warp
     static constexpr int kMl = (kWalk + 8 * (int)sizeof(Walk) + 15) / 16 * 16;       // [128][2]: tile b's, to be joined
-    static constexpr int kTurn = kMl + 128 * 8;            // [2][4] key tiles that a softmax warp is done with
-    static constexpr int kBar = kTurn + 32;
-    // q_full, q_empty, s_full[2], s_empty[2], p_full[2], p_half[2], pv_done[2],
-    // o_free[2], joined, drain[2], k_full, k_empty, v_full, v_empty [stages]
-    static constexpr int kNumBars = 17 + 4 * kStages;
+    static constexpr int kBar = kMl + 128 * 8;
+    // q_full, q_empty, s_full[2], p_full[2], p_half[2], pv_done[2], o_free[2],
+    // joined, drain, k_full, k_empty, v_full, v_empty [stages]
+    static constexpr int kNumBars = 14 + 4 * kStages;
     static constexpr int kTotal = kBar + kNumBars * 8 + 16 + 1024;
 };
 
@@ -116,10 +113,10 @@ __global__ void __launch_bounds__(384, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4;
-    uint64_t *p_full = bars + 6, *p_half = bars + 8, *pv_done = bars + 10, *o_free = bars + 12;
-    uint64_t *joined = bars + 14, *drain = bars + 15;
-    uint64_t *k_full = bars + 17, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4;
+    uint64_t *p_half = bars + 6, *pv_done = bars + 8, *o_free = bars + 10, *joined = bars + 12;
+    uint64_t *drain = bars + 13;
+    uint64_t *k_full = bars + 14, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
@@ -129,29 +126,24 @@ __global__ void __launch_bounds__(384, 1)
     tc::launch_dependents();
 
     if (threadIdx.x == 0) {
-        // (both sides hand every query, key and value tile back, also one that
-        // they do not use: a side that skipped some could not tell a later
-        // phase of the same parity from the one it waits for)
         tc::mbar_init(q_full, 1);
-        tc::mbar_init(q_empty, 2);
+        tc::mbar_init(q_empty, 1);
         for (int x = 0; x < 2; x++) {
             tc::mbar_init(&s_full[x], 1);
-            tc::mbar_init(&s_empty[x], 4);
             tc::mbar_init(&p_full[x], 4);
             tc::mbar_init(&p_half[x], 4);
             tc::mbar_init(&pv_done[x], 1);
             tc::mbar_init(&o_free[x], 4);
-            tc::mbar_init(&drain[x], 1);
         }
         tc::mbar_init(joined, 4);
+        tc::mbar_init(drain, 1);
         for (int i = 0; i < S; i++) {
             tc::mbar_init(&k_full[i], 1);
-            tc::mbar_init(&k_empty[i], 2);
+            tc::mbar_init(&k_empty[i], 1);
             tc::mbar_init(&v_full[i], 1);
-            tc::mbar_init(&v_empty[i], 2);
+            tc::mbar_init(&v_empty[i], 1);
         }
         *abort_flag = 0;
-        for (int i = 0; i < 8; i++) reinterpret_cast<uint32_t *>(smem + L::kTurn)[i] = 0;
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmQ);
         tc::tma_prefetch_desc(&tmK);
@@ -165,8 +157,7 @@ __global__ void __launch_bounds__(384, 1)
     const bool any = plan_run<384>(a, item_tok, plan);
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    constexpr bool kOwnP = D == 64;         // P beside S, not over it
-    constexpr uint32_t kColO = 256, kColP = kOwnP ? 384 : 0, kStepP = kOwnP ? 64 : 128;
+    constexpr uint32_t kColO = 256;
 
     if (warp < 4) {
       // warpgroup 0: one setmaxnreg for all four warps, then the roles
@@ -188,7 +179,7 @@ __global__ void __launch_bounds__(384, 1)
         while (more) {
             if (j == w.j0 && keys) {
                 const Span sa = span_of(a, w, 0);
-                ok = wait_phase(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+                ok = tc::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) {
@@ -209,7 +200,7 @@ __global__ void __launch_bounds__(384, 1)
                 j = w.j0;
             }
             if (more) f = frag_of(a, w, j, lane);
-            ok = wait_phase(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = tc::mbar_wait(&empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int row = frag_row(a, f_now, h), count = frag_count(row);
@@ -232,111 +223,115 @@ __global__ void __launch_bounds__(384, 1)
             for (int i = 0; i < S; i++)
                 if (armed >> i & 1) drain_wait(&full[i], last_ph >> i & 1);
         }
-      } else {
+      } else if (warp == 1) {
         if (lane == 0) {
-            // ------------------------------------------------- MMA of tile x
-            const int x = warp - 1;
+            // ----------------------------------------------------------- MMA
             constexpr uint32_t idesc_s = tc::idesc_f16_f32(128, kKeys, false, false, kBf16);
             constexpr uint32_t idesc_o = tc::idesc_f16_f32(128, D, true, false, kBf16);
             const uint32_t sQ = tc::smem_u32(smem + L::kQ);
             const uint32_t sK = tc::smem_u32(smem + L::kK);
             const uint32_t sV = tc::smem_u32(smem + L::kV);
-            const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + kColO + x * D;
-            const uint32_t t_p = tmem_base + kColP + x * kStepP;
             Walk w = plan.start;
-            int seg = 0, g0 = 0;                 // segments; key tiles of the earlier ones
-            int k_pos = 0, v_pos = 0;            // key and value tiles handed back
-            uint32_t n = 0, segs = 0;            // key tiles and segments of this side so far
+            int seg = 0, g0 = 0;                         // segments; key tiles of the earlier ones
+            uint32_t n[2] = {0, 0}, segs[2] = {0, 0};    // key tiles and segments of each side so far
             bool ok = true;
-            auto wait_full = [&](uint64_t *full, int gk) {
-                return wait_phase(&full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
-            };
-            // tiles that this side does not use
-            auto pass = [&](uint64_t *full, uint64_t *empty, int &pos, int upto) {
-                for (; pos < upto && ok; pos++) {
-                    ok = wait_full(full, pos);
-                    if (ok) tc::mbar_arrive(&empty[pos % S]);
-                }
-            };
             do {
-                const Span s = span_of(a, w, x);
-                const uint32_t qb = sQ + (s.alt ? 0 : x * L::kTile);
-                const int g1 = g0 + (w.j1 - w.j0);
-                auto issue_s = [&](int j) {
-                    const int gk = g0 + (j - w.j0), st = gk % S;
-                    pass(k_full, k_empty, k_pos, gk);
-                    ok = ok && wait_full(k_full, gk);
-                    if (!ok) return;
-                    tc::tc_fence_after();
-                    const uint32_t kb = sK + st * L::kTile;
+                const Span sp[2] = {span_of(a, w, 0), span_of(a, w, 1)};
+                const bool alt = sp[0].alt;
+                const int j0 = w.j0, len = w.j1 - w.j0;
+                auto wait_full = [&](uint64_t *full, int i) {
+                    const int gk = g0 + i;
+                    ok = ok && tc::mbar_wait(&full[gk % S], (gk / S) & 1, abort_flag, err_word,
+                                             kErrWaitFull);
+                    if (ok) tc::tc_fence_after();
+                };
+                // S_x = Q K^T of the segment's key tile i; `last`: nobody needs the tile after
+                auto issue_s = [&](int x, int i, bool last) {
+                    const int st = (g0 + i) % S;
+                    const uint32_t kb = sK + st * L::kTile, qb = sQ + (alt ? 0 : x * L::kTile);
 #pragma unroll
                     for (int k = 0; k < D / 16; k++) {
                         const uint32_t off = (k >> 2) * kSubTile + (k & 3) * 32;
-                        tc::mma_ss<tc::MmaKind::F16>(t_s, tc::sdesc_kmajor_sw128(qb + off),
+                        tc::mma_ss<tc::MmaKind::F16>(tmem_base + x * 128, tc::sdesc_kmajor_sw128(qb + off),
                                                      tc::sdesc_kmajor_sw128(kb + off), idesc_s,
                                                      k > 0 ? 1u : 0u);
                     }
                     tc::mma_commit(&s_full[x]);
-                    tc::mma_commit(&k_empty[st]);
-                    k_pos = gk + 1;
-                    if (j + s.step >= s.end) tc::mma_commit(q_empty);
-                    // the other side's tile, so that its stage is not held up
-                    if (s.alt) pass(k_full, k_empty, k_pos, min(gk + 2, g1));
-                };
-                // O_x += P_x V for the keys of K steps k0 .. k0+3 (64 keys)
-                auto issue_pv = [&](int st, bool first, int k0) {
-                    const uint32_t vb = sV + st * L::kTile;
-#pragma unroll
-                    for (int k = k0; k < k0 + 4; k++)
-                        tc::mma_ts_f16(t_o, t_p + k * 8,
-                                       tc::sdesc_mnmajor_sw128(vb + k * 2048, kSubTile, 1024), idesc_o,
-                                       (!first || k > 0) ? 1u : 0u);
-                };
-                ok = wait_phase(q_full, seg & 1, abort_flag, err_word, kErrWaitFull);
-                if (s.start < s.end) {
-                    // (S_x of the last segment has been read: its softmax handed P over,
-                    // and with P beside S also S itself)
-                    if (ok && kOwnP && n > 0)
-                        ok = wait_phase(&s_empty[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
-                    if (ok) issue_s(s.start);
-                    for (int j = s.start; j < s.end && ok; j += s.step, n++) {
-                        const int gk = g0 + (j - w.j0), st = gk % S;
-                        const bool first = j == s.start;
-                        if (kOwnP && j + s.step < s.end) {
-                            ok = wait_phase(&s_empty[x], n & 1, abort_flag, err_word, kErrWaitAccum);
-                            if (ok) issue_s(j + s.step);
-                        }
-                        pass(v_full, v_empty, v_pos, gk);
-                        ok = ok && wait_full(v_full, gk) &&
-                             (!first || wait_phase(&o_free[x], (segs & 1) ^ 1, abort_flag, err_word,
-                                                      kErrWaitAccum)) &&
-                             // the first 64 keys' P V runs while the softmax warps
-                             // still compute the other half of P
-                             wait_phase(&p_half[x], n & 1, abort_flag, err_word, kErrWaitFull);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        issue_pv(st, first, 0);
-                        ok = wait_phase(&p_full[x], n & 1, abort_flag, err_word, kErrWaitFull);
-                        if (!ok) break;
-                        tc::tc_fence_after();
-                        issue_pv(st, false, 4);
-                        tc::mma_commit(&pv_done[x]);
-                        tc::mma_commit(&v_empty[st]);
-                        v_pos = gk + 1;
-                        if (!kOwnP && j + s.step < s.end) issue_s(j + s.step);
+                    if (last) {
+                        tc::mma_commit(&k_empty[st]);
+                        if (i == len - 1) tc::mma_commit(q_empty);
                     }
-                    segs++;
-                } else if (ok) {
-                    tc::mbar_arrive(q_empty);
+                };
+                // O_x += P_x V of key tile i, in two halves of 64 keys: the first
+                // runs while the softmax warps still compute the second of P
+                auto issue_pv = [&](int x, int i, bool first, bool last) {
+                    const uint32_t c = n[x]++;
+                    const int st = (g0 + i) % S;
+                    const uint32_t vb = sV + st * L::kTile;
+                    for (int half = 0; half < 2; half++) {
+                        ok = ok &&
+                             tc::mbar_wait(half == 0 ? &p_half[x] : &p_full[x], c & 1, abort_flag, err_word,
+                                           kErrWaitFull) &&
+                             (half == 1 || !first ||
+                              tc::mbar_wait(&o_free[x], (segs[x] & 1) ^ 1, abort_flag, err_word,
+                                            kErrWaitAccum));
+                        if (!ok) return;
+                        tc::tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc::mma_ts_f16(tmem_base + kColO + x * D,
+                                           tmem_base + x * 128 + half * 32 + k * 8,
+                                           tc::sdesc_mnmajor_sw128(vb + half * 8192 + k * 2048, kSubTile, 1024),
+                                           idesc_o, (!first || half > 0 || k > 0) ? 1u : 0u);
+                    }
+                    tc::mma_commit(&pv_done[x]);
+                    if (last) tc::mma_commit(&v_empty[st]);
+                };
+                ok = tc::mbar_wait(q_full, seg & 1, abort_flag, err_word, kErrWaitFull);
+                if (alt) {
+                    for (int i = 0; i < len && i < 2; i++) {
+                        wait_full(k_full, i);
+                        if (ok) issue_s(i, i, true);
+                    }
+                    for (int i = 0; i < len && ok; i++) {
+                        const int x = i & 1;
+                        wait_full(v_full, i);
+                        issue_pv(x, i, i < 2, true);
+                        if (i + 2 < len) {
+                            wait_full(k_full, i + 2);
+                            if (ok) issue_s(x, i + 2, true);
+                        }
+                    }
+                } else {
+                    // tile a's key tiles end first, if not together with b's
+                    const int len_a = sp[0].end - j0;
+                    wait_full(k_full, 0);
+                    if (ok && len_a > 0) issue_s(0, 0, false);
+                    if (ok) issue_s(1, 0, true);
+                    for (int i = 0; i < len && ok; i++) {
+                        wait_full(v_full, i);
+                        if (i < len_a) {
+                            issue_pv(0, i, i == 0, false);
+                            if (i + 1 < len_a) {
+                                wait_full(k_full, i + 1);
+                                if (ok) issue_s(0, i + 1, false);
+                            }
+                        }
+                        issue_pv(1, i, i == 0, true);
+                        if (i + 1 < len) {
+                            if (i + 1 >= len_a) wait_full(k_full, i + 1);
+                            if (ok) issue_s(1, i + 1, true);
+                        }
+                    }
                 }
-                if (ok) pass(k_full, k_empty, k_pos, g1);
-                if (ok) pass(v_full, v_empty, v_pos, g1);
-                g0 = g1;
+                for (int x = 0; x < 2; x++)
+                    if (sp[x].count() > 0) segs[x]++;
+                g0 += len;
                 seg++;
             } while (ok && w.next(a, item_tok));
-            tc::mma_commit(&drain[x]);
+            tc::mma_commit(drain);
             const uint64_t t0 = tc::globaltimer();
-            while (!tc::mbar_try_wait(&drain[x], 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
+            while (!tc::mbar_try_wait(drain, 0) && tc::globaltimer() - t0 < kWaitBudgetNs) {
             }
         }
       }
@@ -349,8 +344,6 @@ __global__ void __launch_bounds__(384, 1)
         const uint32_t lane_base = (uint32_t)(q * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_base + x * 128;
         const uint32_t o_addr = tmem_base + lane_base + kColO + x * D;
-        const uint32_t p_addr = tmem_base + lane_base + kColP + x * kStepP;
-        volatile uint32_t *turn = reinterpret_cast<volatile uint32_t *>(smem + L::kTurn);
         float2 *ml_b = reinterpret_cast<float2 *>(smem + L::kMl);
         Walk *wp = reinterpret_cast<Walk *>(smem + L::kWalk) + (warp - 4);
         uint32_t n = 0, n_other = 0, joins = 0;  // key tiles so far, of the other side; joined segments
@@ -365,12 +358,11 @@ __global__ void __launch_bounds__(384, 1)
             const int lim = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0 + tok_row));
             const int lim0 = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0));   // the tile's fewest
             const int count_other = span_of(a, *wp, x ^ 1).count();
-            const uint32_t n0 = n;
             float m_ref = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int j = s.start; j < s.end; j += s.step, n++) {
                 const uint32_t c = n;
-                ok = wait_phase(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
+                ok = tc::mbar_wait(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
                 const int key0 = j * kKeys;
@@ -382,11 +374,6 @@ __global__ void __launch_bounds__(384, 1)
                 tc::reg_fence(sr[1]);
                 tc::reg_fence(sr[2]);
                 tc::reg_fence(sr[3]);
-                if (kOwnP) {
-                    tc::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&s_empty[x]);
-                }
                 if (key0 + kKeys > lim0) {
                     const int rest = lim - key0;
 #pragma unroll
@@ -416,7 +403,7 @@ __global__ void __launch_bounds__(384, 1)
                     // max rose by more than 8 (P stays below 2^8 otherwise).
                     const bool need = m_new > m_ref + 8.0f;
                     if (__any_sync(0xffffffffu, need)) {
-                        ok = wait_phase(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
+                        ok = tc::mbar_wait(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
                                            kErrWaitAccum);
                         if (!__all_sync(0xffffffffu, ok)) break;
                         tc::tc_fence_after();
@@ -438,41 +425,18 @@ __global__ void __launch_bounds__(384, 1)
                         }
                     }
                 }
-                if (kOwnP && c > 0) {
-                    // P's columns were last read by the P V of the tile before
-                    ok = wait_phase(&pv_done[x], (c - 1) & 1, abort_flag, err_word, kErrWaitAccum);
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    tc::tc_fence_after();
-                }
                 if (key0 + kKeys > kv_len) {
                     // zeros in the values behind the last cached token, by each
                     // side before it hands its P over (all four warps have then;
                     // that the other side writes the same zeros does not matter)
                     const int gk = g0 + (j - j0);
-                    ok = wait_phase(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
+                    ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
                     if (!__all_sync(0xffffffffu, ok)) break;
                     clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, kv_len - key0);
                     tc::fence_proxy_async_smem();
                 }
-                // The sides take their exponentials in turn, a's i-th tile, b's i-th,
-                // a's next: while one has the MUFU unit the other has its MMAs, its
-                // loads and its maximum.  (A matter of time only: a wait that runs
-                // out goes on.)
-                {
-                    const int i = (int)(c - n0) - (x == 0 ? 1 : 0);
-                    if (i >= 0 && i < count_other) {
-                        const uint32_t target = n_other + i + 1;
-                        for (int polls = 0; polls < 2000; polls++) {
-                            const volatile uint32_t *v = turn + (x ^ 1) * 4;
-                            if ((int)(v[0] - target) >= 0 && (int)(v[1] - target) >= 0 &&
-                                (int)(v[2] - target) >= 0 && (int)(v[3] - target) >= 0)
-                                break;
-                        }
-                        __syncwarp();
-                    }
-                }
                 // P = 2^(s*scale*log2e - m_ref) from the registers, as 16-bit
-                // pairs in columns 16cc..16cc+15; the row sum in four
+                // pairs over S columns 16cc..16cc+15; the row sum in four
                 // packed pairs.  A row that sees nothing yet has no reference.
                 uint64_t acc2[4] = {0, 0, 0, 0};
                 const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
@@ -498,9 +462,8 @@ __global__ void __launch_bounds__(384, 1)
                         acc2[e & 3] = add_pair(acc2[e & 3], pair(p0, p1));
                         pk[e] = pack2<T>(p0, p1);
                     }
-                    tc::tmem_st_32x32b_x16(p_addr + cc * 16, pk);
+                    tc::tmem_st_32x32b_x16(s_addr + cc * 16, pk);
                 }
-                if (lane == 0) turn[x * 4 + q] = c + 1;
                 tc::tmem_st_wait();
                 {
                     float s0, s1, s2, s3, s4, s5, s6, s7;
@@ -518,7 +481,7 @@ __global__ void __launch_bounds__(384, 1)
             // ---- end of the segment
             const bool used = s.start < s.end;
             if (used) {
-                ok = wait_phase(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                ok = tc::mbar_wait(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
             }
@@ -534,8 +497,8 @@ __global__ void __launch_bounds__(384, 1)
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(joined);
                 } else {
-                    ok = wait_phase(joined, joins & 1, abort_flag, err_word, kErrWaitOther) &&
-                         wait_phase(&pv_done[1], (n_other - 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    ok = tc::mbar_wait(joined, joins & 1, abort_flag, err_word, kErrWaitOther) &&
+                         tc::mbar_wait(&pv_done[1], (n_other - 1) & 1, abort_flag, err_word, kErrWaitAccum);
                     if (!__all_sync(0xffffffffu, ok)) break;
                     tc::tc_fence_after();
                     const float2 b = ml_b[row];

@@ -21,18 +21,6 @@ constexpr int kKeys = 128;              // keys per tile
 constexpr int kSubTile = kKeys * 128;   // 64 columns of a key tile: 128 rows x 128 bytes
 constexpr int kPartRows = 256;          // rows of a partial result, at most
 
-// Bounded wait as tc::mbar_wait, which looks at the timer after every test that
-// fails: a wake-up then comes some 700 cycles late.  Here the first tests (each
-// sleeps in the hardware until the phase completes or a time limit passes) go
-// without it.
-__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort,
-                                           int *err_word, int code) {
-#pragma unroll 1
-    for (int i = 0; i < 64; i++)
-        if (tc::mbar_try_wait(bar, parity)) return true;
-    return tc::mbar_wait(bar, parity, abort, err_word, code);
-}
-
 struct PartRec {
     int h, row0, ntok, nparts;          // nparts 0: the CTA's last item is not its to join
 };

@@ -21,7 +21,7 @@
 // gives.  With few rows the kernel is bound by HBM (each key once); with many
 // by the exponentials, one per score.
 //
-// Every wait is bounded; see wait_phase.
+// Every wait is bounded; see mbar_wait.
 #include <math.h>
 
 #include "paged_tc.cuh"
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(384, 1)
                 tok = token(w);
                 page = page_of(w, tok);
             }
-            ok = wait_phase(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            ok = tc::mbar_wait(&k_empty[st], ph ^ 1, abort_flag, err_word, kErrWaitEmpty);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             int row = -1;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(384, 1)
                 const int t_end = w.row_tiles(a);
                 for (int t = w.first_tile(a, 0); t < t_end; t++, u++) {
                     const int qs = u % QS;
-                    ok = wait_phase(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word,
+                    ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word,
                                        kErrWaitEmpty);
                     if (!ok) break;
                     tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
@@ -371,16 +371,16 @@ __global__ void __launch_bounds__(384, 1)
             uint32_t ph = 0, u = 0, n[2] = {0, 0};       // units; score tiles of each half
             bool ok = true;
             do {
-                ok = wait_phase(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                ok = tc::mbar_wait(&k_full[st], ph, abort_flag, err_word, kErrWaitFull);
                 const int t_end = w.row_tiles(a), t1 = w.first_tile_1(a);
                 for (int t = w.first_tile(a, 0); t < t_end && ok; t++, u++) {
                     const int qs = u % QS;
-                    ok = wait_phase(&q_full[qs], (u / QS) & 1, abort_flag, err_word, kErrWaitFull);
+                    ok = tc::mbar_wait(&q_full[qs], (u / QS) & 1, abort_flag, err_word, kErrWaitFull);
                     const uint32_t qb = sQ + qs * L::kQTile;
                     for (int x = 0; x < 2 && ok; x++) {
                         if (x == 1 && t < t1) continue;
                         const int buf = x * 2 + (n[x] & 1);
-                        ok = wait_phase(&s_empty[buf], ((n[x] >> 1) & 1) ^ 1, abort_flag, err_word,
+                        ok = tc::mbar_wait(&s_empty[buf], ((n[x] >> 1) & 1) ^ 1, abort_flag, err_word,
                                            kErrWaitAccum);
                         if (!ok) break;
                         tc::tc_fence_after();
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(384, 1)
                 if (more) t = w.first_tile(a, 0);
             }
             if (more) load(t, zn);
-            bool ok = wait_phase(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            bool ok = tc::mbar_wait(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
             if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
             for (int i = 0; i < kPer; i++)
@@ -473,12 +473,12 @@ __global__ void __launch_bounds__(384, 1)
                 const int lb = u & 3;
                 // (also a half that skips the unit waits for its lse values: it
                 // must not hand back a place that is not filled yet)
-                ok = wait_phase(&l_full[lb], (u >> 2) & 1, abort_flag, err_word, kErrWaitFull);
+                ok = tc::mbar_wait(&l_full[lb], (u >> 2) & 1, abort_flag, err_word, kErrWaitFull);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (t >= t_mine) {
                     const int buf = x * 2 + (n & 1);
-                    ok = wait_phase(&s_full[buf], (n >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                    ok = tc::mbar_wait(&s_full[buf], (n >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc::tc_fence_after();
