@@ -132,9 +132,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a) {
     const int t = i / a.group;
     const int row = t / a.tok * 128 + (t % a.tok) * a.group + i % a.group;
     auto slot = [&](int k) { return ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * kPartRows + row; };
+    const float2 *mls = reinterpret_cast<const float2 *>(a.part_ml);
     float top = -INFINITY;
     for (int k = lane; k < r.nparts; k += 32) {
-        const float2 ml = reinterpret_cast<const float2 *>(a.part_ml)[slot(k)];
+        const float2 ml = mls[slot(k)];
         if (ml.y != 0.0f) top = fmaxf(top, ml.x);
     }
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -142,24 +143,30 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a) {
     float acc[V], sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; v++) acc[v] = 0.0f;
+    // 32 parts at a time: lane k has part k's weight, then all lanes add up rows
+    for (int k0 = 0; k0 < r.nparts; k0 += 32) {
+        float w = 0.0f, l = 0.0f;
+        if (k0 + lane < r.nparts) {
+            const float2 ml = mls[slot(k0 + lane)];
+            // (a part without a visible key has no output)
+            if (ml.y != 0.0f) w = tc::ex2(ml.x - top);
+            l = w * ml.y;
+        }
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        sum += l;
+        const int n = min(32, r.nparts - k0);
 #pragma unroll 4
-    for (int k = 0; k < r.nparts; k++) {
-        const float2 ml = reinterpret_cast<const float2 *>(a.part_ml)[slot(k)];
-        // (a part without a visible key has no output)
-        const float w = ml.y == 0.0f ? 0.0f : tc::ex2(ml.x - top);
-        if (w == 0.0f) continue;
-        sum += w * ml.y;
-        const float *o = a.part_o + slot(k) * D + lane * V;
-        if constexpr (V == 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(o);
-            acc[0] += w * x.x;
-            acc[1] += w * x.y;
-            acc[2] += w * x.z;
-            acc[3] += w * x.w;
-        } else {
-            const float2 x = *reinterpret_cast<const float2 *>(o);
-            acc[0] += w * x.x;
-            acc[1] += w * x.y;
+        for (int k = 0; k < n; k++) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            const float *o = a.part_o + slot(k0 + k) * D + lane * V;
+            float x[V];
+            if constexpr (V == 4)
+                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(o);
+            else
+                *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(o);
+#pragma unroll
+            for (int v = 0; v < V; v++)
+                if (wk != 0.0f) acc[v] += wk * x[v];
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -300,7 +307,7 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
         const int low = page_size & -page_size;
         a.frag = low < kKeys ? low : kKeys;
         a.map_rows = num_pages * kv_heads * page_size;
-        a.min_tiles = 2;
+        a.min_units = 2;
         a.scale_log2 = scale * 1.4426950408889634f;
         a.out = out;
         a.lse = lse;

@@ -35,8 +35,8 @@ namespace {
 // The register file is split with setmaxnreg: the control warpgroup drops to
 // kRegsCtl, the softmax warpgroups rise to kRegsSoftmax (a whole score row of
 // 128 fp32 and its weights).
-constexpr int kRegsCtl = 104;
-constexpr int kRegsSoftmax = 200;
+constexpr int kRegsCtl = 120;
+constexpr int kRegsSoftmax = 192;
 constexpr int kRegsPool = 128 * kRegsCtl + 256 * kRegsSoftmax;
 
 template <int D>
@@ -231,102 +231,143 @@ __global__ void __launch_bounds__(384, 1)
             const uint32_t sQ = tc::smem_u32(smem + L::kQ);
             const uint32_t sK = tc::smem_u32(smem + L::kK);
             const uint32_t sV = tc::smem_u32(smem + L::kV);
+            // (the thread's own instructions are on the critical path between a
+            // softmax and its next scores: descriptors are made once, sides are
+            // compile-time constants)
+            const uint64_t dq = tc::sdesc_kmajor_sw128(sQ), dk = tc::sdesc_kmajor_sw128(sK);
+            const uint64_t dv = tc::sdesc_mnmajor_sw128(sV, kSubTile, 1024);
+            constexpr uint64_t kTileStep = L::kTile >> 4;
+            const std::integral_constant<int, 0> A{};
+            const std::integral_constant<int, 1> B{};
             Walk w = plan.start;
-            int seg = 0, g0 = 0;                         // segments; key tiles of the earlier ones
+            int seg = 0;
             uint32_t n[2] = {0, 0}, segs[2] = {0, 0};    // key tiles and segments of each side so far
+            int k_st = 0, v_st = 0;                      // the rings' next stages and phases
+            uint32_t k_ph = 0, v_ph = 0;
             bool ok = true;
+            auto wait_k = [&]() {
+                ok = ok && tc::mbar_wait(&k_full[k_st], k_ph, abort_flag, err_word, kErrWaitFull);
+                tc::tc_fence_after();
+            };
+            auto wait_v = [&]() {
+                ok = ok && tc::mbar_wait(&v_full[v_st], v_ph, abort_flag, err_word, kErrWaitFull);
+                tc::tc_fence_after();
+            };
+            auto done_k = [&]() {
+                tc::mma_commit(&k_empty[k_st]);
+                if (++k_st == S) {
+                    k_st = 0;
+                    k_ph ^= 1;
+                }
+            };
+            auto done_v = [&]() {
+                tc::mma_commit(&v_empty[v_st]);
+                if (++v_st == S) {
+                    v_st = 0;
+                    v_ph ^= 1;
+                }
+            };
+            // S_x = Q K^T of the key tile in stage k_st; q: the query tile
+            auto issue_s = [&](auto X, int q) {
+                constexpr int x = decltype(X)::value;
+                const uint64_t da = dq + q * kTileStep, db = dk + k_st * kTileStep;
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    constexpr int kSub4 = kSubTile >> 4;
+                    tc::mma_ss<tc::MmaKind::F16>(tmem_base + x * 128, da + (k >> 2) * kSub4 + (k & 3) * 2,
+                                                 db + (k >> 2) * kSub4 + (k & 3) * 2, idesc_s,
+                                                 k > 0 ? 1u : 0u);
+                }
+                tc::mma_commit(&s_full[x]);
+            };
+            // O_x += P_x V of the key tile in stage v_st, in two halves of 64 keys:
+            // the first runs while the softmax warps still compute the second of P
+            auto issue_pv = [&](auto X, bool first) {
+                constexpr int x = decltype(X)::value;
+                const uint32_t c = n[x]++ & 1;
+                const uint64_t db = dv + v_st * kTileStep;
+                ok = ok && tc::mbar_wait(&p_half[x], c, abort_flag, err_word, kErrWaitFull) &&
+                     (!first || tc::mbar_wait(&o_free[x], (segs[x] & 1) ^ 1, abort_flag, err_word,
+                                              kErrWaitAccum));
+                if (!ok) return;
+                tc::tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    tc::mma_ts_f16(tmem_base + kColO + x * D, tmem_base + x * 128 + k * 8,
+                                   db + k * (2048 >> 4), idesc_o, (!first || k > 0) ? 1u : 0u);
+                ok = tc::mbar_wait(&p_full[x], c, abort_flag, err_word, kErrWaitFull);
+                if (!ok) return;
+                tc::tc_fence_after();
+#pragma unroll
+                for (int k = 4; k < 8; k++)
+                    tc::mma_ts_f16(tmem_base + kColO + x * D, tmem_base + x * 128 + k * 8,
+                                   db + k * (2048 >> 4), idesc_o, 1u);
+                tc::mma_commit(&pv_done[x]);
+            };
             do {
-                const Span sp[2] = {span_of(a, w, 0), span_of(a, w, 1)};
-                const bool alt = sp[0].alt;
-                const int j0 = w.j0, len = w.j1 - w.j0;
-                auto wait_full = [&](uint64_t *full, int i) {
-                    const int gk = g0 + i;
-                    ok = ok && tc::mbar_wait(&full[gk % S], (gk / S) & 1, abort_flag, err_word,
-                                             kErrWaitFull);
-                    if (ok) tc::tc_fence_after();
-                };
-                // S_x = Q K^T of the segment's key tile i; `last`: nobody needs the tile after
-                auto issue_s = [&](int x, int i, bool last) {
-                    const int st = (g0 + i) % S;
-                    const uint32_t kb = sK + st * L::kTile, qb = sQ + (alt ? 0 : x * L::kTile);
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = (k >> 2) * kSubTile + (k & 3) * 32;
-                        tc::mma_ss<tc::MmaKind::F16>(tmem_base + x * 128, tc::sdesc_kmajor_sw128(qb + off),
-                                                     tc::sdesc_kmajor_sw128(kb + off), idesc_s,
-                                                     k > 0 ? 1u : 0u);
-                    }
-                    tc::mma_commit(&s_full[x]);
-                    if (last) {
-                        tc::mma_commit(&k_empty[st]);
-                        if (i == len - 1) tc::mma_commit(q_empty);
-                    }
-                };
-                // O_x += P_x V of key tile i, in two halves of 64 keys: the first
-                // runs while the softmax warps still compute the second of P
-                auto issue_pv = [&](int x, int i, bool first, bool last) {
-                    const uint32_t c = n[x]++;
-                    const int st = (g0 + i) % S;
-                    const uint32_t vb = sV + st * L::kTile;
-                    for (int half = 0; half < 2; half++) {
-                        ok = ok &&
-                             tc::mbar_wait(half == 0 ? &p_half[x] : &p_full[x], c & 1, abort_flag, err_word,
-                                           kErrWaitFull) &&
-                             (half == 1 || !first ||
-                              tc::mbar_wait(&o_free[x], (segs[x] & 1) ^ 1, abort_flag, err_word,
-                                            kErrWaitAccum));
-                        if (!ok) return;
-                        tc::tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc::mma_ts_f16(tmem_base + kColO + x * D,
-                                           tmem_base + x * 128 + half * 32 + k * 8,
-                                           tc::sdesc_mnmajor_sw128(vb + half * 8192 + k * 2048, kSubTile, 1024),
-                                           idesc_o, (!first || half > 0 || k > 0) ? 1u : 0u);
-                    }
-                    tc::mma_commit(&pv_done[x]);
-                    if (last) tc::mma_commit(&v_empty[st]);
-                };
+                const Span sa = span_of(a, w, 0);
+                const int len = w.j1 - w.j0;
                 ok = tc::mbar_wait(q_full, seg & 1, abort_flag, err_word, kErrWaitFull);
-                if (alt) {
-                    for (int i = 0; i < len && i < 2; i++) {
-                        wait_full(k_full, i);
-                        if (ok) issue_s(i, i, true);
+                if (sa.alt) {
+                    // one query tile, the key tiles in turn
+                    auto score = [&](auto X, int i) {
+                        wait_k();
+                        if (!ok) return;
+                        issue_s(X, 0);
+                        done_k();
+                        if (i == len - 1) tc::mma_commit(q_empty);
+                    };
+                    auto step = [&](auto X, int i) {
+                        wait_v();
+                        issue_pv(X, i < 2);
+                        if (!ok) return;
+                        done_v();
+                        if (i + 2 < len) score(X, i + 2);
+                    };
+                    score(A, 0);
+                    if (len > 1) score(B, 1);
+                    for (int i = 0; i < len && ok; i += 2) {
+                        step(A, i);
+                        if (i + 1 < len) step(B, i + 1);
                     }
-                    for (int i = 0; i < len && ok; i++) {
-                        const int x = i & 1;
-                        wait_full(v_full, i);
-                        issue_pv(x, i, i < 2, true);
-                        if (i + 2 < len) {
-                            wait_full(k_full, i + 2);
-                            if (ok) issue_s(x, i + 2, true);
-                        }
-                    }
+                    segs[0]++;
+                    if (len > 1) segs[1]++;
                 } else {
-                    // tile a's key tiles end first, if not together with b's
-                    const int len_a = sp[0].end - j0;
-                    wait_full(k_full, 0);
-                    if (ok && len_a > 0) issue_s(0, 0, false);
-                    if (ok) issue_s(1, 0, true);
+                    // both query tiles; a's key tiles end first, if not together
+                    // with b's
+                    const int len_a = sa.end - w.j0;
+                    wait_k();
+                    if (ok && len_a > 0) issue_s(A, 0);
+                    if (ok) {
+                        issue_s(B, 1);
+                        done_k();
+                        if (len == 1) tc::mma_commit(q_empty);
+                    }
                     for (int i = 0; i < len && ok; i++) {
-                        wait_full(v_full, i);
+                        wait_v();
+                        bool k_ready = false;
                         if (i < len_a) {
-                            issue_pv(0, i, i == 0, false);
+                            issue_pv(A, i == 0);
                             if (i + 1 < len_a) {
-                                wait_full(k_full, i + 1);
-                                if (ok) issue_s(0, i + 1, false);
+                                wait_k();
+                                k_ready = true;
+                                if (ok) issue_s(A, 0);
                             }
                         }
-                        issue_pv(1, i, i == 0, true);
+                        issue_pv(B, i == 0);
+                        if (!ok) break;
+                        done_v();
                         if (i + 1 < len) {
-                            if (i + 1 >= len_a) wait_full(k_full, i + 1);
-                            if (ok) issue_s(1, i + 1, true);
+                            if (!k_ready) wait_k();
+                            if (!ok) break;
+                            issue_s(B, 1);
+                            done_k();
+                            if (i + 1 == len - 1) tc::mma_commit(q_empty);
                         }
                     }
+                    if (len_a > 0) segs[0]++;
+                    segs[1]++;
                 }
-                for (int x = 0; x < 2; x++)
-                    if (sp[x].count() > 0) segs[x]++;
-                g0 += len;
                 seg++;
             } while (ok && w.next(a, item_tok));
             tc::mma_commit(drain);
@@ -352,20 +393,24 @@ __global__ void __launch_bounds__(384, 1)
         if (any && lane == 0) *wp = plan.start;
         __syncwarp();
         while (more) {
-            const Span s = span_of(a, *wp, x);
-            const int j0 = wp->j0, kv_len = wp->kv_len;
-            const int tok_row = row / a.group;
-            const int lim = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0 + tok_row));
-            const int lim0 = min(kv_len, seen_by(a.s, kv_len, wp->q_len, s.t0));   // the tile's fewest
-            const int count_other = span_of(a, *wp, x ^ 1).count();
+            // (what the segment's end needs is worked out again there: the loop
+            // has no registers to spare)
+            int left, rest, rest0, step_keys;   // key tiles; keys that the row, the tile's first row still see
+            {
+                const Span s = span_of(a, *wp, x);
+                left = s.count();
+                step_keys = s.step * kKeys;
+                rest = min(wp->kv_len, seen_by(a.s, wp->kv_len, wp->q_len, s.t0 + row / a.group)) -
+                       s.start * kKeys;
+                rest0 = min(wp->kv_len, seen_by(a.s, wp->kv_len, wp->q_len, s.t0)) - s.start * kKeys;
+            }
+            bool first = true;
             float m_ref = -INFINITY, l = 0.0f;
             bool ok = true;
-            for (int j = s.start; j < s.end; j += s.step, n++) {
-                const uint32_t c = n;
-                ok = tc::mbar_wait(&s_full[x], c & 1, abort_flag, err_word, kErrWaitAccum);
+            for (; left > 0; left--, n++, rest -= step_keys, rest0 -= step_keys, first = false) {
+                ok = tc::mbar_wait(&s_full[x], n & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
-                const int key0 = j * kKeys;
                 // the whole score row into registers: four loads, one wait
                 uint32_t sr[4][32];
 #pragma unroll
@@ -374,8 +419,7 @@ __global__ void __launch_bounds__(384, 1)
                 tc::reg_fence(sr[1]);
                 tc::reg_fence(sr[2]);
                 tc::reg_fence(sr[3]);
-                if (key0 + kKeys > lim0) {
-                    const int rest = lim - key0;
+                if (rest0 < kKeys) {
 #pragma unroll
                     for (int cc = 0; cc < 4; cc++)
 #pragma unroll
@@ -396,14 +440,14 @@ __global__ void __launch_bounds__(384, 1)
                                       fmaxf(mx[6], mx[7])) *
                                  a.scale_log2;
                 const float m_new = fmaxf(m_ref, mt);
-                if (j == s.start) {
+                if (first) {
                     m_ref = m_new;
                 } else {
                     // Lazy rescale: the reference max moves only when the row
                     // max rose by more than 8 (P stays below 2^8 otherwise).
                     const bool need = m_new > m_ref + 8.0f;
                     if (__any_sync(0xffffffffu, need)) {
-                        ok = tc::mbar_wait(&pv_done[x], (c - 1) & 1, abort_flag, err_word,
+                        ok = tc::mbar_wait(&pv_done[x], (n - 1) & 1, abort_flag, err_word,
                                            kErrWaitAccum);
                         if (!__all_sync(0xffffffffu, ok)) break;
                         tc::tc_fence_after();
@@ -425,15 +469,19 @@ __global__ void __launch_bounds__(384, 1)
                         }
                     }
                 }
-                if (key0 + kKeys > kv_len) {
+                if (left == 1 && wp->kv_len < wp->j1 * kKeys) {
                     // zeros in the values behind the last cached token, by each
                     // side before it hands its P over (all four warps have then;
                     // that the other side writes the same zeros does not matter)
-                    const int gk = g0 + (j - j0);
-                    ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word, kErrWaitFull);
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, kv_len - key0);
-                    tc::fence_proxy_async_smem();
+                    const Span s = span_of(a, *wp, x);
+                    const int j = s.start + (s.count() - 1) * s.step, gk = g0 + (j - wp->j0);
+                    if (j * kKeys + kKeys > wp->kv_len) {
+                        ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word,
+                                           kErrWaitFull);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, wp->kv_len - j * kKeys);
+                        tc::fence_proxy_async_smem();
+                    }
                 }
                 // P = 2^(s*scale*log2e - m_ref) from the registers, as 16-bit
                 // pairs over S columns 16cc..16cc+15; the row sum in four
@@ -479,6 +527,9 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (!__all_sync(0xffffffffu, ok)) break;
             // ---- end of the segment
+            const Span s = span_of(a, *wp, x);
+            const int j0 = wp->j0, tok_row = row / a.group;
+            const int count_other = span_of(a, *wp, x ^ 1).count();
             const bool used = s.start < s.end;
             if (used) {
                 ok = tc::mbar_wait(&pv_done[x], (n - 1) & 1, abort_flag, err_word, kErrWaitAccum);

@@ -2,12 +2,14 @@
 // the tensor maps, the loads of a 128-key tile page by page, and the even
 // split of a ragged batch over the CTAs.
 //
-// Split.  A work item is (sequence, key head, tile of query rows) and takes
-// ceil(keys its last row sees / 128) key tiles, at least one (a row that sees
-// nothing is still written).  The tiles of all items, in that order, are
-// numbered 0 .. T - 1 and CTA c of C takes c T / C .. (c + 1) T / C - 1: a
-// run of items, the first and the last perhaps only in part.  Lengths live on
-// the device, so each CTA derives its own run from them (a prefix sum over the
+// Split.  A work item is (sequence, key head, one or two tiles of query rows)
+// and takes ceil(keys its last row sees / 128) key tiles, at least one (a row
+// that sees nothing is still written).  A key tile costs one unit, or two when
+// the item has two query tiles (measured 1700 and 3300 cycles at dim 64, 2600
+// and 4000 at dim 128).  The units of all items, in that order, are numbered
+// 0 .. T - 1 and CTA c of C takes the key tiles that start in units c T / C ..
+// (c + 1) T / C - 1: a run of items, the first and the last perhaps only in
+// part.  Lengths live on the device, so each CTA derives its own run from them (a prefix sum over the
 // sequences).  An item that is cut leaves one partial result per CTA: the
 // unnormalised output, the reference maximum and the sum of each row.  A
 // second kernel joins them, in CTA order, so results do not depend on timing.
@@ -32,7 +34,7 @@ struct PagedTc {
     int tok;                 // tokens of a query tile: rows / group
     int frag;                // rows of one page load: a power of two, 8 to 128
     int map_rows;            // rows of the cache: a coordinate behind the last
-    int min_tiles;           // fewer tiles than this are not worth a CTA
+    int min_units;           // of a CTA's run, at least 2: then it has a key tile
     float scale_log2;        // scale * log2(e)
     void *out;
     float *lse;
@@ -58,21 +60,27 @@ __device__ __forceinline__ int tiles_to(const PagedSeqs &s, int kv_len, int q_le
     return max(1, (seen + kKeys - 1) / kKeys);
 }
 
+// Units of a key tile of an item (its two query tiles are 2 * a.tok tokens).
+__device__ __forceinline__ int units_of(const PagedTc &a, int item_tok, int q_len, int rt) {
+    return item_tok > a.tok && q_len - rt * item_tok > a.tok ? 2 : 1;
+}
+
 // A CTA's run of items, one segment (item, key tiles j0 .. j1 - 1) at a time.
 // Every role of the CTA walks its own copy.
 struct Walk {
-    int b, h, rt, j0, j1, nt;
+    int b, h, rt, j0, j1, nt, cost;
     int first, q_len, kv_len;
-    long long pos, end;      // first tile of the segment, end of the run
+    long long pos, end;      // first unit of the segment, end of the run
 
     // the segment at (b, h, rt, j0), pos
     __device__ __forceinline__ void open(const PagedTc &a, int item_tok) {
         nt = tiles_to(a.s, kv_len, q_len, (rt + 1) * item_tok);
-        const long long left = end - pos;
+        cost = units_of(a, item_tok, q_len, rt);
+        const long long left = (end - pos + cost - 1) / cost;
         j1 = left < nt - j0 ? j0 + (int)left : nt;
     }
     __device__ __forceinline__ bool next(const PagedTc &a, int item_tok) {
-        pos += j1 - j0;
+        pos += (long long)(j1 - j0) * cost;
         if (pos >= end) return false;
         j0 = 0;
         if (++rt * item_tok >= q_len) {
@@ -103,17 +111,18 @@ template <int THREADS>
 __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanShared &sh) {
     const int per = (a.s.batch + THREADS - 1) / THREADS;
     const int b0 = min(a.s.batch, (int)threadIdx.x * per), b1 = min(a.s.batch, b0 + per);
-    auto tiles_of = [&](int q_len, int kv_len) {
+    auto units = [&](int q_len, int kv_len) {       // of one key head
         long long n = 0;
-        for (int t = item_tok; t - item_tok < q_len; t += item_tok)
-            n += tiles_to(a.s, kv_len, q_len, t);
+        for (int rt = 0; rt * item_tok < q_len; rt++)
+            n += (long long)tiles_to(a.s, kv_len, q_len, (rt + 1) * item_tok) *
+                 units_of(a, item_tok, q_len, rt);
         return n;
     };
     long long mine = 0;
     for (int b = b0; b < b1; b++) {
         int first;
         const int q_len = seq_q_len(a.s, b, first), kv_len = seq_kv_len(a.s, b);
-        mine += tiles_of(q_len, kv_len) * a.kv_heads;
+        mine += units(q_len, kv_len) * a.kv_heads;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long upto = mine;
@@ -128,7 +137,7 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
         if (w < warp) upto += sh.sums[w];
         total += sh.sums[w];
     }
-    const long long want = (total + a.min_tiles - 1) / a.min_tiles;
+    const long long want = max(total / a.min_units, total > 0 ? 1LL : 0LL);
     const int ctas = want < (int)gridDim.x ? (int)want : (int)gridDim.x;
     const bool any = (int)blockIdx.x < ctas;
     if (any) {
@@ -138,7 +147,7 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
             Walk w;
             for (int b = b0; b < b1; b++) {
                 quiet_seq(a.s, b, w.first, w.q_len, w.kv_len);
-                const long long n = tiles_of(w.q_len, w.kv_len);
+                const long long n = units(w.q_len, w.kv_len);
                 if (at >= n * a.kv_heads) {
                     at -= n * a.kv_heads;
                     continue;
@@ -147,16 +156,22 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
                 w.h = (int)(at / n);
                 at -= w.h * n;
                 for (w.rt = 0;; w.rt++) {
-                    const int nt = tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok);
-                    if (at < nt) break;
-                    at -= nt;
+                    const int units = tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok) *
+                                      units_of(a, item_tok, w.q_len, w.rt);
+                    if (at < units) break;
+                    at -= units;
                 }
-                w.j0 = (int)at;
                 break;
             }
-            w.pos = lo;
+            // the first key tile that starts here: perhaps the next item's first
+            w.cost = units_of(a, item_tok, w.q_len, w.rt);
+            w.j0 = w.j1 = (int)((at + w.cost - 1) / w.cost);
+            w.pos = lo + (w.j0 * w.cost - at);
             w.end = hi;
-            w.open(a, item_tok);
+            if (w.j0 < tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok))
+                w.open(a, item_tok);
+            else
+                w.next(a, item_tok);
             sh.start = w;
             sh.ctas = ctas;
             sh.total = total;
@@ -173,12 +188,12 @@ __device__ __forceinline__ void note_parts(const PagedTc &a, const PlanShared &s
                                            int item_tok) {
     PartRec r{0, 0, 0, 0};
     if (w.j0 == 0 && w.j1 < w.nt) {
-        // the CTA that holds the item's last tile e - 1: the largest c with c T / C <= e - 1
-        const long long e = w.pos + w.nt;
+        // the CTA where the item's last tile starts, in unit u: the largest c with c T / C <= u
+        const long long u = w.pos + (long long)(w.nt - 1) * w.cost;
         r.h = w.h;
         r.row0 = w.first + w.rt * item_tok;
         r.ntok = min(item_tok, w.q_len - w.rt * item_tok);
-        r.nparts = (int)((e * sh.ctas - 1) / sh.total) - (int)blockIdx.x + 1;
+        r.nparts = (int)(((u + 1) * sh.ctas - 1) / sh.total) - (int)blockIdx.x + 1;
     }
     a.recs[blockIdx.x] = r;
 }
