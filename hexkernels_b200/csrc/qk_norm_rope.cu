@@ -27,6 +27,7 @@ struct NormRope {
     float *scores;
     int tokens, heads, kv_heads, dim, rot, halves, norm, table_len;
     int num_pages, page_size;
+    int page_shift;         // log2 of page_size, or -1
     float eps;
     int *err_word;
 };
@@ -39,8 +40,8 @@ __device__ __forceinline__ bool token_place(const NormRope &a, int pos, int slot
     off = 0;
     if (a.slots) {
         if (slot < 0) return false;
-        page = slot / a.page_size;
-        off = slot % a.page_size;
+        page = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page_size;
+        off = slot - (int)page * a.page_size;
         if (page >= a.num_pages) {
             flag_index(a.err_word);
             return false;
@@ -70,137 +71,184 @@ __device__ __forceinline__ T *row_target(const NormRope &a, int t, int r, int64_
     return pages + ((page * a.kv_heads + r) * a.page_size + off) * a.dim;
 }
 
-// Four values as 32-bit floats, and back.
-template <typename T>
-__device__ __forceinline__ void widen(uint2 w, float (&x)[4]) {
-    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-    x[0] = a.x;
-    x[1] = a.y;
-    x[2] = b.x;
-    x[3] = b.y;
+// Packed pairs of 32-bit floats (one instruction for two).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
 template <typename T>
-__device__ __forceinline__ uint2 narrow(const float (&x)[4]) {
-    return make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+__device__ __forceinline__ void widen(const uint4 &w, uint64_t (&x)[4]) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpack2<T>(v[i]);
+        x[i] = pair(f.x, f.y);
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpair(x[i]);
+        v[i] = pack2<T>(f.x, f.y);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// Head sizes that are multiples of 8, 8-byte aligned rows: LPR lanes a row (8
-// values a lane), 256 / LPR rows at a time, every thread in the same columns
-// of all its rows, so that a token's cosines and sines and the gains are read
-// once.  A lane's 8 values are two pieces of 4 chosen so that a pair never
-// leaves the lane: columns 4c.. and rot/2 + 4c.. when halves turn together,
-// 8c.. and 8c + 4.. otherwise; in both the lane's four pairs are 4c .. 4c + 3.
-// `ysplit` blocks share a token when tokens are few.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(256, 4) norm_rope_kernel(const NormRope a, int ysplit) {
-    constexpr int kRows = 256 / LPR, U = 4;
-    const int c = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-    const int per_token = a.heads + a.kv_heads * (a.v ? 2 : 1);
-    const bool in_row = c * 8 < a.dim, turns = c * 8 < a.rot;
-    const int o0 = turns && a.halves ? 4 * c : 8 * c;
-    const int o1 = turns && a.halves ? a.rot / 2 + 4 * c : 8 * c + 4;
-    // the gains of this lane's columns, as they are stored
-    uint2 gq0, gq1, gk0, gk1;
-    const uint2 ones = make_uint2(pack2<T>(1.0f, 1.0f), pack2<T>(1.0f, 1.0f));
-    auto gain_of = [&](const void *g, uint2 &x, uint2 &y) {
-        x = y = ones;
-        if (g && a.norm && in_row) {
-            x = *reinterpret_cast<const uint2 *>((const T *)g + o0);
-            y = *reinterpret_cast<const uint2 *>((const T *)g + o1);
+// Head sizes and rot_dim that are multiples of 16, 16-byte aligned rows: a block
+// takes up to U passes of 128 / LPR rows of a token, LPR lanes a row (16 values a
+// lane), all loads in flight together; blocks are short and many, so that those
+// which load and those which compute overlap.  A lane's 16 values are two pieces
+// of 8, chosen so that a pair never leaves the lane: columns 8c.. and rot/2 +
+// 8c.. when halves turn together, 16c.. and 16c + 8.. otherwise; in both the
+// lane's eight pairs are 8c .. 8c + 7.  What bounds it besides HBM is the number
+// of instructions, a third of them the same for every warp of a token (its slot
+// and pointers): hence the small block, 16 values a lane and 32-bit strides.
+constexpr int U = 3;
+
+constexpr int kWideThreads = 128;
+
+template <typename T, int LPR, bool HALVES>
+__global__ void __launch_bounds__(kWideThreads, 8) norm_rope_kernel(const NormRope a, int passes) {
+    constexpr int kRows = kWideThreads / LPR;
+    const int c = threadIdx.x % LPR, t = blockIdx.x;
+    const int r0 = blockIdx.y * passes * kRows + threadIdx.x / LPR;
+    const int k_end = a.heads + a.kv_heads, r_end = k_end + (a.v ? a.kv_heads : 0);
+    const int pos = a.rot > 0 ? a.positions[t] : 0, slot = a.slots ? a.slots[t] : 0;
+    const bool in_row = c * 16 < a.dim, turns = c * 16 < a.rot;
+    const int o0 = turns && HALVES ? 8 * c : 16 * c;
+    const int o1 = turns && HALVES ? a.rot / 2 + 8 * c : 16 * c + 8;
+    // (strides and head offsets are below 2^31 here)
+    const T *qs = (const T *)a.q + (int64_t)t * (int)a.q_stride;
+    const T *ks = (const T *)a.k + (int64_t)t * (int)a.k_stride;
+    const T *vs = (const T *)a.v + (int64_t)t * (int)a.v_stride;
+    uint4 wx[U], wy[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int r = r0 + u * kRows;
+        wx[u] = wy[u] = make_uint4(0, 0, 0, 0);
+        if (u < passes && r < r_end && in_row && slot >= 0) {
+            const T *p = (r < a.heads ? qs : r < k_end ? ks : vs) +
+                         (r - (r < a.heads ? 0 : r < k_end ? a.heads : k_end)) * a.dim;
+            wx[u] = *reinterpret_cast<const uint4 *>(p + o0);
+            wy[u] = *reinterpret_cast<const uint4 *>(p + o1);
         }
-    };
-    gain_of(a.q_gain, gq0, gq1);
-    gain_of(a.k_gain, gk0, gk1);
+    }
+    int64_t page;
+    int off;
+    if (!token_place(a, pos, slot, page, off)) return;
+    // (columns that do not turn have a cosine of 1 and a sine of 0)
+    uint64_t cs[4], sn[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        cs[i] = pair(1.0f, 1.0f);
+        sn[i] = pair(0.0f, 0.0f);
+    }
+    if (turns) {
+        const int64_t o = (int64_t)pos * (a.rot / 2) + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float4 f = reinterpret_cast<const float4 *>(a.cos_t + o)[i];
+            const float4 g = reinterpret_cast<const float4 *>(a.sin_t + o)[i];
+            cs[2 * i] = pair(f.x, f.y);
+            cs[2 * i + 1] = pair(f.z, f.w);
+            sn[2 * i] = pair(g.x, g.y);
+            sn[2 * i + 1] = pair(g.z, g.w);
+        }
+    }
+    const int64_t kv_at = page * (int64_t)(a.kv_heads * a.page_size * a.dim) + off * a.dim;
+    T *qd = (T *)a.q_out + (int64_t)t * (a.heads * a.dim);
+    T *kd = (T *)a.k_pages + kv_at, *vd = (T *)a.v_pages + kv_at;
     const float inv_dim = 1.0f / (float)a.dim;
-    const int64_t items = (int64_t)a.tokens * ysplit;
-    const int step = kRows * ysplit;
-    // a token's position and slot, fetched while the token before it is worked on
-    auto fetch = [&](int64_t item, int &pos, int &at) {
-        const int t = (int)(item / ysplit);
-        pos = a.rot > 0 ? a.positions[t] : 0;
-        at = a.slots ? a.slots[t] : 0;
-    };
-    int pos_next = 0, slot_next = 0;
-    if ((int64_t)blockIdx.x < items) fetch(blockIdx.x, pos_next, slot_next);
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int t = (int)(item / ysplit), pos = pos_next, at = slot_next;
-        if (item + gridDim.x < items) fetch(item + gridDim.x, pos_next, slot_next);
-        int64_t page;
-        int off;
-        if (!token_place(a, pos, at, page, off)) continue;
-        float4 cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (turns) {
-            cs = *reinterpret_cast<const float4 *>(a.cos_t + (int64_t)pos * (a.rot / 2) + 4 * c);
-            sn = *reinterpret_cast<const float4 *>(a.sin_t + (int64_t)pos * (a.rot / 2) + 4 * c);
-        }
-        const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
-        // (rows of one warp may end at different passes; all lanes stay for the shuffles)
-        for (int r0 = (int)(item % ysplit) * kRows; r0 < per_token; r0 += U * step) {
-            uint2 w0[U], w1[U];
+    const uint64_t minus = pair(-1.0f, -1.0f);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int r = r0 + u * step + slot;
-                w0[u] = w1[u] = make_uint2(0, 0);
-                if (r < per_token && in_row) {
-                    const T *src = row_source<T>(a, t, r);
-                    w0[u] = *reinterpret_cast<const uint2 *>(src + o0);
-                    w1[u] = *reinterpret_cast<const uint2 *>(src + o1);
+    for (int u = 0; u < U; u++) {
+        if (u >= passes) break;
+        const int r = r0 + u * kRows;
+        uint64_t x[4], y[4];
+        widen<T>(wx[u], x);
+        widen<T>(wy[u], y);
+        float inv = 1.0f;
+        if (a.norm) {
+            uint64_t s2 = mul2(x[0], x[0]);
+#pragma unroll
+            for (int i = 1; i < 4; i++) s2 = fma2(x[i], x[i], s2);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s2 = fma2(y[i], y[i], s2);
+            const float2 s = unpair(s2);
+            float sum = s.x + s.y;
+            // (all lanes take part, also those past the row or the token)
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            inv = rsqrtf(fmaf(sum, inv_dim, a.eps));
+        }
+        if (r >= r_end || !in_row) continue;
+        const bool is_q = r < a.heads;
+        T *p = (is_q ? qd : r < k_end ? kd : vd) +
+               (r - (is_q ? 0 : r < k_end ? a.heads : k_end)) * (is_q ? a.dim : a.page_size * a.dim);
+        if (r < k_end) {
+            const T *gain = (const T *)(is_q ? a.q_gain : a.k_gain);
+            const uint64_t iv = pair(inv, inv);
+            if (a.norm && gain) {
+                uint64_t g[4], h[4];
+                widen<T>(*reinterpret_cast<const uint4 *>(gain + o0), g);
+                widen<T>(*reinterpret_cast<const uint4 *>(gain + o1), h);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[i] = mul2(x[i], mul2(iv, g[i]));
+                    y[i] = mul2(y[i], mul2(iv, h[i]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[i] = mul2(x[i], iv);
+                    y[i] = mul2(y[i], iv);
                 }
             }
+            if (HALVES) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int r = r0 + u * step + slot;
-                if (r0 + u * step >= per_token) break;
-                float x[4], y[4];
-                widen<T>(w0[u], x);
-                widen<T>(w1[u], y);
-                float inv = 1.0f;
-                if (a.norm) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum += x[i] * x[i] + y[i] * y[i];
-#pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    inv = rsqrtf(sum * inv_dim + a.eps);
+                for (int i = 0; i < 4; i++) {
+                    const uint64_t f = x[i];
+                    x[i] = fma2(f, cs[i], mul2(mul2(y[i], sn[i]), minus));
+                    y[i] = fma2(f, sn[i], mul2(y[i], cs[i]));
                 }
-                if (r >= per_token || !in_row) continue;
-                T *dst = row_target<T>(a, t, r, page, off);
-                if (r < a.heads + a.kv_heads) {
-                    const bool is_q = r < a.heads;
-                    float g0[4], g1[4];
-                    widen<T>(is_q ? gq0 : gk0, g0);
-                    widen<T>(is_q ? gq1 : gk1, g1);
+            } else {
+                auto turn = [](uint64_t &v, float co, float si) {
+                    const float2 f = unpair(v);
+                    v = pair(f.x * co - f.y * si, f.x * si + f.y * co);
+                };
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[i] *= inv * g0[i];
-                        y[i] *= inv * g1[i];
-                    }
-                    if (a.halves) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float p = x[i], q = y[i];
-                            x[i] = p * cv[i] - q * sv[i];
-                            y[i] = p * sv[i] + q * cv[i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2) {
-                            const float p = x[i], q = x[i + 1], e = y[i], f = y[i + 1];
-                            x[i] = p * cv[i / 2] - q * sv[i / 2];
-                            x[i + 1] = p * sv[i / 2] + q * cv[i / 2];
-                            y[i] = e * cv[2 + i / 2] - f * sv[2 + i / 2];
-                            y[i + 1] = e * sv[2 + i / 2] + f * cv[2 + i / 2];
-                        }
-                    }
-                    w0[u] = narrow<T>(x);
-                    w1[u] = narrow<T>(y);
-                    if (a.scores && !is_q && c == 0)
-                        a.scores[(page * a.kv_heads + (r - a.heads)) * a.page_size + off] = 0.0f;
+                for (int i = 0; i < 4; i++) {
+                    const float2 c0 = unpair(cs[i / 2]), s0 = unpair(sn[i / 2]);
+                    const float2 c1 = unpair(cs[2 + i / 2]), s1 = unpair(sn[2 + i / 2]);
+                    turn(x[i], i & 1 ? c0.y : c0.x, i & 1 ? s0.y : s0.x);
+                    turn(y[i], i & 1 ? c1.y : c1.x, i & 1 ? s1.y : s1.x);
                 }
-                *reinterpret_cast<uint2 *>(dst + o0) = w0[u];
-                *reinterpret_cast<uint2 *>(dst + o1) = w1[u];
             }
+            wx[u] = narrow<T>(x);
+            wy[u] = narrow<T>(y);
+            if (a.scores && !is_q && c == 0)
+                a.scores[(page * a.kv_heads + (r - a.heads)) * a.page_size + off] = 0.0f;
         }
+        *reinterpret_cast<uint4 *>(p + o0) = wx[u];
+        *reinterpret_cast<uint4 *>(p + o1) = wy[u];
     }
 }
 
@@ -257,26 +305,36 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRope a) {
     }
 }
 
-// Whether the tensors and strides allow the 8- and 16-byte accesses above.
+// Whether the tensors and strides allow the 16-byte accesses above.
 bool wide_rows(const NormRope &a) {
-    const uintptr_t p8 = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out |
-                         (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.q_gain |
-                         (uintptr_t)a.k_gain;
-    const uintptr_t p16 = (uintptr_t)a.cos_t | (uintptr_t)a.sin_t;
+    const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out |
+                        (uintptr_t)a.k_pages | (uintptr_t)a.v_pages | (uintptr_t)a.q_gain |
+                        (uintptr_t)a.k_gain | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t;
     const int64_t strides = (a.heads ? a.q_stride : 0) | (a.kv_heads ? a.k_stride : 0) |
                             (a.v ? a.v_stride : 0);
-    return a.dim % 8 == 0 && a.rot % 8 == 0 && strides % 4 == 0 && p8 % 8 == 0 &&
-           (a.rot == 0 || p16 % 16 == 0);
+    // (strides and offsets between heads are 32-bit there)
+    if (((int64_t)a.heads + a.kv_heads * (int64_t)a.page_size) * a.dim > 0x7fffffff ||
+        a.q_stride > 0x7fffffff || a.k_stride > 0x7fffffff || a.v_stride > 0x7fffffff)
+        return false;
+    return a.dim % 16 == 0 && a.rot % 16 == 0 && strides % 8 == 0 && p % 16 == 0;
 }
 
-template <typename T, int LPR>
+template <typename T, int LPR, bool HALVES>
 void launch_wide(Dev *d, const NormRope &a) {
-    constexpr auto kern = norm_rope_kernel<T, LPR>;
     const int rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
-    const int passes = (rows + 256 / LPR - 1) / (256 / LPR);
+    constexpr int kRows = kWideThreads / LPR;
+    const int all = (rows + kRows - 1) / kRows;
     // few tokens: a block per pass, so that a token's rows go out at once
-    const int ysplit = a.tokens < 4 * d->sms ? passes : 1;
-    kern<<<resident_blocks<kern>(d, (int64_t)a.tokens * ysplit * 256), 256, 0, d->stream>>>(a, ysplit);
+    const int passes = a.tokens < 4 * d->sms ? 1 : all < U ? all : U;
+    const dim3 grid((unsigned)a.tokens, (unsigned)((all + passes - 1) / passes));
+    norm_rope_kernel<T, LPR, HALVES><<<grid, kWideThreads, 0, d->stream>>>(a, passes);
+}
+template <typename T, int LPR>
+void launch_halves(Dev *d, const NormRope &a) {
+    if (a.halves)
+        launch_wide<T, LPR, true>(d, a);
+    else
+        launch_wide<T, LPR, false>(d, a);
 }
 template <typename T>
 void launch_rows(Dev *d, const NormRope &a) {
@@ -285,11 +343,11 @@ void launch_rows(Dev *d, const NormRope &a) {
         const int64_t rows = (int64_t)a.tokens * (a.heads + a.kv_heads * (a.v ? 2 : 1));
         kern<<<resident_blocks<kern>(d, rows * 32), 256, 0, d->stream>>>(a);
     } else if (a.dim <= 64) {
-        launch_wide<T, 8>(d, a);
+        launch_halves<T, 4>(d, a);
     } else if (a.dim <= 128) {
-        launch_wide<T, 16>(d, a);
+        launch_halves<T, 8>(d, a);
     } else {
-        launch_wide<T, 32>(d, a);
+        launch_halves<T, 16>(d, a);
     }
 }
 
@@ -359,6 +417,9 @@ HX_EXPORT int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_
     a.table_len = table_len;
     a.num_pages = num_pages;
     a.page_size = page_size;
+    a.page_shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (page_size == 1 << i) a.page_shift = i;
     a.eps = eps;
     a.err_word = d->err_word;
     launch_begin(d);
