@@ -25,6 +25,7 @@ struct Evict {
     int *new_lens, *kept;
     int batch, kv_heads, dim, num_pages, page_size, max_pages, dst_max_pages;
     int budget, sink, recent;
+    int page_shift;         // log2 of page_size, or -1
     int *err_word;
 };
 
@@ -51,14 +52,13 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;             // 11 bits of a key a pass (the last pass has 10)
 constexpr int kSmemKeys = 49152;        // keys of a CTA that fit shared memory
 constexpr int kMaxCluster = 8;
 
 // shared memory of one CTA of the cluster that works on a (sequence, key head)
 struct Select {
-    int hist[2][kBins];
+    alignas(16) int hist[2][kBins];
     int warp_sum[32], warp_eq[32];
     int counts[2];                      // keys above the threshold, equal to it
     int bin, left;
@@ -69,6 +69,14 @@ __device__ __forceinline__ int peer_int(const int *p, uint32_t rank) {
     int v;
     asm volatile("ld.shared::cluster.b32 %0, [%1];"
                  : "=r"(v)
+                 : "r"(tc::mapa_shared(tc::smem_u32(p), rank))
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ int2 peer_pair(const int *p, uint32_t rank) {
+    int2 v;
+    asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];"
+                 : "=r"(v.x), "=r"(v.y)
                  : "r"(tc::mapa_shared(tc::smem_u32(p), rank))
                  : "memory");
     return v;
@@ -87,8 +95,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
 // distributed shared memory) and finds the bin where the count from the top
 // reaches what is wanted.  Then the places are written in ascending order,
 // each warp on a contiguous run, with ballots for the ranks in it.
-template <bool SMEM>
+template <bool SMEM, int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a) {
+    constexpr int kWarps = kSelThreads / 32, kPer = kBins / kSelThreads;
+    tc::launch_dependents();
     __shared__ Select sh;
     extern __shared__ uint32_t keys[];
     const uint32_t ranks = cluster_size(), rank = tc::cluster_ctarank();
@@ -114,100 +124,140 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
     const int per = ((hi - lo + (int)ranks - 1) / (int)ranks + 31) & ~31;
     const int first = lo + (int)rank * per;
     const int count = max(0, min(per, hi - first));
+    auto page_no = [&](int j) { return a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size; };
     auto read_key = [&](int i) -> uint32_t {
-        const int j = first + i, pi = j / a.page_size;
+        const int j = first + i, pi = page_no(j);
         const int page = evict_page(a, a.table, a.max_pages, b, pi);
         if (page < 0) return 0u;
         return order_key(
             a.scores[((int64_t)page * a.kv_heads + h) * a.page_size + (j - pi * a.page_size)]);
     };
+    auto key_at = [&](int i) { return SMEM ? keys[i] : read_key(i); };
+    // one more key in the bin for each lane whose `in` is set; equal scores are
+    // common, and lanes that agree on the bin add once
+    auto count_in = [&](int *hist, bool in, int bin) {
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (who == 0) return;
+        const int leader = __ffs((int)who) - 1;
+        const int bin0 = __shfl_sync(0xffffffffu, bin, leader);
+        if (__ballot_sync(0xffffffffu, in && bin != bin0) == 0) {
+            if (lane == leader) atomicAdd(&hist[bin0], __popc(who));
+        } else if (in) {
+            atomicAdd(&hist[bin], 1);
+        }
+    };
+    for (int i = threadIdx.x; i < kBins; i += kSelThreads) sh.hist[0][i] = 0;
+    __syncthreads();
     if (SMEM) {
-        // eight keys a thread at a time: all their pages, then all their scores
-        constexpr int U = 8;
-        for (int i0 = threadIdx.x; i0 < count; i0 += U * kSelThreads) {
+        // sixteen keys a thread at a time: all their pages, then all their scores,
+        // then the first pass's count while they are in registers
+        constexpr int U = 16;
+        for (int i0 = warp * 32; i0 < count; i0 += U * kSelThreads) {
             int page[U];
             float x[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int i = i0 + u * kSelThreads;
-                page[u] = i < count
-                              ? a.table[(int64_t)b * a.max_pages + (first + i) / a.page_size]
-                              : 0;
+                const int i = i0 + lane + u * kSelThreads;
+                page[u] = 0;
+                if (i < count) page[u] = a.table[(int64_t)b * a.max_pages + page_no(first + i)];
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int i = i0 + u * kSelThreads;
+                const int i = i0 + lane + u * kSelThreads, j = first + i;
                 x[u] = 0.0f;
                 if (i < count && page[u] >= 0 && page[u] < a.num_pages)
                     x[u] = a.scores[((int64_t)page[u] * a.kv_heads + h) * a.page_size +
-                                    (first + i) % a.page_size];
+                                    (j - page_no(j) * a.page_size)];
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int i = i0 + u * kSelThreads;
-                if (i >= count) break;
-                const bool bad = page[u] < 0 || page[u] >= a.num_pages;
-                if (bad) flag_index(a.err_word);
-                keys[i] = bad ? 0u : order_key(x[u]);
+                const int i = i0 + lane + u * kSelThreads;
+                if (i - lane >= count) break;
+                uint32_t key = order_key(x[u]);
+                if (i < count) {
+                    if (page[u] < 0 || page[u] >= a.num_pages) {
+                        flag_index(a.err_word);
+                        key = 0u;
+                    }
+                    keys[i] = key;
+                }
+                count_in(sh.hist[0], i < count, (int)(key >> 21));
             }
         }
     }
-    auto key_at = [&](int i) { return SMEM ? keys[i] : read_key(i); };
     uint32_t prefix = 0, mask = 0;
     int left = want;
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         int *hist = sh.hist[pass & 1];
-        for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i0 = warp * 32; i0 < count; i0 += kSelThreads) {
-            const int i = i0 + lane;
-            uint32_t key = 0;
-            bool in = false;
-            if (i < count) {
-                key = key_at(i);
-                in = (key & mask) == prefix;
-            }
-            const int bin = in ? (int)(key >> shift & ((1u << bits) - 1)) : -1;
-            // (equal scores are common; a warp of one bin adds once)
-            const int bin0 = __shfl_sync(0xffffffffu, bin, 0);
-            if (__all_sync(0xffffffffu, bin == bin0)) {
-                if (lane == 0 && in) atomicAdd(&hist[bin], 32);
-            } else if (in) {
-                atomicAdd(&hist[bin], 1);
+        if (pass > 0) {
+            for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
+            __syncthreads();
+        }
+        if (pass > 0 || !SMEM) {
+#pragma unroll 4
+            for (int i0 = warp * 32; i0 < count; i0 += kSelThreads) {
+                const int i = i0 + lane;
+                const uint32_t key = i < count ? key_at(i) : 0u;
+                count_in(hist, i < count && (key & mask) == prefix,
+                         (int)(key >> shift & ((1u << bits) - 1)));
             }
         }
         tc::cluster_sync_all();
-        // thread t has bins kBins - 1 - 2t and the one below, counted from the top
-        const int top = kBins - 1 - 2 * (int)threadIdx.x;
-        int h0 = 0, h1 = 0;
-        for (uint32_t r = 0; r < ranks; r++) {
-            h0 += peer_int(&hist[top], r);
-            h1 += peer_int(&hist[top - 1], r);
+        // thread t has the kPer bins from kBins - 1 - kPer * t down
+        const int top = kBins - 1 - kPer * (int)threadIdx.x;
+        int in_bin[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i += 2) {
+            int2 v[kMaxCluster];
+            if (ranks == 1) {
+                v[0] = *reinterpret_cast<const int2 *>(&hist[top - i - 1]);
+#pragma unroll
+                for (int r = 1; r < kMaxCluster; r++) v[r] = int2{0, 0};
+            } else {
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; r++)
+                    v[r] = r < (int)ranks ? peer_pair(&hist[top - i - 1], r) : int2{0, 0};
+            }
+            in_bin[i] = in_bin[i + 1] = 0;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; r++) {
+                in_bin[i] += v[r].y;
+                in_bin[i + 1] += v[r].x;
+            }
         }
-        int upto = h0 + h1;
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) mine += in_bin[i];
+        int upto = mine;
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
         }
         if (lane == 31) sh.warp_sum[warp] = upto;
         __syncthreads();
-        if (warp == 0) {
-            int v = sh.warp_sum[lane];
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += y;
-            }
-            sh.warp_eq[lane] = v;
+        // (every warp scans the warps' sums for itself)
+        int v = lane < kWarps ? sh.warp_sum[lane] : 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += y;
         }
-        __syncthreads();
-        if (warp > 0) upto += sh.warp_eq[warp - 1];
-        const int before = upto - h0 - h1;
+        const int before_warp = __shfl_sync(0xffffffffu, v, warp > 0 ? warp - 1 : 0);
+        if (warp > 0) upto += before_warp;
+        int before = upto - mine;
         if (before < left && left <= upto) {
-            const bool second = left > before + h0;
-            sh.bin = second ? top - 1 : top;
-            sh.left = left - before - (second ? h0 : 0);
+            int bin = 0, rest = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                if (before < left && left <= before + in_bin[i]) {
+                    bin = top - i;
+                    rest = left - before;
+                }
+                before += in_bin[i];
+            }
+            sh.bin = bin;
+            sh.left = rest;
         }
         __syncthreads();
         prefix |= (uint32_t)sh.bin << shift;
@@ -216,9 +266,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
         // (the next pass counts in the other histogram: peers may still read this one)
     }
     // ranks: keys above the threshold and equal to it in the places before a warp's run
-    const int run = ((count + 31) / 32 + 31) / 32 * 32;         // 32 warps, whole ballots
+    const int run = ((count + kWarps - 1) / kWarps + 31) / 32 * 32;     // whole ballots
     const int i_lo = min(count, warp * run), i_hi = min(count, i_lo + run);
     int above = 0, equal = 0;
+#pragma unroll 4
     for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
         const bool in = i0 + lane < i_hi;
         const uint32_t key = in ? key_at(i0 + lane) : 0u;
@@ -231,7 +282,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
     }
     __syncthreads();
     if (warp == 0) {
-        int x = sh.warp_sum[lane], y = sh.warp_eq[lane];
+        int x = lane < kWarps ? sh.warp_sum[lane] : 0, y = lane < kWarps ? sh.warp_eq[lane] : 0;
         const int x0 = x, y0 = y;
         for (int o = 1; o < 32; o <<= 1) {
             const int p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
@@ -256,6 +307,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const Evict a
     }
     // every key above the threshold, and the first `left` equal to it
     const uint32_t below = (1u << lane) - 1;
+#pragma unroll 4
     for (int i0 = i_lo; i0 < i_hi; i0 += 32) {
         const bool in = i0 + lane < i_hi;
         const uint32_t key = in ? key_at(i0 + lane) : 0u;
@@ -288,6 +340,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Evict a,
                                                                   int slices) {
     constexpr int U = 8;
     __shared__ int64_t from[2][kMoveRows], to[2][kMoveRows];
+    tc::grid_dependency_wait();
     const int parts = 2 * slices + 1;
     const int part = blockIdx.x % parts;
     const int bh = blockIdx.x / parts;
@@ -367,16 +420,16 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Evict a,
     }
 }
 
-template <bool SMEM>
+template <bool SMEM, int kThreads>
 int launch_select(Dev *d, const Evict &a, int ranks, size_t smem) {
-    static size_t allowed[64] = {};
-    if (smem > 24576 && smem > allowed[d->ordinal & 63]) {
-        if (int rc = check(cudaFuncSetAttribute(evict_select_kernel<SMEM>,
-                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+    static bool allowed[64] = {};
+    auto kern = evict_select_kernel<SMEM, kThreads>;
+    if (smem > 24576 && !allowed[d->ordinal & 63]) {
+        if (int rc = check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                 kSmemKeys * 4),
                            "cudaFuncSetAttribute(evict_select)"))
             return rc;
-        allowed[d->ordinal & 63] = kSmemKeys * 4;
+        allowed[d->ordinal & 63] = true;
     }
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -384,12 +437,28 @@ int launch_select(Dev *d, const Evict &a, int ranks, size_t smem) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.batch * a.kv_heads * ranks));
-    cfg.blockDim = dim3(kSelThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = d->stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return check(cudaLaunchKernelEx(&cfg, evict_select_kernel<SMEM>, a), "launch evict_select");
+    return check(cudaLaunchKernelEx(&cfg, kern, a), "launch evict_select");
+}
+
+// The move, a programmatic dependent of the choice: its launch overlaps it.
+template <typename W>
+int launch_move(Dev *d, const Evict &a, dim3 grid, int row_words, int slices) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kMoveThreads);
+    cfg.stream = d->stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return check(cudaLaunchKernelEx(&cfg, evict_move_kernel<W>, a, row_words, slices),
+                 "launch evict_move");
 }
 
 }  // namespace
@@ -427,20 +496,28 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
     if (!d) return HEXCUDA_ERR_NODEV;
     Evict a{k_pages, v_pages, scores, block_table, dst_table ? dst_table : block_table, kv_lens,
             new_lens, kept, batch, kv_heads, head_dim, num_pages, page_size, max_pages, width,
-            budget, sink, recent, d->err_word};
+            budget, sink, recent, -1, d->err_word};
+    for (int i = 0; i < 31; i++)
+        if (page_size == 1 << i) a.page_shift = i;
     launch_begin(d);
     const int bh = batch * kv_heads;
     // CTAs a sequence and key head: as many as keep the device busy, while each
-    // has some thousands of places left
+    // has some thousands of places left.  More of them than SMs: of 512 threads,
+    // so that two are resident.
     const int64_t longest = (int64_t)max_pages * page_size;
     int ranks = 1;
     while (ranks < kMaxCluster && (bh * 2 * ranks <= d->sms || longest > (int64_t)ranks * kSmemKeys) &&
-           longest > (int64_t)ranks * 4096)
+           longest > (int64_t)ranks * 8192)
         ranks *= 2;
     const int64_t per = ((longest + ranks - 1) / ranks + 31) / 32 * 32;
-    if (int rc = per <= kSmemKeys ? launch_select<true>(d, a, ranks, (size_t)per * 4)
-                                  : launch_select<false>(d, a, ranks, 0))
-        return rc;
+    const bool half = bh * (int64_t)ranks > d->sms;
+    int rc;
+    if (per <= kSmemKeys)
+        rc = half ? launch_select<true, 512>(d, a, ranks, (size_t)per * 4)
+                  : launch_select<true, 1024>(d, a, ranks, (size_t)per * 4);
+    else
+        rc = launch_select<false, 512>(d, a, ranks, 0);
+    if (rc) return rc;
     const bool vec = head_dim % 8 == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15u) == 0;
     // column slices of 64 bytes, as far as CTAs are missing
     int slices = 1;
@@ -449,9 +526,8 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
     const int per_cta = kMoveRows * slices;
     const int chunks = (int)std::min<int64_t>(((int64_t)budget + per_cta - 1) / per_cta, 65535);
     const dim3 grid((unsigned)(bh * (2 * slices + 1)), (unsigned)chunks);
-    if (vec)
-        evict_move_kernel<uint4><<<grid, kMoveThreads, 0, d->stream>>>(a, head_dim / 8, slices);
-    else
-        evict_move_kernel<uint16_t><<<grid, kMoveThreads, 0, d->stream>>>(a, head_dim, 1);
+    rc = vec ? launch_move<uint4>(d, a, grid, head_dim / 8, slices)
+             : launch_move<uint16_t>(d, a, grid, head_dim, 1);
+    if (rc) return rc;
     return launch_end(d, name, 2);
 }
