@@ -12,9 +12,10 @@
 // tok = R / group tokens a tile).  Items go to the CTAs whole, in order, CTA c
 // taking those that start in units c T / C .. (c + 1) T / C - 1.
 //
-// Per CTA (one per SM), 384 threads: warp 0 TMA of key tiles (page fragments,
-// one lane each), warp 3 TMA of query tiles, warp 1 tensor memory and MMA
-// issue, warp 2 the rows' lse * log2e (plus infinity where a row counts for
+// Per CTA (one per SM), 384 threads: warps 0 and 3 TMA of the halves of the keys
+// (page fragments, one lane each; 16-token pages make more loads than one warp
+// can start in time), warp 1 tensor memory and MMA issue, warp 2 TMA of query
+// tiles and the rows' lse * log2e (plus infinity where a row counts for
 // nothing), then a warpgroup for each half of the keys, each with two score
 // tiles in tensor memory.  256 keys to a query tile, because the query tiles
 // come from L2 again and again: with 128 keys they asked for more than L2
@@ -41,8 +42,10 @@ template <int D, int R>
 struct ScSmem {
     static constexpr int kSubs = D / 64;
     static constexpr int kTile = kSubs * kSubTile;           // 128 keys
-    static constexpr int kKStages = (R == 128 ? 2 : 3) * (128 / D);
-    static constexpr int kQStages = R == 16 ? 4 : 2;
+    // (many rows: the query tiles stream, and a load takes longer than a unit's
+    // exponentials; few: the keys do)
+    static constexpr int kKStages = (R == 128 ? 1 : 3) * (128 / D);
+    static constexpr int kQStages = R == 32 ? 2 : 4;
     static constexpr int kQTile = kSubs * R * 128;
     static constexpr int kK = 0;
     static constexpr int kQ = kK + kKStages * 2 * kTile;
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(384, 1)
             tc::mbar_init(&q_empty[i], 1);
         }
         for (int i = 0; i < KS; i++) {
-            tc::mbar_init(&k_full[i], 1);
+            tc::mbar_init(&k_full[i], 2);       // a warp for each half of the keys
             tc::mbar_init(&k_empty[i], 1);
         }
         *abort_flag = 0;
@@ -274,8 +277,9 @@ __global__ void __launch_bounds__(384, 1)
 
     if (!any) {
         // nothing to do but free the tensor memory
-    } else if (warp == 0) {
-        // ---------------------------------------------------------- TMA, keys
+    } else if (warp == 0 || warp == 3) {
+        // ------------------------------- TMA, the first and second half's keys
+        const int x = warp == 0 ? 0 : 1;
         KeyWalk w = plan.start;
         int st = 0;
         uint32_t ph = 0, armed = 0, k_ph = 0;
@@ -284,8 +288,8 @@ __global__ void __launch_bounds__(384, 1)
         // it, its page; the load is not waited for until the item's turn
         const int span = lane * a.frag;
         auto token = [&](const KeyWalk &v) {
-            const int t = v.kt * kItemKeys + span;
-            return span < kItemKeys && t < v.kv_len ? t : -1;
+            const int t = v.kt * kItemKeys + x * kKeys + span;
+            return span < kKeys && t < v.kv_len ? t : -1;
         };
         auto page_of = [&](const KeyWalk &v, int t) {
             return t < 0 ? -1 : a.s.table[(int64_t)v.b * a.s.max_pages + t / a.s.page_size];
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(384, 1)
                 tc::mbar_arrive_expect_tx(&k_full[st], (uint32_t)(count * a.frag * 128 * kSubs));
             __syncwarp();
             if (row >= 0) {
-                uint8_t *dst = smem + L::kK + (st * 2 + span / kKeys) * L::kTile + span % kKeys * 128;
+                uint8_t *dst = smem + L::kK + (st * 2 + x) * L::kTile + span * 128;
                 for (int c = 0; c < kSubs; c++)
                     tc::tma_load_2d(dst + c * kSubTile, &tmK, &k_full[st], c * 64, row);
             }
@@ -328,38 +332,15 @@ __global__ void __launch_bounds__(384, 1)
             }
         } while (more);
         if (lane == 0) {
-            // drain our own loads (a no-op when every load was consumed)
-            const uint64_t t0 = tc::globaltimer();
+            // drain our own loads (a no-op when every load was consumed; after an
+            // abort the other half's warp may not have armed the phase: 10 ms, in
+            // which any copy has landed)
+            const uint64_t t0 = tc::globaltimer(), limit = ok ? kWaitBudgetNs : 10000000ull;
             for (int i = 0; i < KS; i++)
                 if (armed >> i & 1)
                     while (!tc::mbar_try_wait(&k_full[i], k_ph >> i & 1) &&
-                           tc::globaltimer() - t0 < kWaitBudgetNs) {
+                           tc::globaltimer() - t0 < limit) {
                     }
-        }
-    } else if (warp == 3) {
-        // ------------------------------------------------------- TMA, queries
-        if (lane == 0) {
-            KeyWalk w = plan.start;
-            uint32_t u = 0;
-            bool ok = true;
-            do {
-                const int t_end = w.row_tiles(a);
-                for (int t = w.first_tile(a, 0); t < t_end; t++, u++) {
-                    const int qs = u % QS;
-                    ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word,
-                                       kErrWaitEmpty);
-                    if (!ok) break;
-                    tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
-                    for (int c = 0; c < kSubs; c++)
-                        tc::tma_load_3d(smem + L::kQ + qs * L::kQTile + c * R * 128, &tmQ, &q_full[qs],
-                                        c * 64, w.h * a.group, w.first + t * a.tok);
-                }
-            } while (ok && w.next(a));
-            const uint64_t t0 = tc::globaltimer();
-            for (uint32_t i = u > QS ? u - QS : 0; i < u; i++)
-                while (!tc::mbar_try_wait(&q_full[i % QS], (i / QS) & 1) &&
-                       tc::globaltimer() - t0 < kWaitBudgetNs) {
-                }
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -412,7 +393,7 @@ __global__ void __launch_bounds__(384, 1)
             }
         }
     } else if (warp == 2) {
-        // ------------------------------------------------- the rows' lse * log2e
+        // ------------------------------ query tiles, and the rows' lse * log2e
         constexpr int kPer = (R + 31) / 32;
         KeyWalk w = plan.start;
         float *sl = reinterpret_cast<float *>(smem + L::kLse);
@@ -433,27 +414,45 @@ __global__ void __launch_bounds__(384, 1)
         };
         float z[kPer], zn[kPer];
         int t = w.first_tile(a, 0);
-        load(t, z);
         bool more = true;
+        load(t, z);
         while (more) {
+            const int q_head = w.h * a.group, q_row = w.first + t * a.tok, qs = u % QS;
             // the next unit's values, while this one's place is waited for
             if (++t >= w.row_tiles(a)) {
                 more = w.next(a);
                 if (more) t = w.first_tile(a, 0);
             }
             if (more) load(t, zn);
-            bool ok = tc::mbar_wait(&l_empty[u & 3], ((u >> 2) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            bool ok = tc::mbar_wait(&q_empty[qs], ((u / QS) & 1) ^ 1, abort_flag, err_word, kErrWaitEmpty);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (lane == 0) {
+                tc::mbar_arrive_expect_tx(&q_full[qs], (uint32_t)(a.tok * a.group * 128 * kSubs));
+                for (int c = 0; c < kSubs; c++)
+                    tc::tma_load_3d(smem + L::kQ + qs * L::kQTile + c * R * 128, &tmQ, &q_full[qs],
+                                    c * 64, q_head, q_row);
+            }
+            u++;
+            ok = tc::mbar_wait(&l_empty[(u - 1) & 3], (((u - 1) >> 2) & 1) ^ 1, abort_flag, err_word,
+                               kErrWaitEmpty);
             if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
             for (int i = 0; i < kPer; i++)
                 if (lane + 32 * i < R)
-                    sl[(u & 3) * R + lane + 32 * i] =
+                    sl[((u - 1) & 3) * R + lane + 32 * i] =
                         z[i] == -INFINITY ? INFINITY : z[i] * 1.4426950408889634f;
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&l_full[u & 3]);
-            u++;
+            if (lane == 0) tc::mbar_arrive(&l_full[(u - 1) & 3]);
 #pragma unroll
             for (int i = 0; i < kPer; i++) z[i] = zn[i];
+        }
+        if (lane == 0) {
+            // drain our own loads
+            const uint64_t t0 = tc::globaltimer();
+            for (uint32_t i = u > QS ? u - QS : 0; i < u; i++)
+                while (!tc::mbar_try_wait(&q_full[i % QS], (i / QS) & 1) &&
+                       tc::globaltimer() - t0 < kWaitBudgetNs) {
+                }
         }
     } else {
         // ------------------------------------------------------------- weights

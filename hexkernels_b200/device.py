@@ -10,6 +10,10 @@ import ctypes as C
 from ._lib import check, load
 
 
+_PLAIN = frozenset((int, float, type(None)))
+_entries: dict[str, C._CFuncPtr] = {}
+
+
 def _arg(a):
     if hasattr(a, "data_ptr"):
         return a.data_ptr()
@@ -18,8 +22,18 @@ def _arg(a):
 
 def launch(name: str, dev: int, *args) -> None:
     """Call ``hexcuda_<name>(dev, *args)``; raises on a non-zero status."""
-    fn = getattr(load(), "hexcuda_" + name)
-    check(fn(dev, *[_arg(a) for a in args]))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), "hexcuda_" + name)
+    # (a small launch is bound by this call: numbers are told apart by type
+    # alone, and the rest is taken for a tensor first)
+    try:
+        values = [a if type(a) in _PLAIN else a.data_ptr() for a in args]
+    except AttributeError:
+        values = [_arg(a) for a in args]
+    rc = fn(dev, *values)
+    if rc:
+        check(rc)
 
 
 def bind_stream(dev: int, stream=None) -> None:
