@@ -386,7 +386,7 @@ HX_EXPORT int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_
     if (kv_heads > 0 &&
         (num_pages < 1 || page_size < 1 || (int64_t)num_pages * page_size > 0x7fffffff))
         return fail(HEXCUDA_ERR_ARG, "%s: num_pages %d page_size %d", name, num_pages, page_size);
-    if ((int64_t)heads + 2 * (int64_t)kv_heads > (1 << 20))
+    if ((int64_t)heads + 2 * (int64_t)kv_heads > (1 << 16))
         return fail(HEXCUDA_ERR_ARG, "%s: heads %d kv_heads %d", name, heads, kv_heads);
     Dev *d = get_dev(dev);
     if (!d) return HEXCUDA_ERR_NODEV;

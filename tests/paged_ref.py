@@ -63,7 +63,7 @@ class Cache:
         """The cached rows of sequence b and key head h in 64 bits."""
         n = int(self.kv_lens[b])
         j = np.arange(n)
-        return to64(pages)[self.table[b, j // self.page], h, j % self.page]
+        return to64(pages[self.table[b, j // self.page], h, j % self.page])
 
     def hidden(self, b, causal):
         n, m = int(self.kv_lens[b]), int(self.q_offs[b + 1] - self.q_offs[b])
@@ -84,7 +84,7 @@ def paged_attn(c: Cache, causal=True):
         hide = c.hidden(b, causal)
         for h in range(c.heads):
             k, v = c.rows(c.k, b, h // group), c.rows(c.v, b, h // group)
-            q = to64(c.q)[lo:hi, h]
+            q = to64(c.q[lo:hi, h])
             with np.errstate(all="ignore"):
                 x = np.where(hide, -np.inf, q @ k.T * c.scale)
                 top = x.max(1, initial=-np.inf)
@@ -121,7 +121,7 @@ def cache_scores(c: Cache, lse, scores, causal=True):
             k = c.rows(c.k, b, h)
             total, off = np.zeros(len(j)), np.zeros(len(j))
             for g in range(group):
-                q, z = to64(c.q)[lo:hi, h * group + g], lse[lo:hi, h * group + g].astype(np.float64)[:, None]
+                q, z = to64(c.q[lo:hi, h * group + g]), lse[lo:hi, h * group + g].astype(np.float64)[:, None]
                 with np.errstate(all="ignore"):
                     x = q @ k.T * c.scale
                     none = hide | (z == -np.inf)

@@ -141,6 +141,97 @@ def test_chunks(dev, n, kind):
     attn_case(dev, 50 + n, *CHUNK[n][:-1], kind, CHUNK[n][-1])
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("kv, q, heads, kv_heads, dim, page", [
+    ([500, 1, 129, 0], [1, 1, 1, 1], 8, 2, 128, 16), ([300, 77], [4, 2], 4, 1, 64, 32), ([1000], [7], 4, 1, 128, 64)])
+def test_few_tokens_without_the_causal_rule(dev, kv, q, heads, kv_heads, dim, page, kind):
+    attn_case(dev, 31, kv, q, heads, kv_heads, dim, page, kind, False)
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_many_sequences(dev, most):
+    """More sequences than a CTA has threads, most of them short, some empty."""
+    rng = np.random.default_rng(37)
+    n = 1500 if most == 1 else 500
+    kv = rng.integers(0, 300, n) * (rng.random(n) < 0.9)
+    q = np.minimum(rng.integers(0, most + 1, n), kv)
+    attn_case(dev, 38, kv.tolist(), q.tolist(), 4, 2, 64, 16, "f16", True)
+
+
+def test_a_cache_of_more_than_4g_elements(dev):
+    """A sequence at the far end of pages whose element offsets pass 32 bits."""
+    import torch
+    kv_heads, dim, page = 8, 128, 16
+    pages = 2 ** 32 // (kv_heads * dim * page) + 40
+    for q in ([1], [90]):
+        c = ref.Cache(np.random.default_rng(41), [500], q, 8, kv_heads, dim, page, "f16")
+        o = OnDevice(dev, c)
+        s = up(np.zeros(c.k.shape[:3], np.float32))
+        o.attn()
+        o.scores(s)
+        dev.sync(0)
+        want = (*o.results(), down(s, np.zeros(0, np.float32)))
+        far = pages - c.pages
+        big = []
+        for small in (o.k, o.v, s):
+            t = torch.empty((pages, *small.shape[1:]), dtype=small.dtype, device="cuda")
+            t[far:] = small if small is not s else 0
+            big.append(t)
+        o.k, o.v, s = big
+        o.table += far * (o.table < c.pages)
+        c.pages = pages
+        o.out.zero_()
+        o.attn()
+        o.scores(s)
+        dev.sync(0)
+        for a, b in zip((*o.results(), s[far:].cpu().numpy()), want):
+            np.testing.assert_array_equal(a, b)
+        # cut to 100 tokens there, and append one
+        lens, kept = o.lens.clone(), torch.empty(1, kv_heads, 100, dtype=torch.int32, device="cuda")
+        k0, v0 = o.k[far:].clone(), o.v[far:].clone()
+        dev.launch("cache_evict", 0, o.k, o.v, s, o.table, None, lens, lens, kept, 1, kv_heads, dim, pages, page, c.wide, 0, 100, 4, 10)
+        dev.sync(0)
+        place = ref.evict_kept(want[2][c.table[0, np.arange(500) // page], 3, np.arange(500) % page], 100, 4, 10)
+        np.testing.assert_array_equal(kept[0, 3].cpu().numpy(), place)
+        i = torch.arange(100)
+        j = torch.from_numpy(place)
+        tab = torch.from_numpy(c.table[0]).long()
+        for now, was in ((o.k, k0), (o.v, v0)):
+            assert torch.equal(now[far:][tab[i // page], 3, i % page], was[tab[j // page], 3, j % page])
+        x = torch.randn(3 * kv_heads * dim, device="cuda").to(torch.float16)
+        slot = torch.tensor([(pages - 1) * page + 5], dtype=torch.int32, device="cuda")
+        out = torch.empty(kv_heads * dim, dtype=torch.float16, device="cuda")
+        dev.launch("qk_norm_rope", 0, 0, x, 3 * kv_heads * dim, x[kv_heads * dim:], 3 * kv_heads * dim, x[2 * kv_heads * dim:],
+                   3 * kv_heads * dim, None, None, None, None, None, slot, out, o.k, o.v, s, 1, kv_heads, kv_heads, dim, 0, 0, 0, 0,
+                   pages, page, 0.0)
+        dev.sync(0)
+        half = o.k.view(torch.float16)
+        assert torch.equal(half[pages - 1, :, 5].flatten(), x[kv_heads * dim:2 * kv_heads * dim])
+        assert torch.equal(o.v.view(torch.float16)[pages - 1, :, 5].flatten(), x[2 * kv_heads * dim:])
+        del o, s, big, half, k0, v0
+        torch.cuda.empty_cache()
+
+
+def test_two_streams_at_once(dev):
+    """Calls in flight on two streams, each with a workspace of its own."""
+    import torch
+    rng = np.random.default_rng(43)
+    cs = [ref.Cache(rng, [3000, 200], [1, 1], 16, 4, 128, 16, "bf16"), ref.Cache(rng, [700, 900], [200, 60], 8, 2, 128, 32, "f16")]
+    os = [OnDevice(dev, c) for c in cs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    try:
+        for _ in range(5):
+            for o, st in zip(os, streams):
+                dev.bind_stream(0, st)
+                o.attn()
+        torch.cuda.synchronize()
+        for o in os:
+            check_attn(o, True)
+    finally:
+        dev.bind_stream(0)
+
+
 OTHER = [([70, 200], [3, 40], 4, 2, 80, 16), ([33], [5], 3, 1, 1, 7), ([150], [1], 2, 2, 256, 16), ([64, 9], [2, 2], 6, 3, 96, 5),
          ([130], [129], 2, 1, 128, 1), ([77], [1], 4, 1, 128, 3), ([40], [6], 2, 1, 33, 4)]
 
@@ -451,6 +542,25 @@ def test_evict_ties_and_special_scores(dev, what):
          "one ulp": np.nextafter(np.float32(1), np.float32(2), dtype=np.float32) ** rng.integers(0, 2, shape)}[what].astype(np.float32)
     for budget, sink, recent in ((1000, 4, 100), (700, 0, 0), (699, 1, 0)):
         same(evict(dev, c, s, budget, sink, recent), ref.cache_evict(c, s, budget, sink, recent))
+
+
+@pytest.mark.parametrize("wide", [600, 2000, 30000])
+def test_evict_with_wide_tables(dev, wide):
+    """Tables that could name far more tokens than there are: more CTAs to a
+    sequence, and (480000 tokens) keys that are not kept in shared memory."""
+    rng = np.random.default_rng(59)
+    c = ref.Cache(rng, [3000, 10, 7777], [0] * 3, 2, 2, 64, 16, "f16", wide=wide)
+    s = weights(rng, c)
+    for budget, sink, recent in ((1000, 4, 100), (64, 0, 0)):
+        same(evict(dev, c, s, budget, sink, recent), ref.cache_evict(c, s, budget, sink, recent))
+
+
+def test_evict_many_sequences(dev):
+    rng = np.random.default_rng(67)
+    kv = rng.integers(0, 900, 120)
+    c = ref.Cache(rng, kv.tolist(), [0] * 120, 4, 4, 64, 16, "bf16")
+    s = weights(rng, c)
+    same(evict(dev, c, s, 128, 4, 32), ref.cache_evict(c, s, 128, 4, 32))
 
 
 def test_evict_lengths_in_the_same_buffer(dev):
