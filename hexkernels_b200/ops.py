@@ -834,7 +834,9 @@ def _heads(x):
     return x, (x.strides[0] // size if T > 1 else H * D)
 
 
-def _inplace(a, shape, what):
+def _inplace(a, shape, what, dtype=None):
+    if dtype is not None and a.dtype != np.dtype(dtype):
+        raise TypeError(f"{what}: expected {np.dtype(dtype)}, got {a.dtype}")
     if not (a.flags.c_contiguous and a.flags.writeable) or a.shape != shape:
         raise ValueError(f"{what}: expected a writeable C-contiguous array of shape {shape}")
     return a
@@ -862,7 +864,7 @@ def qk_norm_rope(q, k, v, k_pages, v_pages, cos, sin, positions, slots, q_gain=N
     gains = [None if g is None else np.ascontiguousarray(g) for g in (q_gain, k_gain)]
     assert all(g is None or g.shape == (D,) for g in gains)
     if scores is not None:
-        _inplace(_c(scores, np.float32), (pages, KV, page), "scores")
+        _inplace(scores, (pages, KV, page), "scores", np.float32)
     out = np.zeros((T, H, D), q.dtype)
     pp = lambda a: None if a is None else _p(a)
     check(load().hexcuda_host_qk_norm_rope(
@@ -907,7 +909,7 @@ def cache_scores(q, lse, k_pages, block_table, kv_lens, q_offs, scores,
     q, k_pages, lse = np.ascontiguousarray(q), np.ascontiguousarray(k_pages), _c(lse, np.float32)
     table, lens, offs, dims = _paged(q, k_pages, block_table, kv_lens, q_offs, max_q)
     assert lse.shape == q.shape[:2]
-    _inplace(_c(scores, np.float32), k_pages.shape[:3], "scores")
+    _inplace(scores, k_pages.shape[:3], "scores", np.float32)
     check(load().hexcuda_host_cache_scores(
         kind, _p(q), _p(lse), _p(k_pages), _p(table), _p(lens), _p(offs), _p(scores), *dims,
         q.shape[2] ** -0.5 if scale is None else scale, int(causal)))
@@ -924,7 +926,7 @@ def cache_evict(k_pages, v_pages, scores, block_table, kv_lens, budget: int, sin
     pages, KV, page, D = k_pages.shape
     for a, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         _inplace(a, (pages, KV, page, D), what)
-    _inplace(_c(scores, np.float32), (pages, KV, page), "scores")
+    _inplace(scores, (pages, KV, page), "scores", np.float32)
     table, lens = _c(block_table, np.int32), _c(kv_lens, np.int32)
     B, wide = table.shape
     assert lens.shape == (B,)

@@ -106,6 +106,19 @@ def test_numpy_level_refusals():
         ops.cache_evict(c.k[:, :, ::2], c.v, s, c.table, c.kv_lens, 3)
     with pytest.raises(ValueError):
         ops.cache_scores(c.q, np.zeros((2, 2), np.float32), c.k, c.table, c.kv_lens, c.q_offs, s[:1])
+    # scores are written in place: a strided or read-only array is not copied and lost
+    strided = np.zeros((*s.shape[:2], 2 * s.shape[2]), np.float32)[..., ::2]
+    fixed = s.copy()
+    fixed.flags.writeable = False
+    x, tab = np.zeros((2, 1, 16), np.float16), np.ones((8, 8), np.float32)
+    for bad, error in ((strided, ValueError), (fixed, ValueError), (s.astype(np.float64), TypeError)):
+        with pytest.raises(error):
+            ops.cache_scores(c.q, np.zeros((2, 2), np.float32), c.k, c.table, c.kv_lens, c.q_offs, bad)
+        with pytest.raises(error):
+            ops.cache_evict(c.k, c.v, bad, c.table, c.kv_lens, 3)
+        with pytest.raises(error):
+            ops.qk_norm_rope(c.q, x, x, c.k, c.v, tab, tab, np.zeros(2, np.int32), np.arange(2, dtype=np.int32),
+                             scores=bad)
 
 
 # ------------------------------------------- the 64-bit implementations themselves
