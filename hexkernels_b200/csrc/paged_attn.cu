@@ -122,8 +122,9 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
 // of the item that starts in CTA c and ends in a later one, one warp per row.
 // The parts are taken in CTA order:
 //   M = max m_k,  out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
+// Rows that are not finite are looked at again (mend_row).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int item_tok) {
     tc::grid_dependency_wait();
     const int c = blockIdx.x, lane = threadIdx.x & 31;
     const PartRec r = a.recs[c];
@@ -181,12 +182,22 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a) {
         *reinterpret_cast<uint32_t *>(out) = w[0];
     if (a.lse && lane == 0)
         a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    float zero = 0.0f;      // not-a-number once a value is not finite
+#pragma unroll
+    for (int v = 0; v < V; v++) zero = fmaf(acc[v] * inv, 0.0f, zero);
+    if (__any_sync(0xffffffffu, zero != 0.0f) && a.s.causal) {
+        const int b = a.recs[c].b, t0 = a.recs[c].rt * item_tok;
+        int first, q_len, kv_len;
+        quiet_seq(a.s, b, first, q_len, kv_len);
+        mend_row<T, D>(a, b, at, r.h * a.group + i % a.group, seen_by(a.s, kv_len, q_len, t0 + t),
+                       min(kv_len, tiles_to(a.s, kv_len, q_len, t0 + item_tok) * kKeys));
+    }
 }
 
 // The join starts while the kernel before it on the stream still runs, and
 // waits for it on the device (a programmatic dependent launch).
 template <typename T, int D>
-int launch_join(Dev *d, const PagedTc &a, int rows) {
+int launch_join(Dev *d, const PagedTc &a, int rows, int item_tok) {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -196,7 +207,7 @@ int launch_join(Dev *d, const PagedTc &a, int rows) {
     cfg.stream = d->stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return check(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a), "launch paged_join");
+    return check(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a, item_tok), "launch paged_join");
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
@@ -309,6 +320,9 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
         a.map_rows = num_pages * kv_heads * page_size;
         a.min_units = 2;
         a.scale_log2 = scale * 1.4426950408889634f;
+        a.q = q;
+        a.k = k_pages;
+        a.v = v_pages;
         a.out = out;
         a.lse = lse;
         uint8_t *p = reinterpret_cast<uint8_t *>(workspace);
@@ -326,11 +340,12 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
             return rc;
         const bool half = dtype == HEXCUDA_F16;
         const int join_rows = few ? n : 2 * n;      // of one item
+        const int item_tok = few ? a.tok : 2 * a.tok;
         if (int rc = head_dim == 128
-                         ? (half ? launch_join<__half, 128>(d, a, join_rows)
-                                 : launch_join<__nv_bfloat16, 128>(d, a, join_rows))
-                         : (half ? launch_join<__half, 64>(d, a, join_rows)
-                                 : launch_join<__nv_bfloat16, 64>(d, a, join_rows)))
+                         ? (half ? launch_join<__half, 128>(d, a, join_rows, item_tok)
+                                 : launch_join<__nv_bfloat16, 128>(d, a, join_rows, item_tok))
+                         : (half ? launch_join<__half, 64>(d, a, join_rows, item_tok)
+                                 : launch_join<__nv_bfloat16, 64>(d, a, join_rows, item_tok)))
             return rc;
         note_mech(kMechTcgen05 | kMechTma);
         return launch_end(d, "paged_attn", 2);

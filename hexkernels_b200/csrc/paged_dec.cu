@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t *k_full = bars + 15, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *odd_flag = abort_flag + 1;     // an output that is not finite
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err_word = a.s.err_word;
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(384, 1)
             tc::mbar_init(&v_empty[i], 1);
         }
         *abort_flag = 0;
+        *odd_flag = 0;
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmQ);
         tc::tma_prefetch_desc(&tmK);
@@ -482,16 +484,21 @@ __global__ void __launch_bounds__(384, 1)
             if (key < D) {
                 if (whole) {
                     int t = n0 / a.group, i = n0 % a.group;
+                    float zero = 0.0f;          // not-a-number once a value is not finite
 #pragma unroll
                     for (int n = 0; n < C; n++) {
-                        if (n0 + n < nrows)
+                        if (n0 + n < nrows) {
+                            const float y = __uint_as_float(o[n]) * res[n0 + n];
+                            zero = fmaf(y, 0.0f, zero);
                             out[((int64_t)(w.first + t0 + t) * a.heads + w.h * a.group + i) * D + key] =
-                                from_f32<T>(__uint_as_float(o[n]) * res[n0 + n]);
+                                from_f32<T>(y);
+                        }
                         if (++i == a.group) {
                             i = 0;
                             t++;
                         }
                     }
+                    if (zero != 0.0f) *odd_flag = 1;
                 } else {
                     float *po = a.part_o + ((size_t)slot * kPartRows + n0) * D + key;
 #pragma unroll
@@ -514,6 +521,8 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         tc::tmem_dealloc(tmem_base, kCols);
     }
+    if (warp >= 4 && a.s.causal && *odd_flag && !*abort_flag)
+        mend_items<T, D>(a, plan.start, a.tok, warp - 4);
 }
 
 template <typename T, int D, int N>

@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t *k_full = bars + 14, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *odd_flag = abort_flag + 1;     // an output that is not finite
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err_word = a.s.err_word;
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(384, 1)
             tc::mbar_init(&v_empty[i], 1);
         }
         *abort_flag = 0;
+        *odd_flag = 0;
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmQ);
         tc::tma_prefetch_desc(&tmK);
@@ -591,6 +593,10 @@ __global__ void __launch_bounds__(384, 1)
                     if (whole) {
                         uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + orow * D +
                                                                cc * 32);
+                        float zero = 0.0f;      // not-a-number once a value is not finite
+#pragma unroll
+                        for (int e = 0; e < 32; e++) zero = fmaf(__uint_as_float(o[e]), 0.0f, zero);
+                        if (zero != 0.0f) *odd_flag = 1;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             uint32_t v[4];
@@ -640,6 +646,8 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         tc::tmem_dealloc(tmem_base, 512);
     }
+    if (warp >= 4 && a.s.causal && *odd_flag && !*abort_flag)
+        mend_items<T, D>(a, plan.start, item_tok, warp - 4);
 }
 
 template <typename T, int D>

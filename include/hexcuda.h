@@ -512,8 +512,7 @@ int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, con
  * causal != 0 new token t of q_len sees cached tokens up to its own place
  * kv_len - q_len + t; without it every cached token (cross attention over an
  * encoder's states).  Nothing past kv_lens[b] is used, whatever it holds
- * (not-a-number included).  A new token's own K and V must be finite when
- * other tokens of its chunk are to be.
+ * (not-a-number included), and a row is not touched by what it does not see.
  * Tables, lengths, offsets, slots and positions are device data: an entry out
  * of range is skipped, never followed, and the next hexcuda_sync returns
  * HEXCUDA_ERR_ARG.  Page, token and row counts are below 2^31; element offsets

@@ -317,6 +317,53 @@ def test_a_non_finite_sequence_leaves_the_others(dev):
         near(lse[lo:hi, 2:], z[lo:hi, 2:], b_lse[lo:hi, 2:])
 
 
+LATER = [   # kv, q, heads, kv_heads, dim, page: single tiles and pairs, whole items and cut ones
+    ([300] * 40, [4] * 40, 4, 1, 128, 16), ([5000], [3], 10, 2, 128, 16), ([700] * 30, [7, 8] * 15, 4, 1, 64, 16),
+    ([90] * 80, [40] * 80, 4, 2, 64, 16), ([4000], [60], 4, 2, 128, 16), ([200] * 90, [200] * 90, 4, 2, 128, 32),
+    ([1500], [400], 2, 2, 64, 64), ([33, 20], [33, 50], 4, 1, 80, 16), ([40] * 20, [90] * 20, 2, 1, 128, 16),
+]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n", range(len(LATER)), ids=lambda n: "-".join(map(str, LATER[n][2:])) + f"x{len(LATER[n][0])}")
+def test_later_tokens_that_are_not_finite(dev, n, kind):
+    """Rows before a token whose key or values are not finite do not know of it."""
+    kv, q, heads, kv_heads, dim, page = LATER[n]
+    rng = np.random.default_rng(70 + n)
+    c = ref.Cache(rng, kv, q, heads, kv_heads, dim, page, kind, fill=np.nan)
+    k, v = ref.to64(c.k), ref.to64(c.v)
+    first, second = np.zeros(len(kv), int), np.zeros(len(kv), int)
+    for b, (n_kv, n_q) in enumerate(zip(kv, q)):
+        new = min(n_q, n_kv)
+        first[b], second[b] = sorted(rng.integers(n_kv - new + 1, n_kv, 2)) if new > 2 else (n_kv - 1, n_kv - 1)
+        at = lambda j: (c.table[b, j // page], slice(None), j % page)
+        v[at(first[b])] = np.where(np.arange(dim) < 5, np.nan, np.where(np.arange(dim) < 8, -np.inf, v[at(first[b])]))
+        v[at(second[b])] = np.where(np.arange(dim) % 7 == 3, np.inf, v[at(second[b])])
+        k[at(second[b])] = np.nan
+    c.k, c.v = ref.to16(k, kind), ref.to16(v, kind)
+    o = OnDevice(dev, c)
+    o.attn()
+    dev.sync(0)
+    out, lse = o.results()
+    # what no key of a row is, it must not see: the expected values come from finite keys
+    c.k = ref.to16(np.where(np.isnan(k), 0.0, k), kind)
+    want, z, b_out, b_lse = ref.paged_attn(c)
+    got = ref.to64(out)
+    for b, (n_kv, n_q) in enumerate(zip(kv, q)):
+        rows = np.arange(c.q_offs[b], c.q_offs[b + 1])
+        sees = n_kv - n_q + np.arange(n_q)                 # the last token that each sees
+        before = rows[sees < first[b]]
+        near(out[before], want[before], b_out[before], f"sequence {b} before")
+        near(lse[before], z[before], b_lse[before], f"sequence {b} lse before")
+        if first[b] < second[b]:
+            mid = rows[(sees >= first[b]) & (sees < second[b])]
+            assert np.isnan(got[mid][..., :5]).all() and (got[mid][..., 5:8] == -np.inf).all()
+            near(out[mid][..., 8:], want[mid][..., 8:], b_out[mid][..., 8:], f"sequence {b} between")
+            near(lse[mid], z[mid], b_lse[mid], f"sequence {b} lse between")
+        last = rows[sees >= second[b]]
+        assert np.isnan(got[last]).all() and np.isnan(lse[last]).all()
+
+
 @pytest.mark.parametrize("dim", [128, 64, 80])
 @pytest.mark.parametrize("q", [[1, 1, 1], [60, 35, 50]])
 def test_bad_indices_are_skipped_and_reported(dev, dim, q):
