@@ -9,10 +9,10 @@
 // and 4000 at dim 128).  The units of all items, in that order, are numbered
 // 0 .. T - 1 and CTA c of C takes the key tiles that start in units c T / C ..
 // (c + 1) T / C - 1: a run of items, the first and the last perhaps only in
-// part.  Lengths live on the device, so each CTA derives its own run from them (a prefix sum over the
-// sequences).  An item that is cut leaves one partial result per CTA: the
-// unnormalised output, the reference maximum and the sum of each row.  A
-// second kernel joins them, in CTA order, so results do not depend on timing.
+// part.  Lengths live on the device, so each CTA derives its own run from them (a
+// prefix sum over the sequences).  An item that is cut leaves one partial result
+// per CTA: the unnormalised output, the reference maximum and the sum of each row.
+// A second kernel joins them, in CTA order, so results do not depend on timing.
 #pragma once
 #include "paged.cuh"
 #include "tc_common.cuh"

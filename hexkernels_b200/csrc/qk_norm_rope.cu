@@ -9,7 +9,9 @@
 //                                              row position of the tables
 //
 // Everything between the load and the one rounding at the store is fp32.
-// HBM-bound: each row is read once and written once, 4 bytes a value.
+// HBM-bound: each row is read once and written once, 4 bytes a value.  Measured
+// with 32 + 2 x 8 heads of 128: 16384 tokens 82 us for 411 MB, 5.0 TB/s (a copy 6.5);
+// one token 4.5 us on the device.
 #include "ew_launch.cuh"
 #include "paged.cuh"
 
@@ -324,7 +326,9 @@ void launch_wide(Dev *d, const NormRope &a) {
     const int rows = a.heads + a.kv_heads * (a.v ? 2 : 1);
     constexpr int kRows = kWideThreads / LPR;
     const int all = (rows + kRows - 1) / kRows;
-    // few tokens: a block per pass, so that a token's rows go out at once
+    // few tokens: a block per pass, so that a token's rows go out at once (16 and 64
+    // tokens 6.1 us, with U passes a block 8.2; 4096 tokens 32.7 and 26.6, from 253
+    // to 1200 the same)
     const int passes = a.tokens < 4 * d->sms ? 1 : all < U ? all : U;
     const dim3 grid((unsigned)a.tokens, (unsigned)((all + passes - 1) / passes));
     norm_rope_kernel<T, LPR, HALVES><<<grid, kWideThreads, 0, d->stream>>>(a, passes);
@@ -337,7 +341,7 @@ void launch_halves(Dev *d, const NormRope &a) {
         launch_wide<T, LPR, false>(d, a);
 }
 template <typename T>
-void launch_rows(Dev *d, const NormRope &a) {
+void launch_norm_rope(Dev *d, const NormRope &a) {
     if (!wide_rows(a)) {
         constexpr auto kern = norm_rope_any_kernel<T>;
         const int64_t rows = (int64_t)a.tokens * (a.heads + a.kv_heads * (a.v ? 2 : 1));
@@ -424,8 +428,8 @@ HX_EXPORT int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_
     a.err_word = d->err_word;
     launch_begin(d);
     if (dtype == HEXCUDA_F16)
-        launch_rows<__half>(d, a);
+        launch_norm_rope<__half>(d, a);
     else
-        launch_rows<__nv_bfloat16>(d, a);
+        launch_norm_rope<__nv_bfloat16>(d, a);
     return launch_end(d, name);
 }

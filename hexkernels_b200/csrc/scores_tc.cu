@@ -8,8 +8,8 @@
 // made by one CTA, in a fixed order, and added to the cache once.
 //
 // A work item is (sequence, key head, 256 keys); it costs one unit per query
-// tile that sees it (R = 16 or 32 rows when a key head has that few, else 128;
-// tok = R / group tokens a tile).  Items go to the CTAs whole, in order, CTA c
+// tile that sees it (R = 16 or 32 rows when a key head has few, else 128; tok =
+// R / group tokens a tile).  Items go to the CTAs whole, in order, CTA c
 // taking those that start in units c T / C .. (c + 1) T / C - 1.
 //
 // Per CTA (one per SM), 384 threads: warps 0 and 3 TMA of the halves of the keys
@@ -19,8 +19,12 @@
 // nothing), then a warpgroup for each half of the keys, each with two score
 // tiles in tensor memory.  256 keys to a query tile, because the query tiles
 // come from L2 again and again: with 128 keys they asked for more than L2
-// gives.  With few rows the kernel is bound by HBM (each key once); with many
-// by the exponentials, one per score.
+// gives.  With few rows the kernel is bound by HBM (each key once): 64 sequences of
+// 8192, one new token, 32 heads of 128 over 8 key heads: 107 us for 563 MB, 5.2
+// TB/s.  With many it is bound by the exponentials, one per score: 3 x 1000 new tokens
+// of 6000: 129 us, a unit of 256 keys x 128 rows taking 3000 cycles, 2048 of them
+// the MUFU's.  Items are not cut (a key's sum would need a second pass or lose its
+// fixed order): there the busiest CTA has 64 units for 54 on average.
 //
 // Every wait is bounded; see mbar_wait.
 #include <math.h>
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 template <typename T, int D, int R>
-int launch(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a) {
+int launch_scores(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a) {
     using L = ScSmem<D, R>;
     static_assert(L::kTotal <= 232448, "shared memory of one CTA");
     static bool attr_done[64] = {};
@@ -537,10 +541,10 @@ int launch(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc 
 }
 
 template <typename T, int D>
-int launch_rows(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a, int rows) {
-    if (rows == 16) return launch<T, D, 16>(d, mq, mk, a);
-    if (rows == 32) return launch<T, D, 32>(d, mq, mk, a);
-    return launch<T, D, 128>(d, mq, mk, a);
+int launch_scores_rows(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const ScoresTc &a, int rows) {
+    if (rows == 16) return launch_scores<T, D, 16>(d, mq, mk, a);
+    if (rows == 32) return launch_scores<T, D, 32>(d, mq, mk, a);
+    return launch_scores<T, D, 128>(d, mq, mk, a);
 }
 
 }  // namespace
@@ -554,7 +558,10 @@ int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const
     a.kv_heads = kv_heads;
     a.group = heads / kv_heads;
     const int64_t need = (int64_t)(max_q < 1 ? 1 : max_q) * a.group;
-    const int rows = need <= 16 ? 16 : need <= 32 ? 32 : 128;
+    // Query tiles of 16, 32 or 128 rows.  Measured (us, dim 128, 8 key heads): 64
+    // sequences of 8192, 4 rows to a key head: 195 / 201 / 393; 16 of 4096, 32 rows: 47
+    // / 39 / 59, 64 rows: 74 / 49 / 61, 80 rows: 86 / 64 / 61, 128 rows: 119 / 74 / 57.
+    const int rows = need <= 16 ? 16 : need <= 64 ? 32 : 128;
     a.tok = rows / a.group;
     const int low = s.page_size & -s.page_size;
     a.frag = low < kKeys ? low : kKeys;
@@ -567,10 +574,10 @@ int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const
     if (int rc = make_page_map(&mk, k, a.map_rows, dim, a.frag)) return rc;
     note_mech(kMechTcgen05 | kMechTma);
     if (dtype == HEXCUDA_F16)
-        return dim == 128 ? launch_rows<__half, 128>(d, mq, mk, a, rows)
-                          : launch_rows<__half, 64>(d, mq, mk, a, rows);
-    return dim == 128 ? launch_rows<__nv_bfloat16, 128>(d, mq, mk, a, rows)
-                      : launch_rows<__nv_bfloat16, 64>(d, mq, mk, a, rows);
+        return dim == 128 ? launch_scores_rows<__half, 128>(d, mq, mk, a, rows)
+                          : launch_scores_rows<__half, 64>(d, mq, mk, a, rows);
+    return dim == 128 ? launch_scores_rows<__nv_bfloat16, 128>(d, mq, mk, a, rows)
+                      : launch_scores_rows<__nv_bfloat16, 64>(d, mq, mk, a, rows);
 }
 
 }  // namespace hx

@@ -427,6 +427,15 @@ def test_no_lse_and_any_max_q(dev):
             near(down(s, np.zeros(0, np.float32)), want, bound, f"q {q} max_q {max_q}")
 
 
+def test_output_must_not_be_the_queries(dev):
+    from hexkernels_b200 import HexcudaError
+    c = ref.Cache(np.random.default_rng(4), [40], [3], 4, 1, 64, 16)
+    o = OnDevice(dev, c)
+    o.out = o.q
+    with pytest.raises(HexcudaError, match="out is q"):
+        o.attn()
+
+
 def test_workspace_must_be_large_enough(dev):
     from hexkernels_b200 import HexcudaError
     c = ref.Cache(np.random.default_rng(1), [30], [1], 4, 1, 64, 16)
