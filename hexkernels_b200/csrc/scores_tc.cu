@@ -561,7 +561,8 @@ int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const
     // Query tiles of 16, 32 or 128 rows.  Measured (us, dim 128, 8 key heads): 64
     // sequences of 8192, 4 rows to a key head: 195 / 201 / 393; 16 of 4096, 32 rows: 47
     // / 39 / 59, 64 rows: 74 / 49 / 61, 80 rows: 86 / 64 / 61, 128 rows: 119 / 74 / 57.
-    const int rows = need <= 16 ? 16 : need <= 64 ? 32 : 128;
+    // A tile holds a token's heads.
+    const int rows = need <= 16 ? 16 : need <= 64 && a.group <= 32 ? 32 : 128;
     a.tok = rows / a.group;
     const int low = s.page_size & -s.page_size;
     a.frag = low < kKeys ? low : kKeys;

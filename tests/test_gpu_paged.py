@@ -126,6 +126,12 @@ def test_single_tokens(dev, n, kind):
     attn_case(dev, 10 + n, *DECODE[n], kind, True)
 
 
+@pytest.mark.parametrize("group", [15, 16, 17, 31, 32, 33, 64, 65, 128, 129])
+@pytest.mark.parametrize("most", [1, 2])
+def test_many_heads_to_a_key_head(dev, group, most):
+    attn_case(dev, 300 + group, [150, 20], [most, 1], 2 * group, 2, 64, 16, "bf16", True)
+
+
 CHUNK = [
     ([300], [300], 4, 2, 128, 16, True), ([300], [77], 8, 2, 128, 16, True), ([700, 129, 1], [300, 129, 1], 4, 4, 64, 32, True),
     ([1000, 250, 0, 40], [200, 250, 0, 8], 10, 2, 128, 16, True), ([50, 600, 7], [70, 100, 9], 8, 1, 64, 16, True),
