@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int it
 #pragma unroll 4
         for (int k = 0; k < n; k++) {
             const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float *o = a.part_o + slot(k0 + k) * D + lane * V;
+            const float *o = a.part_o + (slot(k0 + k) - row) * D + (int64_t)row * a.part_row +
+                             lane * V / 4 * a.part_col + lane * V % 4;
             float x[V];
             if constexpr (V == 4)
                 *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(o);
@@ -337,6 +338,9 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
         p += round_up(sizeof(PartRec) * d->sms, 256);
         a.part_ml = reinterpret_cast<float *>(p);
         a.part_o = a.part_ml + (size_t)d->sms * 2 * kPartRows * 2;
+        // single tokens: the columns are in a warp's lanes; chunks: the rows are
+        a.part_row = few ? head_dim : 4;
+        a.part_col = few ? 4 : 4 * kPartRows;
         CUtensorMap mq, mk, mv;
         if (int rc = make_query_map(&mq, q, total_q, heads, head_dim, group, a.tok)) return rc;
         if (int rc = make_page_map(&mk, k_pages, a.map_rows, head_dim, a.frag)) return rc;

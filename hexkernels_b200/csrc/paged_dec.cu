@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(384, 1)
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    const bool any = plan_run<384>(a, a.tok, plan);
+    const bool any = plan_run<384, 0>(a, a.tok, plan);
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_o = tmem_base + 2 * N;

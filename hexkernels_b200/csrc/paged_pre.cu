@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(384, 1)
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    const bool any = plan_run<384>(a, item_tok, plan);
+    const bool any = plan_run<384, 5>(a, item_tok, plan);
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     constexpr uint32_t kColO = 256;
@@ -614,10 +614,14 @@ __global__ void __launch_bounds__(384, 1)
                             dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
                         }
                     } else {
-                        uint4 *dst = reinterpret_cast<uint4 *>(a.part_o + prow * D + cc * 32);
+                        // (a row's neighbours are four columns of the next row: a
+                        // warp stores 512 bytes in one piece)
+                        uint4 *dst = reinterpret_cast<uint4 *>(a.part_o) +
+                                     (prow - x * 128 - row) * (D / 4) + x * 128 + row;
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            dst[(cc * 8 + e) * kPartRows] =
+                                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                 }
                 tc::tc_fence_before();

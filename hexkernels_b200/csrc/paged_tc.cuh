@@ -6,7 +6,10 @@
 // and takes ceil(keys its last row sees / 128) key tiles, at least one (a row
 // that sees nothing is still written).  A key tile costs one unit, or two when
 // the item has two query tiles (measured 1700 and 3300 cycles at dim 64, 2600
-// and 4000 at dim 128).  The units of all items, in that order, are numbered
+// and 4000 at dim 128), and an item of a chunk five more for its queries, its first
+// loads and its output (some 9000 cycles; when the CTAs have at least eight units:
+// 40 x 40 new tokens of 3000, 16 heads of 64: 142 us without them, 108 with five, 110
+// with three and 108 with eight).  The units of all items, in that order, are numbered
 // 0 .. T - 1 and CTA c of C takes the key tiles that start in units c T / C ..
 // (c + 1) T / C - 1: a run of items, the first and the last perhaps only in
 // part.  Lengths live on the device, so each CTA derives its own run from them (a
@@ -42,7 +45,8 @@ struct PagedTc {
     float *lse;
     PartRec *recs;           // [grid]
     float *part_ml;          // [grid][2][kPartRows][2]: reference maximum, sum
-    float *part_o;           // [grid][2][kPartRows][D]
+    float *part_o;           // [grid][2] outputs of kPartRows x D, whose rows and groups
+    int part_row, part_col;  // of four columns are so many floats apart
 };
 
 // Tokens of a sequence without raising the error word (the plan has).
@@ -70,7 +74,7 @@ __device__ __forceinline__ int units_of(const PagedTc &a, int item_tok, int q_le
 // A CTA's run of items, one segment (item, key tiles j0 .. j1 - 1) at a time.
 // Every role of the CTA walks its own copy.
 struct Walk {
-    int b, h, rt, j0, j1, nt, cost;
+    int b, h, rt, j0, j1, nt, cost, extra;
     int first, q_len, kv_len;
     long long pos, end;      // first unit of the segment, end of the run
 
@@ -78,11 +82,13 @@ struct Walk {
     __device__ __forceinline__ void open(const PagedTc &a, int item_tok) {
         nt = tiles_to(a.s, kv_len, q_len, (rt + 1) * item_tok);
         cost = units_of(a, item_tok, q_len, rt);
-        const long long left = (end - pos + cost - 1) / cost;
+        // (the first key tile's unit is followed by the item's extra ones)
+        const long long room = end - pos - (j0 == 0 ? extra : 0);
+        const long long left = room > 0 ? (room + cost - 1) / cost : 1;
         j1 = left < nt - j0 ? j0 + (int)left : nt;
     }
     __device__ __forceinline__ bool next(const PagedTc &a, int item_tok) {
-        pos += (long long)(j1 - j0) * cost;
+        pos += (long long)(j1 - j0) * cost + (j0 == 0 ? extra : 0);
         if (pos >= end) return false;
         j0 = 0;
         if (++rt * item_tok >= q_len) {
@@ -101,7 +107,7 @@ struct Walk {
 };
 
 struct PlanShared {
-    long long sums[32];
+    long long sums[32], items[32];
     Walk start;
     int ctas;
     long long total;
@@ -109,36 +115,56 @@ struct PlanShared {
 
 // Whole block.  Leaves this CTA's first segment in sh.start; false when it has
 // none.  item_tok: tokens of an item (one or two query tiles).
-template <int THREADS>
+// EXTRA: units that an item costs beside its key tiles.
+template <int THREADS, int EXTRA>
 __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanShared &sh) {
     const int per = (a.s.batch + THREADS - 1) / THREADS;
     const int b0 = min(a.s.batch, (int)threadIdx.x * per), b1 = min(a.s.batch, b0 + per);
-    auto units = [&](int q_len, int kv_len) {       // of one key head
+    auto units = [&](int q_len, int kv_len) {       // of one key head's key tiles
         long long n = 0;
         for (int rt = 0; rt * item_tok < q_len; rt++)
             n += (long long)tiles_to(a.s, kv_len, q_len, (rt + 1) * item_tok) *
                  units_of(a, item_tok, q_len, rt);
         return n;
     };
-    long long mine = 0;
+    auto items = [&](int q_len) { return (q_len + item_tok - 1) / item_tok; };
+    long long mine = 0, mine_items = 0;
     for (int b = b0; b < b1; b++) {
         int first;
         const int q_len = seq_q_len(a.s, b, first), kv_len = seq_kv_len(a.s, b);
         mine += units(q_len, kv_len) * a.kv_heads;
+        if (EXTRA) mine_items += (long long)items(q_len) * a.kv_heads;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long upto = mine;
+    long long upto = mine, upto_items = mine_items;
     for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
+        const long long z = EXTRA ? __shfl_up_sync(0xffffffffu, upto_items, o) : 0;
+        if (lane >= o) {
+            upto += y;
+            upto_items += z;
+        }
     }
-    if (lane == 31) sh.sums[warp] = upto;
+    if (lane == 31) {
+        sh.sums[warp] = upto;
+        if (EXTRA) sh.items[warp] = upto_items;
+    }
     __syncthreads();
-    long long total = 0;
+    long long total = 0, total_items = 0;
     for (int w = 0; w < THREADS / 32; w++) {
-        if (w < warp) upto += sh.sums[w];
+        if (w < warp) {
+            upto += sh.sums[w];
+            if (EXTRA) upto_items += sh.items[w];
+        }
         total += sh.sums[w];
+        if (EXTRA) total_items += sh.items[w];
     }
+    // (a run must be longer than a first key tile with the extra units, so that
+    // some key tile starts in it)
+    const int extra = total >= (EXTRA + 3LL) * gridDim.x ? EXTRA : 0;
+    mine += mine_items * extra;
+    upto += upto_items * extra;
+    total += total_items * extra;
     const long long want = max(total / a.min_units, total > 0 ? 1LL : 0LL);
     const int ctas = want < (int)gridDim.x ? (int)want : (int)gridDim.x;
     const bool any = (int)blockIdx.x < ctas;
@@ -149,7 +175,7 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
             Walk w;
             for (int b = b0; b < b1; b++) {
                 quiet_seq(a.s, b, w.first, w.q_len, w.kv_len);
-                const long long n = units(w.q_len, w.kv_len);
+                const long long n = units(w.q_len, w.kv_len) + (long long)items(w.q_len) * extra;
                 if (at >= n * a.kv_heads) {
                     at -= n * a.kv_heads;
                     continue;
@@ -159,7 +185,8 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
                 at -= w.h * n;
                 for (w.rt = 0;; w.rt++) {
                     const int units = tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok) *
-                                      units_of(a, item_tok, w.q_len, w.rt);
+                                          units_of(a, item_tok, w.q_len, w.rt) +
+                                      extra;
                     if (at < units) break;
                     at -= units;
                 }
@@ -167,8 +194,10 @@ __device__ __forceinline__ bool plan_run(const PagedTc &a, int item_tok, PlanSha
             }
             // the first key tile that starts here: perhaps the next item's first
             w.cost = units_of(a, item_tok, w.q_len, w.rt);
-            w.j0 = w.j1 = (int)((at + w.cost - 1) / w.cost);
-            w.pos = lo + (w.j0 * w.cost - at);
+            w.extra = extra;
+            w.j0 = at == 0 ? 0 : max(1, ((int)at - extra + w.cost - 1) / w.cost);
+            w.j1 = w.j0;
+            w.pos = lo + (w.j0 == 0 ? 0 : w.j0 * w.cost + extra - at);
             w.end = hi;
             if (w.j0 < tiles_to(a.s, w.kv_len, w.q_len, (w.rt + 1) * item_tok))
                 w.open(a, item_tok);
@@ -191,7 +220,7 @@ __device__ __forceinline__ void note_parts(const PagedTc &a, const PlanShared &s
     PartRec r = {};
     if (w.j0 == 0 && w.j1 < w.nt) {
         // the CTA where the item's last tile starts, in unit u: the largest c with c T / C <= u
-        const long long u = w.pos + (long long)(w.nt - 1) * w.cost;
+        const long long u = w.pos + (long long)(w.nt - 1) * w.cost + w.extra;
         r.h = w.h;
         r.row0 = w.first + w.rt * item_tok;
         r.ntok = min(item_tok, w.q_len - w.rt * item_tok);
