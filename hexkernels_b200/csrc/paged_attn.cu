@@ -119,80 +119,91 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
 }
 
 // Joins the parts of the items that several CTAs worked on: block (c, y) those
-// of the item that starts in CTA c and ends in a later one, one warp per row.
-// The parts are taken in CTA order:
+// of the item that starts in CTA c and ends in a later one, half a warp a row, so
+// that two rows' groups of four columns, neighbours in a chunk's parts, make whole
+// sectors.  The parts are taken in CTA order:
 //   M = max m_k,  out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
-// Rows that are not finite are looked at again (mend_row).  A row a warp and 32 to 48
-// registers: 13 us for 11 chunks of 301 tokens of 64, 21 us for 148 items of 256 rows
-// of 128 (four rows a warp 14 and 18, but the whole call 3 us slower and the same).
+// Rows that are not finite are looked at again (mend_row).  Bound by latency: 10.8 us
+// for 11 chunks of 301 tokens of 64 (a warp a row: 15.6), 19 us for 148 items of 256
+// rows of 128, 5.3 us for one token.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int item_tok) {
     tc::grid_dependency_wait();
-    const int c = blockIdx.x, lane = threadIdx.x & 31;
+    const int c = blockIdx.x, lane = threadIdx.x & 31, sub = lane >> 4, l16 = lane & 15;
     const PartRec r = a.recs[c];
-    const int i = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (r.nparts == 0 || i >= r.ntok * a.group) return;
-    const int t = i / a.group;
+    const int i0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 2, n = r.ntok * a.group;
+    if (r.nparts == 0 || i0 >= n) return;
+    const bool live = i0 + sub < n;         // (the last row again for one behind it)
+    const int i = live ? i0 + sub : n - 1, t = i / a.group;
     const int row = t / a.tok * 128 + (t % a.tok) * a.group + i % a.group;
-    auto slot = [&](int k) { return ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * kPartRows + row; };
+    auto slot = [&](int k) { return ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * kPartRows; };
     const float2 *mls = reinterpret_cast<const float2 *>(a.part_ml);
     float top = -INFINITY;
-    for (int k = lane; k < r.nparts; k += 32) {
-        const float2 ml = mls[slot(k)];
+    for (int k = l16; k < r.nparts; k += 16) {
+        const float2 ml = mls[slot(k) + row];
         if (ml.y != 0.0f) top = fmaxf(top, ml.x);
     }
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    constexpr int V = D / 32;
-    float acc[V], sum = 0.0f;
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int G = D / 64;               // groups of four columns of a lane
+    float acc[G][4], sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; v++) acc[v] = 0.0f;
-    // 32 parts at a time: lane k has part k's weight, then all lanes add up rows
-    for (int k0 = 0; k0 < r.nparts; k0 += 32) {
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) acc[g][v] = 0.0f;
+    const float *parts = a.part_o + (int64_t)row * a.part_row + l16 * a.part_col;
+    // 16 parts at a time: lane k has part k's weight, then all lanes add up rows
+    for (int k0 = 0; k0 < r.nparts; k0 += 16) {
         float w = 0.0f, l = 0.0f;
-        if (k0 + lane < r.nparts) {
-            const float2 ml = mls[slot(k0 + lane)];
+        if (k0 + l16 < r.nparts) {
+            const float2 ml = mls[slot(k0 + l16) + row];
             // (a part without a visible key has no output)
             if (ml.y != 0.0f) w = tc::ex2(ml.x - top);
             l = w * ml.y;
         }
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         sum += l;
-        const int n = min(32, r.nparts - k0);
-#pragma unroll 4
-        for (int k = 0; k < n; k++) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float *o = a.part_o + (slot(k0 + k) - row) * D + (int64_t)row * a.part_row +
-                             lane * V / 4 * a.part_col + lane * V % 4;
-            float x[V];
-            if constexpr (V == 4)
-                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(o);
-            else
-                *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(o);
+        const int m = min(16, r.nparts - k0);
+#pragma unroll 2
+        for (int k = 0; k < m; k++) {
+            const float wk = __shfl_sync(0xffffffffu, w, k, 16);
 #pragma unroll
-            for (int v = 0; v < V; v++)
-                if (wk != 0.0f) acc[v] += wk * x[v];
+            for (int g = 0; g < G; g++) {
+                const float4 x = *reinterpret_cast<const float4 *>(parts + slot(k0 + k) * D +
+                                                                   16 * g * a.part_col);
+                if (wk == 0.0f) continue;
+                acc[g][0] += wk * x.x;
+                acc[g][1] += wk * x.y;
+                acc[g][2] += wk * x.z;
+                acc[g][3] += wk * x.w;
+            }
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int64_t at = (int64_t)(r.row0 + t) * a.heads + r.h * a.group + i % a.group;
-    T *out = reinterpret_cast<T *>(a.out) + at * D + lane * V;
-    uint32_t w[V / 2];
-#pragma unroll
-    for (int v = 0; v < V; v += 2) w[v / 2] = pack2<T>(acc[v] * inv, acc[v + 1] * inv);
-    if constexpr (V == 4)
-        *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-    else
-        *reinterpret_cast<uint32_t *>(out) = w[0];
-    if (a.lse && lane == 0)
-        a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     float zero = 0.0f;      // not-a-number once a value is not finite
 #pragma unroll
-    for (int v = 0; v < V; v++) zero = fmaf(acc[v] * inv, 0.0f, zero);
-    if (__any_sync(0xffffffffu, zero != 0.0f) && a.s.causal) {
-        const int b = a.recs[c].b, t0 = a.recs[c].rt * item_tok;
-        int first, q_len, kv_len;
-        quiet_seq(a.s, b, first, q_len, kv_len);
-        mend_row<T, D>(a, b, at, r.h * a.group + i % a.group, seen_by(a.s, kv_len, q_len, t0 + t),
+    for (int g = 0; g < G; g++) {
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            acc[g][v] *= inv;
+            zero = fmaf(acc[g][v], 0.0f, zero);
+        }
+        if (live)
+            *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + at * D + (l16 + 16 * g) * 4) =
+                make_uint2(pack2<T>(acc[g][0], acc[g][1]), pack2<T>(acc[g][2], acc[g][3]));
+    }
+    if (a.lse && l16 == 0 && live)
+        a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    const uint32_t odd = __ballot_sync(0xffffffffu, zero != 0.0f && live);
+    if (odd == 0 || !a.s.causal) return;
+    const int b = a.recs[c].b, t0 = a.recs[c].rt * item_tok;
+    int first, q_len, kv_len;
+    quiet_seq(a.s, b, first, q_len, kv_len);
+    for (int x = 0; x < 2; x++) {
+        if ((odd >> (16 * x) & 0xffffu) == 0) continue;
+        const int ix = i0 + x, tx = ix / a.group, head = r.h * a.group + ix % a.group;
+        mend_row<T, D>(a, b, (int64_t)(r.row0 + tx) * a.heads + head, head,
+                       seen_by(a.s, kv_len, q_len, t0 + tx),
                        min(kv_len, tiles_to(a.s, kv_len, q_len, t0 + item_tok) * kKeys));
     }
 }
@@ -205,7 +216,7 @@ int launch_join(Dev *d, const PagedTc &a, int rows, int item_tok) {
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)d->sms, (unsigned)((rows + 7) / 8));
+    cfg.gridDim = dim3((unsigned)d->sms, (unsigned)((rows + 15) / 16));
     cfg.blockDim = dim3(256);
     cfg.stream = d->stream;
     cfg.attrs = &attr;
