@@ -10,7 +10,7 @@
 //
 // Everything between the load and the one rounding at the store is fp32.
 // HBM-bound: each row is read once and written once, 4 bytes a value.  Measured
-// with 32 + 2 x 8 heads of 128: 16384 tokens 82 us for 411 MB, 5.0 TB/s (a copy 6.5);
+// with 32 + 2 x 8 heads of 128: 16384 tokens 80 us for 411 MB, 5.2 TB/s (a copy 6.5);
 // one token 4.5 us on the device.
 #include "ew_launch.cuh"
 #include "paged.cuh"

@@ -20,7 +20,7 @@
 // tiles in tensor memory.  256 keys to a query tile, because the query tiles
 // come from L2 again and again: with 128 keys they asked for more than L2
 // gives.  With few rows the kernel is bound by HBM (each key once): 64 sequences of
-// 8192, one new token, 32 heads of 128 over 8 key heads: 107 us for 563 MB, 5.2
+// 8192, one new token, 32 heads of 128 over 8 key heads: 101 us for 563 MB, 5.6
 // TB/s.  With many it is bound by the exponentials, one per score: 3 x 1000 new tokens
 // of 6000: 129 us, a unit of 256 keys x 128 rows taking 3000 cycles, 2048 of them
 // the MUFU's.  Items are not cut (a key's sum would need a second pass or lose its
