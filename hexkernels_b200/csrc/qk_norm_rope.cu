@@ -156,13 +156,9 @@ __global__ void __launch_bounds__(kWideThreads, 8) norm_rope_kernel(const NormRo
     int64_t page;
     int off;
     if (!token_place(a, pos, slot, page, off)) return;
-    // (columns that do not turn have a cosine of 1 and a sine of 0)
-    uint64_t cs[4], sn[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        cs[i] = pair(1.0f, 1.0f);
-        sn[i] = pair(0.0f, 0.0f);
-    }
+    // (read where the lane's columns turn: a sine of 0 would not leave the others
+    // alone, since 0 times an infinity is not 0)
+    uint64_t cs[4] = {0, 0, 0, 0}, sn[4] = {0, 0, 0, 0};
     if (turns) {
         const int64_t o = (int64_t)pos * (a.rot / 2) + 8 * c;
 #pragma unroll
@@ -224,7 +220,9 @@ __global__ void __launch_bounds__(kWideThreads, 8) norm_rope_kernel(const NormRo
                     y[i] = mul2(y[i], iv);
                 }
             }
-            if (HALVES) {
+            if (!turns) {
+                // (y as it is)
+            } else if (HALVES) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint64_t f = x[i];

@@ -1,0 +1,55 @@
+"""The paged-cache operators on inputs at the edge of what they take: values
+that are not finite, rows and pages that do not count, calls without a cache.
+Expected values are 64-bit, as in test_gpu_paged."""
+import numpy as np
+import pytest
+
+import paged_ref as ref
+from test_gpu_paged import CODE, OnDevice, dev, down, near, norm_rope, up  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+F32 = np.zeros(0, np.float32)
+
+
+# ------------------------------------------------------------ qk_norm_rope
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("halves", [True, False])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dim, rot, shift", [(128, 64, 0), (128, 0, 0), (64, 16, 0), (80, 32, 0), (256, 128, 0), (128, 64, 1), (72, 32, 0)])
+def test_columns_that_do_not_turn_keep_to_themselves(dev, dim, rot, shift, norm, halves, kind):
+    """An infinity, a not-a-number or a zero of either sign behind the columns
+    that turn is nobody else's."""
+    import torch
+    rng = np.random.default_rng(500 + dim + rot)
+    T, H, KV, page, pages = 24, 3, 2, 16, 2
+    x = rng.standard_normal((T, H + 2 * KV, dim))
+    odd = rng.random(x.shape) < 0.05
+    odd[..., :rot] = False
+    odd[:4] = False
+    x = np.where(odd, rng.choice([np.nan, np.inf, -np.inf], x.shape), x)
+    x = np.where(rng.random(x.shape) < 0.2, rng.choice([0.0, -0.0], x.shape), x)
+    x = ref.to16(x, kind)
+    gain = ref.to16(1 + 0.2 * rng.standard_normal(dim), kind)
+    cos, sin = ref.turns(40, rot)
+    pos, slots = rng.integers(0, 40, T).astype(np.int32), np.arange(T, dtype=np.int32)
+    packed = torch.empty(x.size + shift, dtype=torch.int16, device="cuda")[shift:]
+    packed.copy_(up(x).view(-1))
+    wide = (H + 2 * KV) * dim
+    out = torch.empty(T * H * dim, dtype=torch.int16, device="cuda")
+    k, v = (up(np.zeros((pages, KV, page, dim), x.dtype)) for _ in range(2))
+    dev.launch("qk_norm_rope", 0, CODE[kind], packed, wide, packed[H * dim:], wide, packed[(H + KV) * dim:], wide, up(gain), up(gain),
+               up(cos) if rot else None, up(sin) if rot else None, up(pos), up(slots), out, k, v, None, T, H, KV, dim, rot,
+               int(halves), int(norm), 40, pages, page, 1e-6)
+    dev.sync(0)
+    got_q = out.cpu().numpy().view(x.dtype).reshape(T, H, dim)
+    got_k = down(k, x)[slots // page, :, slots % page]
+    for got, src in ((got_q, x[:, :H]), (got_k, x[:, H:H + KV])):
+        with np.errstate(all="ignore"):
+            want, bound = ref.qk_norm_rope(src, gain, cos, sin, pos, halves, norm, 1e-6)
+        near(got, want, bound)
+        if not norm:    # what does not turn is copied, to the sign of a zero
+            kept = ~np.isnan(ref.to64(src))
+            kept[..., :rot] = False
+            np.testing.assert_array_equal(got.view(np.uint16)[kept], src.view(np.uint16)[kept])
+    np.testing.assert_array_equal(down(v, x)[slots // page, :, slots % page].view(np.uint16), x[:, H + KV:].view(np.uint16))
