@@ -40,8 +40,8 @@ __device__ __forceinline__ bool token_place(const NormRope &a, int pos, int slot
                                             int &off) {
     page = 0;
     off = 0;
-    if (a.slots) {
-        if (slot < 0) return false;
+    if (a.slots && slot < 0) return false;
+    if (a.kv_heads > 0) {       // (without a cache any other slot marks a token that counts)
         page = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page_size;
         off = slot - (int)page * a.page_size;
         if (page >= a.num_pages) {

@@ -532,8 +532,9 @@ int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, con
  * page_size + offset, and scores [num_pages][kv_heads][page_size] (may be
  * null) is set to 0 there.  A negative slot marks padding: nothing of that
  * token is read or written.  Slots of one call are distinct.  kv_heads 0: only
- * queries, slots may be null (every token is taken); v and v_pages may both be
- * null.  head_dim 1 to 256. */
+ * queries, slots may be null (every token is taken) and otherwise name nothing
+ * (negative for padding, else any number); v and v_pages may both be null.
+ * head_dim 1 to 256. */
 int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_stride, const void *k,
                          int64_t k_stride, const void *v, int64_t v_stride, const void *q_gain,
                          const void *k_gain, const float *cos_t, const float *sin_t,

@@ -53,3 +53,27 @@ def test_columns_that_do_not_turn_keep_to_themselves(dev, dim, rot, shift, norm,
             kept[..., :rot] = False
             np.testing.assert_array_equal(got.view(np.uint16)[kept], src.view(np.uint16)[kept])
     np.testing.assert_array_equal(down(v, x)[slots // page, :, slots % page].view(np.uint16), x[:, H + KV:].view(np.uint16))
+
+
+@pytest.mark.parametrize("dim", [128, 72])
+@pytest.mark.parametrize("pages, page", [(0, 16), (1, 1), (0, 1)])
+def test_queries_alone_take_any_slot(dev, pages, page, dim):
+    """Without key heads there is no cache: a slot says only whether the token
+    counts, and the cache's sizes say nothing."""
+    rng = np.random.default_rng(521)
+    T, H = 40, 3
+    x = ref.to16(rng.standard_normal((T, H, dim)), "bf16")
+    cos, sin = ref.turns(64, dim)
+    pos = rng.integers(0, 64, T).astype(np.int32)
+    slots = rng.integers(0, 2 ** 31 - 1, T).astype(np.int32)
+    slots[:2] = 0, 2 ** 31 - 1
+    skip = np.arange(T) % 5 == 2
+    slots[skip], pos[skip] = -1, -7
+    out = up(np.full(x.shape, 0x1234, np.uint16))
+    dev.launch("qk_norm_rope", 0, 1, up(x), H * dim, None, 0, None, 0, None, None, up(cos), up(sin), up(pos), up(slots), out, None,
+               None, None, T, H, 0, dim, dim, 1, 1, 64, pages, page, 1e-6)
+    dev.sync(0)
+    got = down(out, x)
+    want, bound = ref.qk_norm_rope(x[~skip], None, cos, sin, pos[~skip], True, True, 1e-6)
+    near(got[~skip], want, bound)
+    assert (got[skip] == 0x1234).all()
