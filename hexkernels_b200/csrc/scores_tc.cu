@@ -15,8 +15,8 @@
 // Per CTA (one per SM), 384 threads: warps 0 and 3 TMA of the halves of the keys
 // (page fragments, one lane each; 16-token pages make more loads than one warp
 // can start in time), warp 1 tensor memory and MMA issue, warp 2 TMA of query
-// tiles and the rows' lse * log2e (plus infinity where a row counts for
-// nothing), then a warpgroup for each half of the keys, each with two score
+// tiles and the rows' lse * log2e (minus infinity where a row counts for
+// nothing, and a flag for the tile), then a warpgroup for each half of the keys, each with two score
 // tiles in tensor memory.  256 keys to a query tile, because the query tiles
 // come from L2 again and again: with 128 keys they asked for more than L2
 // gives.  With few rows the kernel is bound by HBM (each key once): 64 sequences of
@@ -54,7 +54,8 @@ struct ScSmem {
     static constexpr int kK = 0;
     static constexpr int kQ = kK + kKStages * 2 * kTile;
     static constexpr int kLse = kQ + kQStages * kQTile;      // [4][R]
-    static constexpr int kPlan = kLse + 4 * R * 4;
+    static constexpr int kNone = kLse + 4 * R * 4;           // [4]: a row of the tile has no weight
+    static constexpr int kPlan = kNone + 16;
     static constexpr int kBar = kPlan + 512;
     // l_full, l_empty [4], s_full, s_empty [half][2], drain, q_full, q_empty,
     // k_full, k_empty [stages]
@@ -226,6 +227,28 @@ __device__ __forceinline__ float add_weights(uint32_t s_addr, const float *z, fl
         }
     }
     return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+
+// The same where some row has no weight (z of minus infinity), whatever its score: a
+// row that saw nothing, or that the caller masks.  A loop of its own, because the test
+// within add_weights cost every chunk (3 x 1000 new tokens of 6000 137 us for 129; so
+// 131).
+template <int R>
+__device__ __forceinline__ float add_weights_but(uint32_t s_addr, const float *z, float scale_log2, int lo,
+                                              int hi) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < R; c += 16) {
+        uint32_t r[16];
+        tc::tmem_ld_32x32b_x16(s_addr + c, r);
+        tc::tmem_ld_wait(r);
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float p = tc::ex2(fmaf(__uint_as_float(r[e]), scale_log2, -z[c + e]));
+            if (c + e >= lo && c + e < hi && z[c + e] != -INFINITY) sum += p;
+        }
+    }
+    return sum;
 }
 
 template <typename T, int D, int R>
@@ -401,6 +424,7 @@ __global__ void __launch_bounds__(384, 1)
         constexpr int kPer = (R + 31) / 32;
         KeyWalk w = plan.start;
         float *sl = reinterpret_cast<float *>(smem + L::kLse);
+        int *sn = reinterpret_cast<int *>(smem + L::kNone);
         uint32_t u = 0;
         // lane's rows of a tile: token and head
         int row_tok[kPer], row_at[kPer];
@@ -414,7 +438,7 @@ __global__ void __launch_bounds__(384, 1)
             const float *base = a.lse + ((int64_t)(w.first + t * a.tok) * a.heads + w.h * a.group);
 #pragma unroll
             for (int i = 0; i < kPer; i++)
-                z[i] = row_tok[i] < w.q_len - t * a.tok ? base[row_at[i]] : -INFINITY;
+                z[i] = row_tok[i] < w.q_len - t * a.tok ? base[row_at[i]] : INFINITY;
         };
         float z[kPer], zn[kPer];
         int t = w.first_tile(a, 0);
@@ -440,11 +464,15 @@ __global__ void __launch_bounds__(384, 1)
             ok = tc::mbar_wait(&l_empty[(u - 1) & 3], (((u - 1) >> 2) & 1) ^ 1, abort_flag, err_word,
                                kErrWaitEmpty);
             if (!__all_sync(0xffffffffu, ok)) break;
+            bool none = false;
 #pragma unroll
             for (int i = 0; i < kPer; i++)
-                if (lane + 32 * i < R)
-                    sl[((u - 1) & 3) * R + lane + 32 * i] =
-                        z[i] == -INFINITY ? INFINITY : z[i] * 1.4426950408889634f;
+                if (lane + 32 * i < R) {
+                    none |= z[i] == -INFINITY;
+                    sl[((u - 1) & 3) * R + lane + 32 * i] = z[i] * 1.4426950408889634f;
+                }
+            none = __any_sync(0xffffffffu, none);
+            if (lane == 0) sn[(u - 1) & 3] = none;
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&l_full[(u - 1) & 3]);
 #pragma unroll
@@ -463,6 +491,7 @@ __global__ void __launch_bounds__(384, 1)
         const int x = (warp - 4) >> 2, key = (warp & 3) * 32 + lane;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const float *sl = reinterpret_cast<const float *>(smem + L::kLse);
+        const int *sn = reinterpret_cast<const int *>(smem + L::kNone);
         KeyWalk w = plan.start;
         uint32_t u = 0, n = 0;
         bool ok = true;
@@ -480,7 +509,7 @@ __global__ void __launch_bounds__(384, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (t >= t_mine) {
-                    const int buf = x * 2 + (n & 1);
+                    const int buf = x * 2 + (n & 1), none = sn[lb];
                     ok = tc::mbar_wait(&s_full[buf], (n >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
@@ -491,7 +520,9 @@ __global__ void __launch_bounds__(384, 1)
                     const uint32_t s_addr = tmem_base + lane_base + buf * R;
                     const float *zl = sl + lb * R;
                     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (__any_sync(0xffffffffu, lo > 0 || hi < R))
+                    if (none != 0)
+                        sum += add_weights_but<R>(s_addr, zl, a.scale_log2, lo, hi);
+                    else if (__any_sync(0xffffffffu, lo > 0 || hi < R))
                         sum += add_weights<R, true>(s_addr, zl, a.scale_log2, lo, hi, acc);
                     else
                         sum += add_weights<R, false>(s_addr, zl, a.scale_log2, 0, R, acc);

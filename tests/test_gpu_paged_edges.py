@@ -77,3 +77,41 @@ def test_queries_alone_take_any_slot(dev, pages, page, dim):
     want, bound = ref.qk_norm_rope(x[~skip], None, cos, sin, pos[~skip], True, True, 1e-6)
     near(got[~skip], want, bound)
     assert (got[skip] == 0x1234).all()
+
+
+# ------------------------------------------------------------ cache_scores
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("heads, kv_heads, dim, page, causal", [(8, 2, 128, 16, True), (4, 4, 64, 32, True), (6, 1, 64, 8, False),
+                                                                 (8, 2, 80, 16, True), (40, 1, 128, 16, False)])
+@pytest.mark.parametrize("q", [[1, 1, 1], [9, 1, 3], [60, 33, 128], [300, 1, 40]])
+def test_rows_of_no_weight_add_nothing(dev, q, heads, kv_heads, dim, page, causal, kind):
+    """Rows whose lse is minus infinity count for nothing, whatever their query
+    holds; the rows beside them count as before, one of plus infinity as zero."""
+    rng = np.random.default_rng(531 + sum(q))
+    c = ref.Cache(rng, [700, 90, 257], q, heads, kv_heads, dim, page, kind, fill=np.nan)
+    o = OnDevice(dev, c, causal)
+    o.attn()
+    dev.sync(0)
+    lse = o.results()[1].copy()
+    none = rng.random(lse.shape) < 0.3
+    none[0], none[-1] = True, False
+    odd = np.where(rng.random(c.q.shape) < 0.5, rng.choice([np.nan, np.inf, -np.inf], c.q.shape), 0.0)
+    x = np.where(none[..., None], np.where(odd == 0, ref.to64(c.q), odd), ref.to64(c.q))
+    lse[none] = -np.inf
+    full = ~none & (rng.random(lse.shape) < 0.05)
+    lse[full] = np.inf
+    o.q, o.lse = up(ref.to16(x, kind)), up(lse)
+    base = rng.random((c.pages, kv_heads, page)).astype(np.float32)
+    s = up(base)
+    o.scores(s)
+    dev.sync(0)
+    # (exp(x - inf) is 0 without any rounding, so such a row adds nothing to the bound either)
+    near(down(s, base), *ref.cache_scores(c, np.where(full, -np.inf, lse).astype(np.float32), base, causal))
+    # all rows without weight, beside keys that are not finite: not a bit changes
+    o.k = up(ref.to16(np.where(rng.random(c.k.shape) < 0.1, np.inf, ref.to64(c.k)), kind))
+    o.lse.fill_(-np.inf)
+    s = up(base)
+    o.scores(s)
+    dev.sync(0)
+    np.testing.assert_array_equal(down(s, base), base)
