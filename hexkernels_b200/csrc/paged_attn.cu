@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int it
     }
 }
 
-// The join starts while the kernel before it on the stream still runs, and
+// The join (not launched when the kernel before it was refused: its records would be
+// what the workspace held) starts while that kernel still runs on the stream, and
 // waits for it on the device (a programmatic dependent launch).
 template <typename T, int D>
 int launch_join(Dev *d, const PagedTc &a, int rows, int item_tok) {

@@ -547,8 +547,12 @@ int launch_dec(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUten
             return rc;
         attr_done[d->ordinal & 63] = true;
     }
-    paged_dec_kernel<T, D, N><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, mv, a);
-    return HEXCUDA_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)d->sms);
+    cfg.blockDim = dim3(384);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = d->stream;
+    return check(cudaLaunchKernelEx(&cfg, paged_dec_kernel<T, D, N>, mq, mk, mv, a), "launch paged_dec");
 }
 
 }  // namespace

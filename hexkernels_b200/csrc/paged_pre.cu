@@ -683,8 +683,12 @@ int launch_pre(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const CUten
                         fa.numRegs, (kRegsPool + 383) / 384);
         attr_done[d->ordinal & 63] = true;
     }
-    paged_pre_kernel<T, D><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, mv, a);
-    return HEXCUDA_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)d->sms);
+    cfg.blockDim = dim3(384);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = d->stream;
+    return check(cudaLaunchKernelEx(&cfg, paged_pre_kernel<T, D>, mq, mk, mv, a), "launch paged_pre");
 }
 
 }  // namespace

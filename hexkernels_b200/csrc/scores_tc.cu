@@ -567,8 +567,12 @@ int launch_scores(Dev *d, const CUtensorMap &mq, const CUtensorMap &mk, const Sc
             return rc;
         attr_done[d->ordinal & 63] = true;
     }
-    scores_tc_kernel<T, D, R><<<d->sms, 384, L::kTotal, d->stream>>>(mq, mk, a);
-    return HEXCUDA_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)d->sms);
+    cfg.blockDim = dim3(384);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = d->stream;
+    return check(cudaLaunchKernelEx(&cfg, scores_tc_kernel<T, D, R>, mq, mk, a), "launch scores_tc");
 }
 
 template <typename T, int D>
