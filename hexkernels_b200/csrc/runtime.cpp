@@ -34,6 +34,7 @@ int fail(int code, const char *fmt, ...) {
 
 int check(cudaError_t e, const char *what) {
     if (e == cudaSuccess) return HEXCUDA_OK;
+    cudaGetLastError();         // reported here, not again by the next launch
     return fail(e == cudaErrorMemoryAllocation ? HEXCUDA_ERR_OOM : HEXCUDA_ERR_CUDA,
                 "%s: %s (%d)", what, cudaGetErrorString(e), (int)e);
 }

@@ -115,3 +115,17 @@ def test_rows_of_no_weight_add_nothing(dev, q, heads, kv_heads, dim, page, causa
     o.scores(s)
     dev.sync(0)
     np.testing.assert_array_equal(down(s, base), base)
+
+
+# ----------------------------------------------------------------- errors
+
+def test_a_call_after_one_that_ran_out_of_memory(hx):
+    """A refused allocation is that call's error and not the next one's."""
+    from hexkernels_b200 import _lib
+    lib = _lib.load()
+    assert not lib.hexcuda_alloc(0, 1 << 50)
+    c = ref.Cache(np.random.default_rng(581), [100, 40], [4, 3], 4, 2, 64, 16)
+    out, lse = hx.paged_attn(c.q, c.k, c.v, c.table, c.kv_lens, c.q_offs)
+    want, z, b_out, b_lse = ref.paged_attn(c)
+    near(out, want, b_out)
+    near(lse, z, b_lse)
