@@ -8,8 +8,8 @@
 // of q and the last ones of the sequence's kv_lens[b] cached tokens.
 //
 // The host cannot see those indices, so every kernel checks them before it
-// uses them: what is out of range is skipped (or clamped, for a length) and
-// raises kErrIndex in the device's error word, which hexcuda_sync reports.
+// uses them: what is out of range is skipped (clamped, for a length; taken for a
+// page of zeros by the attention) and raises kErrIndex in the device's error word, which hexcuda_sync reports.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -75,12 +75,13 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
             float x = -INFINITY;
             if (j < seen) {
                 const int page = seq_page(s, b, j / s.page_size);
-                if (page >= 0) {
+                if (page >= 0)
                     row = ((int64_t)page * kv_heads + kvh) * s.page_size + j % s.page_size;
-                    float a = 0.0f;
-                    for (int d = 0; d < dim; d++) a += sq[warp][d] * to_f32(kp[row * dim + d]);
-                    x = a * scale;
-                }
+                // (a page that is not there: keys and values of zeros, as TMA gives them)
+                float a = 0.0f;
+                for (int d = 0; d < dim; d++)
+                    a += sq[warp][d] * (row >= 0 ? to_f32(kp[row * dim + d]) : 0.0f);
+                x = a * scale;
             }
             float top = x;
             for (int o = 16; o > 0; o >>= 1)
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
             const float m_new = fmaxf(m, top);
             const float ref = m_new == -INFINITY ? 0.0f : m_new;
             const float corr = expf(m - ref);
-            const float p = row >= 0 ? expf(x - ref) : 0.0f;
+            const float p = j < seen ? expf(x - ref) : 0.0f;
             float sum = p;
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l = l * corr + sum;

@@ -292,7 +292,7 @@ static int sync_one(Dev *d) {
         if (word == kErrIndex)
             return fail(HEXCUDA_ERR_ARG,
                         "device %d: a page, slot, position, length or row offset in device memory "
-                        "was out of range; what it named was skipped",
+                        "was out of range; it was not followed, and its sequence's outputs are of no use",
                         d->ordinal);
         return fail(HEXCUDA_ERR_TIMEOUT,
                     "device %d: a bounded device-side wait expired (flags 0x%x); outputs of "

@@ -515,7 +515,8 @@ int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, con
  * (not-a-number included), and a row is not touched by what it does not see.
  * Tables, lengths, offsets, slots and positions are device data: an entry out
  * of range is skipped, never followed, and the next hexcuda_sync returns
- * HEXCUDA_ERR_ARG.  Page, token and row counts are below 2^31; element offsets
+ * HEXCUDA_ERR_ARG.  (paged_attn takes keys and values of zeros for a page that
+ * is not there: the rows of that sequence are of no use, the others are right.)  Page, token and row counts are below 2^31; element offsets
  * are 64-bit.  Nothing is allocated and nothing is read back, so calls can be
  * captured into CUDA graphs (with hexcuda_set_timing(0)). */
 #define HEXCUDA_F16 0

@@ -117,6 +117,48 @@ def test_rows_of_no_weight_add_nothing(dev, q, heads, kv_heads, dim, page, causa
     np.testing.assert_array_equal(down(s, base), base)
 
 
+# --------------------------------------------------------- pages that are not there
+
+PAGES = [
+    ([300, 200, 250], [1, 1, 1], 8, 2, 128, 16), ([300, 200, 250], [5, 1, 3], 8, 2, 64, 8), ([300, 200, 250], [60, 35, 50], 8, 2, 128, 16),
+    ([900, 200, 250], [60, 35, 250], 4, 1, 64, 24), ([300, 200, 250], [1, 1, 1], 4, 2, 64, 256), ([300, 200, 250], [7, 60, 9], 4, 4, 128, 128),
+    ([5000, 16, 33], [1, 1, 1], 16, 2, 64, 16), ([3000, 16, 40], [200, 16, 40], 8, 2, 128, 16), ([300, 200, 250], [5, 40, 3], 8, 2, 80, 16),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", range(len(PAGES)), ids=lambda n: "-".join(map(str, PAGES[n][1:])).replace(" ", ""))
+def test_a_page_out_of_range_counts_as_zeros(dev, n, causal):
+    """Its keys and values are zeros in every kernel, and its tokens collect nothing."""
+    from hexkernels_b200 import HexcudaError
+    rng = np.random.default_rng(541 + n)
+    c = ref.Cache(rng, *PAGES[n], "f16" if n % 2 else "bf16", fill=np.nan, q_by=0.5)
+    page = PAGES[n][-1]
+    bad = [(b, i) for b, m in enumerate(c.kv_lens) for i in range(-(-int(m) // page)) if b == 1 or rng.random() < 0.3]
+    o = OnDevice(dev, c, causal)
+    for b, i in bad:
+        o.table[b, i] = int(rng.choice([-1, c.pages, 2 ** 31 - 1, -2 ** 31]))
+    o.attn()
+    with pytest.raises(HexcudaError, match="out of range"):
+        dev.sync(0)
+    out, lse = o.results()
+    gone = [c.table[b, i] for b, i in bad]
+    c.k[gone] = c.v[gone] = 0
+    want, z, b_out, b_lse = ref.paged_attn(c, causal)
+    near(out, want, b_out, "out")
+    near(lse, z, b_lse, "lse")
+    base = rng.random(c.k.shape[:3]).astype(np.float32)
+    s = up(base)
+    o.scores(s)
+    with pytest.raises(HexcudaError, match="out of range"):
+        dev.sync(0)
+    want, bound = ref.cache_scores(c, lse, base, causal)
+    got = down(s, base)
+    np.testing.assert_array_equal(got[gone], base[gone])
+    want[gone] = base[gone]
+    near(got, want, bound, "scores")
+
+
 # ----------------------------------------------------------------- errors
 
 def test_a_call_after_one_that_ran_out_of_memory(hx):
