@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(
 // that two rows' groups of four columns, neighbours in a chunk's parts, make whole
 // sectors.  The parts are taken in CTA order:
 //   M = max m_k,  out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
-// Rows that are not finite are looked at again (mend_row).  Bound by latency: 10.8 us
+// Where a part's CTA took values that are not finite out of a tile, the rows that see
+// them get them here (paged_tc.cuh).  Bound by latency: 10.8 us
 // for 11 chunks of 301 tokens of 64 (a warp a row: 15.6), 19 us for 148 items of 256
 // rows of 128, 5.3 us for one token.
 template <typename T, int D>
@@ -140,8 +141,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int it
     auto slot = [&](int k) { return ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * kPartRows; };
     const float2 *mls = reinterpret_cast<const float2 *>(a.part_ml);
     float top = -INFINITY;
+    int odd = 0;
     for (int k = l16; k < r.nparts; k += 16) {
         const float2 ml = mls[slot(k) + row];
+        odd |= a.recs[c + k].odd;
         if (ml.y != 0.0f) top = fmaxf(top, ml.x);
     }
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -181,32 +184,31 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTc a, int it
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int64_t at = (int64_t)(r.row0 + t) * a.heads + r.h * a.group + i % a.group;
-    float zero = 0.0f;      // not-a-number once a value is not finite
 #pragma unroll
-    for (int g = 0; g < G; g++) {
+    for (int g = 0; g < G; g++)
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-            acc[g][v] *= inv;
-            zero = fmaf(acc[g][v], 0.0f, zero);
-        }
-        if (live)
-            *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + at * D + (l16 + 16 * g) * 4) =
-                make_uint2(pack2<T>(acc[g][0], acc[g][1]), pack2<T>(acc[g][2], acc[g][3]));
+        for (int v = 0; v < 4; v++) acc[g][v] *= inv;
+    if (__any_sync(0xffffffffu, odd != 0)) {
+        int first, q_len, kv_len;
+        quiet_seq(a.s, r.b, first, q_len, kv_len);
+        const int t0 = r.rt * item_tok, seen = min(kv_len, seen_by(a.s, kv_len, q_len, t0 + t));
+#pragma unroll 4
+        for (int j = seen_by(a.s, kv_len, q_len, t0); j < seen; j++)
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                float x[4];
+                odd_values<T, D, 4>(a, r.b, r.h, j, (l16 + 16 * g) * 4, x);
+#pragma unroll
+                for (int v = 0; v < 4; v++) acc[g][v] += x[v];
+            }
     }
-    if (a.lse && l16 == 0 && live)
+    if (!live) return;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + at * D + (l16 + 16 * g) * 4) =
+            make_uint2(pack2<T>(acc[g][0], acc[g][1]), pack2<T>(acc[g][2], acc[g][3]));
+    if (a.lse && l16 == 0)
         a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    const uint32_t odd = __ballot_sync(0xffffffffu, zero != 0.0f && live);
-    if (odd == 0 || !a.s.causal) return;
-    const int b = a.recs[c].b, t0 = a.recs[c].rt * item_tok;
-    int first, q_len, kv_len;
-    quiet_seq(a.s, b, first, q_len, kv_len);
-    for (int x = 0; x < 2; x++) {
-        if ((odd >> (16 * x) & 0xffffu) == 0) continue;
-        const int ix = i0 + x, tx = ix / a.group, head = r.h * a.group + ix % a.group;
-        mend_row<T, D>(a, b, (int64_t)(r.row0 + tx) * a.heads + head, head,
-                       seen_by(a.s, kv_len, q_len, t0 + tx),
-                       min(kv_len, tiles_to(a.s, kv_len, q_len, t0 + item_tok) * kKeys));
-    }
 }
 
 // The join (not launched when the kernel before it was refused: its records would be

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t *k_full = bars + 15, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile int *odd_flag = abort_flag + 1;     // an output that is not finite
+    volatile int *odd_flag = abort_flag + 1;     // some value was not finite (settle_row)
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err_word = a.s.err_word;
@@ -351,7 +351,15 @@ __global__ void __launch_bounds__(384, 1)
             }
             for (int j = w.j0; j < w.j1; j++, g++) {
                 const int buf = g & 1;
-                bool ok = tc::mbar_wait(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
+                bool ok = true;
+                if (x == 0 && j * kKeys + kKeys > seen0) {
+                    // (while the scores are made; P is handed over behind it)
+                    ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
+                    if (ok)
+                        settle_row<T, kSubs>(smem + L::kV + st * L::kTile, key, seen0 - j * kKeys,
+                                             w.kv_len - j * kKeys, odd_flag);
+                }
+                ok = ok && tc::mbar_wait(&s_full[buf], (g >> 1) & 1, abort_flag, err_word, kErrWaitAccum);
                 tc::tc_fence_after();
                 float v[C];
                 if (ok) {
@@ -431,11 +439,6 @@ __global__ void __launch_bounds__(384, 1)
                 if (ok && g >= 2)
                     ok = tc::mbar_wait(&pv_done[buf], ((g - 2) >> 1) & 1, abort_flag, err_word,
                                        kErrWaitAccum);
-                const int valid = w.kv_len - j * kKeys;
-                if (x == 0 && valid < kKeys) {
-                    if (ok) ok = tc::mbar_wait(&v_full[st], ph, abort_flag, err_word, kErrWaitFull);
-                    if (ok) clear_rows<kSubs>(smem + L::kV + st * L::kTile, key, valid);
-                }
                 if (ok) {
                     uint4 *prow = reinterpret_cast<uint4 *>(smem + L::kP + buf * (kKeys * N * 2) +
                                                             key * N * 2);
@@ -492,21 +495,16 @@ __global__ void __launch_bounds__(384, 1)
             if (key < D) {
                 if (whole) {
                     int t = n0 / a.group, i = n0 % a.group;
-                    float zero = 0.0f;          // not-a-number once a value is not finite
 #pragma unroll
                     for (int n = 0; n < C; n++) {
-                        if (n0 + n < nrows) {
-                            const float y = __uint_as_float(o[n]) * res[n0 + n];
-                            zero = fmaf(y, 0.0f, zero);
+                        if (n0 + n < nrows)
                             out[((int64_t)(w.first + t0 + t) * a.heads + w.h * a.group + i) * D + key] =
-                                from_f32<T>(y);
-                        }
+                                from_f32<T>(__uint_as_float(o[n]) * res[n0 + n]);
                         if (++i == a.group) {
                             i = 0;
                             t++;
                         }
                     }
-                    if (zero != 0.0f) *odd_flag = 1;
                 } else {
                     float *po = a.part_o + ((size_t)slot * kPartRows + n0) * D + key;
 #pragma unroll
@@ -529,7 +527,8 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         tc::tmem_dealloc(tmem_base, kCols);
     }
-    if (warp >= 4 && a.s.causal && *odd_flag && !*abort_flag)
+    if (threadIdx.x == 0) a.recs[blockIdx.x].odd = *odd_flag;
+    if (warp >= 4 && *odd_flag && !*abort_flag)
         mend_items<T, D>(a, plan.start, a.tok, warp - 4);
 }
 

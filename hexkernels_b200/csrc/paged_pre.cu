@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t *k_full = bars + 14, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile int *odd_flag = abort_flag + 1;     // an output that is not finite
+    volatile int *odd_flag = abort_flag + 1;     // some value was not finite (settle_row)
     PlanShared &plan = *reinterpret_cast<PlanShared *>(smem + L::kPlan);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err_word = a.s.err_word;
@@ -417,6 +417,24 @@ __global__ void __launch_bounds__(384, 1)
             float m_ref = -INFINITY, l = 0.0f;
             bool ok = true;
             for (; left > 0; left--, n++, rest -= step_keys, rest0 -= step_keys, first = false) {
+                if (rest0 < kKeys) {
+                    // values that no weight of zero may meet, by each side before it
+                    // hands its P over (all four warps have then).  The rows that b
+                    // would settle a has settled, if it takes the tile, before its own
+                    // P V and then b's read it: b writes the same zeros once more, or
+                    // nothing.
+                    const Span s = span_of(a, *wp, x);
+                    const int j = s.start + (s.count() - left) * s.step, gk = g0 + (j - wp->j0);
+                    const int valid = wp->kv_len - j * kKeys;
+                    if (valid < kKeys || rest0 < valid) {
+                        ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word,
+                                           kErrWaitFull);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        settle_row<T, kSubs>(smem + L::kV + gk % S * L::kTile, row, rest0, valid,
+                                             odd_flag);
+                        tc::fence_proxy_async_smem();
+                    }
+                }
                 ok = tc::mbar_wait(&s_full[x], n & 1, abort_flag, err_word, kErrWaitAccum);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
@@ -476,20 +494,6 @@ __global__ void __launch_bounds__(384, 1)
                             l *= corr;
                             m_ref = m_new;
                         }
-                    }
-                }
-                if (left == 1 && wp->kv_len < wp->j1 * kKeys) {
-                    // zeros in the values behind the last cached token, by each
-                    // side before it hands its P over (all four warps have then;
-                    // that the other side writes the same zeros does not matter)
-                    const Span s = span_of(a, *wp, x);
-                    const int j = s.start + (s.count() - 1) * s.step, gk = g0 + (j - wp->j0);
-                    if (j * kKeys + kKeys > wp->kv_len) {
-                        ok = tc::mbar_wait(&v_full[gk % S], (gk / S) & 1, abort_flag, err_word,
-                                           kErrWaitFull);
-                        if (!__all_sync(0xffffffffu, ok)) break;
-                        clear_rows<kSubs>(smem + L::kV + gk % S * L::kTile, row, wp->kv_len - j * kKeys);
-                        tc::fence_proxy_async_smem();
                     }
                 }
                 // P = 2^(s*scale*log2e - m_ref) from the registers, as 16-bit
@@ -600,10 +604,6 @@ __global__ void __launch_bounds__(384, 1)
                     if (whole) {
                         uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + orow * D +
                                                                cc * 32);
-                        float zero = 0.0f;      // not-a-number once a value is not finite
-#pragma unroll
-                        for (int e = 0; e < 32; e++) zero = fmaf(__uint_as_float(o[e]), 0.0f, zero);
-                        if (zero != 0.0f) *odd_flag = 1;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             uint32_t v[4];
@@ -657,7 +657,8 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         tc::tmem_dealloc(tmem_base, 512);
     }
-    if (warp >= 4 && a.s.causal && *odd_flag && !*abort_flag)
+    if (threadIdx.x == 0) a.recs[blockIdx.x].odd = *odd_flag;
+    if (warp >= 4 && *odd_flag && !*abort_flag)
         mend_items<T, D>(a, plan.start, item_tok, warp - 4);
 }
 

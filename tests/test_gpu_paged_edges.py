@@ -159,6 +159,93 @@ def test_a_page_out_of_range_counts_as_zeros(dev, n, causal):
     near(got, want, bound, "scores")
 
 
+# ------------------------------------------------- values that are not finite
+
+def attn_odd(c, causal):
+    """ref.paged_attn where V is not finite: a column of a row that sees such
+    values is their sum (weights are positive), the others never meet them."""
+    v = ref.to64(c.v)
+    keep = c.v
+    c.v = ref.to16(np.where(np.isfinite(v), v, 0.0), c.kind)
+    want, z, b_out, b_lse = ref.paged_attn(c, causal)
+    c.v = keep
+    odd = np.where(np.isfinite(v), 0.0, v)
+    group = c.heads // c.kv_heads
+    for b in range(len(c.kv_lens)):
+        seen = ~c.hidden(b, causal)
+        j = np.arange(int(c.kv_lens[b]))
+        for h in range(c.kv_heads):
+            x = odd[c.table[b, j // c.page], h, j % c.page]
+            with np.errstate(all="ignore"):
+                for t in range(len(seen)):
+                    add = x[seen[t]].sum(0)
+                    if (add != 0).any():
+                        want[c.q_offs[b] + t, h * group:(h + 1) * group] += add
+    return want, z, b_out, b_lse
+
+
+ODD = [     # kv, q, heads, kv_heads, dim, page: whole items and cut ones, one query tile and two
+    ([300, 77], [4, 1], 8, 2, 128, 16), ([5000], [3], 10, 2, 128, 16), ([700, 640, 513], [7, 8, 2], 4, 1, 64, 16), ([900, 40], [60, 40], 4, 2, 64, 32),
+    ([2500], [300], 8, 2, 128, 16), ([1500, 128], [400, 128], 2, 2, 64, 64), ([600], [200], 16, 1, 128, 16), ([260, 20], [33, 50], 4, 1, 80, 16),
+    ([200] * 40, [90] * 40, 8, 2, 128, 32), ([1300], [1300], 4, 1, 64, 16), ([130], [3], 40, 1, 128, 16),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("where", ["channel", "scattered", "new tokens"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n", range(len(ODD)), ids=lambda n: "-".join(map(str, ODD[n][2:])) + f"x{len(ODD[n][0])}")
+def test_values_that_are_not_finite(dev, n, kind, where, causal):
+    rng = np.random.default_rng(551 + n)
+    c = ref.Cache(rng, *ODD[n], kind, fill=np.nan, q_by=0.7)
+    v = ref.to64(c.v)
+    if where == "channel":          # one that overflowed from the start
+        v[..., 5] = np.inf
+        v[..., c.dim - 1] = np.where(np.arange(v.shape[2]) % 2, np.inf, np.nan)
+    elif where == "scattered":
+        v = np.where(rng.random(v.shape) < 2e-4, rng.choice([np.nan, np.inf, -np.inf], v.shape), v)
+    else:
+        for b, (n_kv, n_q) in enumerate(zip(c.kv_lens, np.diff(c.q_offs))):
+            for j in range(max(0, n_kv - n_q), n_kv):
+                at = (c.table[b, j // c.page], slice(None), j % c.page)
+                v[at] = np.where(rng.random(v[at].shape) < 0.02, rng.choice([np.nan, np.inf, -np.inf], v[at].shape), v[at])
+    c.v = ref.to16(v, kind)
+    o = OnDevice(dev, c, causal)
+    o.attn()
+    dev.sync(0)
+    out, lse = o.results()
+    want, z, b_out, b_lse = attn_odd(c, causal)
+    near(out, want, b_out, "out")
+    near(lse, z, b_lse, "lse")
+
+
+@pytest.mark.parametrize("dim, kv, q", [(128, 6000, 600), (64, 6000, 600), (128, 12000, 7)])
+def test_a_channel_of_infinities_costs_little(dev, dim, kv, q):
+    """The time of a call is bounded by its sizes, not by what V holds."""
+    import torch
+    c = ref.Cache(np.random.default_rng(571), [kv], [q], 16, 4, dim, 16, "bf16")
+    o = OnDevice(dev, c)
+
+    def time():
+        ts = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            o.attn()
+            b.record()
+            torch.cuda.synchronize()
+            ts.append(a.elapsed_time(b))
+        return sorted(ts)[2]
+
+    plain = time()
+    o.v.view(torch.bfloat16)[..., 3] = float("inf")
+    odd = time()
+    dev.sync(0)
+    print(f"dim {dim} {q} of {kv}: {plain * 1e3:.0f} us, with an infinite channel {odd * 1e3:.0f} us")
+    assert odd < 4 * plain + 0.5
+
+
 # ----------------------------------------------------------------- errors
 
 def test_a_call_after_one_that_ran_out_of_memory(hx):
