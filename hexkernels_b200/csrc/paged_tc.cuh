@@ -26,11 +26,12 @@ constexpr int kKeys = 128;              // keys per tile
 constexpr int kSubTile = kKeys * 128;   // 64 columns of a key tile: 128 rows x 128 bytes
 constexpr int kPartRows = 256;          // rows of a partial result, at most
 
-struct alignas(32) PartRec {
+struct alignas(16) PartRec {            // (of the workspace's alignment, not more)
     int h, row0, ntok, nparts;          // nparts 0: the CTA's last item is not its to join
     int b, rt;                          // its sequence and place there
     int odd;                            // the CTA took values that are not finite out of a tile
 };
+static_assert(alignof(PartRec) <= 16, "the caller's workspace is 16-byte aligned");
 
 // What both attention kernels get.
 struct PagedTc {

@@ -246,6 +246,25 @@ def test_a_channel_of_infinities_costs_little(dev, dim, kv, q):
     assert odd < 4 * plain + 0.5
 
 
+def test_a_workspace_of_the_least_alignment(dev):
+    """16 bytes, as documented, and not a byte behind its end."""
+    import torch
+    need = dev.paged_attn_workspace(0)
+    for q in ([1, 1], [3, 2], [130, 70]):
+        c = ref.Cache(np.random.default_rng(577), [3000, 900], q, 8, 2, 128, 16, "bf16", fill=np.nan)
+        o = OnDevice(dev, c)
+        whole = torch.full((need + 48,), 0xA5, dtype=torch.uint8, device="cuda")
+        assert whole.data_ptr() % 32 == 0
+        o.space = whole[16:16 + need]
+        o.attn()
+        dev.sync(0)
+        out, lse = o.results()
+        want, z, b_out, b_lse = ref.paged_attn(c)
+        near(out, want, b_out)
+        near(lse, z, b_lse)
+        assert (whole[:16] == 0xA5).all() and (whole[16 + need:] == 0xA5).all()
+
+
 # ----------------------------------------------------------------- errors
 
 def test_a_call_after_one_that_ran_out_of_memory(hx):
