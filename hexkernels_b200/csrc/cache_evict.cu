@@ -480,13 +480,13 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
         return fail(HEXCUDA_ERR_ARG, "%s: batch %d kv_heads %d head_dim %d (1 to 256)", name, batch,
                     kv_heads, head_dim);
     if (num_pages < 1 || page_size < 1 || max_pages < 1 ||
-        (int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > 0x7fffffff)
+        (int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > kMaxTokens)
         return fail(HEXCUDA_ERR_ARG, "%s: num_pages %d page_size %d max_pages %d", name, num_pages,
                     page_size, max_pages);
-    if (budget < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > budget)
+    if (budget < 1 || budget > kMaxTokens || sink < 0 || recent < 0 || (int64_t)sink + recent > budget)
         return fail(HEXCUDA_ERR_ARG, "%s: budget %d sink %d recent %d", name, budget, sink, recent);
     const int width = dst_table ? dst_max_pages : max_pages;
-    if (width < 1 || (int64_t)width * page_size > 0x7fffffff ||
+    if (width < 1 || (int64_t)width * page_size > kMaxTokens ||
         (int64_t)width * page_size < (dst_table ? budget : 1))
         return fail(HEXCUDA_ERR_ARG, "%s: dst_max_pages %d of %d tokens hold no budget of %d", name,
                     width, page_size, budget);

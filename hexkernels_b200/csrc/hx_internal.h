@@ -77,6 +77,10 @@ int replicate_rows(const std::vector<void *> &douts, int64_t rows, size_t row_by
 void replica_clear();
 void collective_release();
 
+// Tokens of a sequence's table, of a budget and of a call at most: the kernels step
+// past them by tiles and blocks in 32 bits.
+constexpr int kMaxTokens = 0x7fff0000;
+
 // The argument checks that the entries over a paged cache share (paged_attn.cu).
 int check_paged(const char *name, int dtype, const void *table, const void *kv_lens,
                 const void *q_offs, int batch, int total_q, int max_q, int heads, int kv_heads,

@@ -19,7 +19,7 @@ int check_paged(const char *name, int dtype, const void *table, const void *kv_l
                 int head_dim, int num_pages, int page_size, int max_pages, float scale) {
     if (dtype != HEXCUDA_F16 && dtype != HEXCUDA_BF16)
         return fail(HEXCUDA_ERR_ARG, "%s: dtype %d", name, dtype);
-    if (batch < 0 || total_q < 0 || max_q < 0)
+    if (batch < 0 || total_q < 0 || total_q > kMaxTokens || max_q < 0)
         return fail(HEXCUDA_ERR_ARG, "%s: batch %d total_q %d max_q %d", name, batch, total_q,
                     max_q);
     if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 65535 || head_dim < 1 ||
@@ -28,7 +28,7 @@ int check_paged(const char *name, int dtype, const void *table, const void *kv_l
                     "%s: heads %d kv_heads %d (a divisor) head_dim %d (1 to 256)", name, heads,
                     kv_heads, head_dim);
     if (num_pages < 1 || page_size < 1 || max_pages < 1 ||
-        (int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > 0x7fffffff)
+        (int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > kMaxTokens)
         return fail(HEXCUDA_ERR_ARG, "%s: num_pages %d page_size %d max_pages %d", name, num_pages,
                     page_size, max_pages);
     if (!(scale > 0.0f) || isinf(scale))

@@ -516,9 +516,11 @@ int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, con
  * Tables, lengths, offsets, slots and positions are device data: an entry out
  * of range is skipped, never followed, and the next hexcuda_sync returns
  * HEXCUDA_ERR_ARG.  (paged_attn takes keys and values of zeros for a page that
- * is not there: the rows of that sequence are of no use, the others are right.)  Page, token and row counts are below 2^31; element offsets
- * are 64-bit.  Nothing is allocated and nothing is read back, so calls can be
- * captured into CUDA graphs (with hexcuda_set_timing(0)). */
+ * is not there: the rows of that sequence are of no use, the others are right.)
+ * The cache's tokens are below 2^31; a table's (max_pages * page_size), a budget
+ * and total_q are at most 2^31 - 2^16; element offsets are 64-bit.  Nothing is
+ * allocated and nothing is read back, so calls can be captured into CUDA graphs
+ * (with hexcuda_set_timing(0)). */
 #define HEXCUDA_F16 0
 #define HEXCUDA_BF16 1
 /* RMS norm and rotation of new tokens' heads, and their way into the cache.
