@@ -497,6 +497,9 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
         return fail(HEXCUDA_ERR_ARG, "%s: batch %d kv_heads %d", name, batch, kv_heads);
     Dev *d = get_dev(dev);
     if (!d) return HEXCUDA_ERR_NODEV;
+    const int64_t pages16 = (int64_t)num_pages * kv_heads * page_size * head_dim;
+    if (overlap16(k_pages, pages16, v_pages, pages16))
+        return fail(HEXCUDA_ERR_ARG, "%s: k_pages and v_pages overlap", name);
     Evict a{k_pages, v_pages, scores, block_table, dst_table ? dst_table : block_table, kv_lens,
             new_lens, kept, batch, kv_heads, head_dim, num_pages, page_size, max_pages, width,
             budget, sink, recent, -1, d->err_word};

@@ -86,6 +86,12 @@ int check_paged(const char *name, int dtype, const void *table, const void *kv_l
                 const void *q_offs, int batch, int total_q, int max_q, int heads, int kv_heads,
                 int head_dim, int num_pages, int page_size, int max_pages, float scale);
 
+// Whether two arrays of 16-bit values share memory (none when either is null).
+inline bool overlap16(const void *a, int64_t an, const void *b, int64_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && an > 0 && bn > 0 && x < y + 2 * (uint64_t)bn && y < x + 2 * (uint64_t)an;
+}
+
 // Watchdog budget for device-side bounded waits, in nanoseconds of
 // %globaltimer.  A wait that exceeds it sets the device error word.
 constexpr unsigned long long kWaitBudgetNs = 4000000000ull;

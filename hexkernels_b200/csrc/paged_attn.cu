@@ -314,7 +314,11 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
     if (!d) return HEXCUDA_ERR_NODEV;
     size_t need = 0;
     if (int rc = hexcuda_paged_attn_workspace(dev, &need)) return rc;
-    if (out == q) return fail(HEXCUDA_ERR_ARG, "paged_attn: out is q");
+    const int64_t rows16 = (int64_t)total_q * heads * head_dim;
+    const int64_t pages16 = (int64_t)num_pages * kv_heads * page_size * head_dim;
+    if (overlap16(out, rows16, q, rows16) || overlap16(out, rows16, k_pages, pages16) ||
+        overlap16(out, rows16, v_pages, pages16))
+        return fail(HEXCUDA_ERR_ARG, "paged_attn: out is q or overlaps an input");
     if (workspace_bytes < need || ((uintptr_t)workspace & 15u))
         return fail(HEXCUDA_ERR_ARG,
                     "paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned",

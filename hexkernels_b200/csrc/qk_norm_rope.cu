@@ -392,6 +392,15 @@ HX_EXPORT int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_
         return fail(HEXCUDA_ERR_ARG, "%s: heads %d kv_heads %d", name, heads, kv_heads);
     Dev *d = get_dev(dev);
     if (!d) return HEXCUDA_ERR_NODEV;
+    const int64_t row = (int64_t)heads * head_dim, kv_row = (int64_t)kv_heads * head_dim;
+    const int64_t last = tokens - 1;
+    if ((overlap16(q_out, tokens * row, q, last * q_stride + row) &&
+         !(q_out == q && (tokens == 1 || q_stride == row))) ||
+        (kv_row > 0 && (overlap16(q_out, tokens * row, k, last * k_stride + kv_row) ||
+                        overlap16(q_out, tokens * row, v, last * v_stride + kv_row))))
+        return fail(HEXCUDA_ERR_ARG, "%s: q_out overlaps an input and is not q in its layout", name);
+    if (overlap16(k_pages, num_pages * kv_row * page_size, v_pages, num_pages * kv_row * page_size))
+        return fail(HEXCUDA_ERR_ARG, "%s: k_pages and v_pages overlap", name);
     NormRope a;
     a.q = q;
     a.k = k;

@@ -531,7 +531,7 @@ int hexcuda_rope_pair_f16(int dev, const uint16_t *x, const uint16_t *cos_t, con
  * [table_len][rot_dim / 2] fp32 at row positions[t]: columns (i, i + rot_dim /
  * 2) when halves != 0, (2 i, 2 i + 1) otherwise; fp32 throughout, one rounding.
  * Queries go to q_out [tokens][heads][head_dim] (may be q itself when q_stride
- * is heads * head_dim), keys and values (unchanged) to slot slots[t] = page *
+ * is heads * head_dim, and overlaps no input otherwise), keys and values (unchanged) to slot slots[t] = page *
  * page_size + offset, and scores [num_pages][kv_heads][page_size] (may be
  * null) is set to 0 there.  A negative slot marks padding: nothing of that
  * token is read or written.  Slots of one call are distinct.  kv_heads 0: only
@@ -548,7 +548,7 @@ int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_stride, co
 /* Attention of new tokens over the cache: out [total_q][heads][head_dim] =
  * softmax(scale * q K^T) V over the tokens a row sees, lse [total_q][heads]
  * (fp32, may be null) = log sum exp of its scaled scores.  A row that sees
- * nothing gets zeros and minus infinity.  out is not q.  scale > 0.  max_q: the largest
+ * nothing gets zeros and minus infinity.  out overlaps no input.  scale > 0.  max_q: the largest
  * number of new tokens of a sequence as far as known (it chooses between
  * kernels; a wrong one costs time only).  workspace: device memory of
  * hexcuda_paged_attn_workspace bytes, 16-byte aligned, its contents free;
@@ -580,7 +580,7 @@ int hexcuda_cache_scores(int dev, int dtype, const void *q, const float *lse, co
  * same pages in the same places: in place.  Otherwise its pages must not be
  * among those that block_table names for cached tokens, nor one page be named
  * for two sequences; in place, sequences share no pages.  K and V elements are
- * 16-bit, of either type.  sink + recent <= budget. */
+ * 16-bit, of either type, and do not overlap.  sink + recent <= budget. */
 int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *scores,
                         const int32_t *block_table, const int32_t *dst_table,
                         const int32_t *kv_lens, int32_t *new_lens, int32_t *kept, int batch,

@@ -35,6 +35,15 @@ cudaError_t cudaFuncGetAttributes(cudaFuncAttributes *a, const void *) {
     a->numRegs = 168;
     return cudaSuccess;
 }
+cudaError_t cudaOccupancyMaxActiveBlocksPerMultiprocessorWithFlags(int *n, const void *, int, size_t,
+                                                                   unsigned) {
+    *n = 8;
+    return cudaSuccess;
+}
+cudaError_t cudaOccupancyMaxActiveBlocksPerMultiprocessor(int *n, const void *, int, size_t) {
+    *n = 8;
+    return cudaSuccess;
+}
 cudaError_t cudaGetDriverEntryPoint(const char *, void **p, unsigned long long,
                                     cudaDriverEntryPointQueryResult *r) {
     *p = reinterpret_cast<void *>(encode);
