@@ -327,9 +327,10 @@ __device__ __forceinline__ void settle_row(uint8_t *tile, int key, int from, int
     // neighbours start at eight different chunks: no bank conflicts.)
     uint32_t bits = 0;
 #pragma unroll 1
-    for (int i = 0; i < 8 * SUBS; i += 8)
+    for (int i = 0; i < 8 * SUBS; i += 4)
 #pragma unroll
-        for (int u = 0; u < 8; u++) bits |= odd_bits<T>(row[(i >> 3) * kStep + ((u ^ key) & 7)]);
+        for (int u = 0; u < 4; u++)
+            bits |= odd_bits<T>(row[(i >> 3) * kStep + (((i + u) ^ key) & 7)]);
     if (bits == 0) return;
     *odd = 1;
 #pragma unroll 1
