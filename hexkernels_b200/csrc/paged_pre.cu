@@ -417,12 +417,17 @@ __global__ void __launch_bounds__(384, 1)
             float m_ref = -INFINITY, l = 0.0f;
             bool ok = true;
             for (; left > 0; left--, n++, rest -= step_keys, rest0 -= step_keys, first = false) {
+                ok = tc::mbar_wait(&s_full[x], n & 1, abort_flag, err_word, kErrWaitAccum);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc::tc_fence_after();
                 if (rest0 < kKeys) {
                     // values that no weight of zero may meet, by each side before it
                     // hands its P over (all four warps have then).  The rows that b
                     // would settle a has settled, if it takes the tile, before its own
                     // P V and then b's read it: b writes the same zeros once more, or
-                    // nothing.
+                    // nothing.  (Behind the scores: they were begun after the P V of the
+                    // tile that had the value stage before, so that the stage's barrier
+                    // is at most one phase behind and its parity is this tile's.)
                     const Span s = span_of(a, *wp, x);
                     const int j = s.start + (s.count() - left) * s.step, gk = g0 + (j - wp->j0);
                     const int valid = wp->kv_len - j * kKeys;
@@ -435,9 +440,6 @@ __global__ void __launch_bounds__(384, 1)
                         tc::fence_proxy_async_smem();
                     }
                 }
-                ok = tc::mbar_wait(&s_full[x], n & 1, abort_flag, err_word, kErrWaitAccum);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                tc::tc_fence_after();
                 // the whole score row into registers: four loads, one wait
                 uint32_t sr[4][32];
 #pragma unroll

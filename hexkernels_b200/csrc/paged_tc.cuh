@@ -284,7 +284,6 @@ __device__ __forceinline__ void load_frags(const PagedTc &a, uint8_t *dst, const
 // no weight changes.  That is the work of an item's own tokens, whatever the cache
 // holds.  Measured with a channel of infinities over the whole cache, 16 heads of 128
 // on 4: 600 new tokens of 6000 128 us (finite values 69), 7 of 12000 41 (38).
-// The tile is settled before its scores are waited for: behind them chunks took up to 5 % more.
 
 // Whether a chunk of eight values holds one that is not finite, as bits that are not
 // all zero: a product with zero keeps infinities and not-a-numbers apart from the rest.

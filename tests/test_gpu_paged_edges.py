@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import CODE, OnDevice, dev, down, near, norm_rope, up  # noqa: F401
+from test_gpu_paged import CODE, OnDevice, check_attn, dev, down, near, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F32 = np.zeros(0, np.float32)
@@ -263,6 +263,34 @@ def test_a_workspace_of_the_least_alignment(dev):
         near(out, want, b_out)
         near(lse, z, b_lse)
         assert (whole[:16] == 0xA5).all() and (whole[16 + need:] == 0xA5).all()
+
+
+AGAIN = [   # kv, q, heads, kv_heads, dim, page: items of one query tile, many of them to a CTA, and pairs
+    ([5107, 2554], [43, 22], 32, 16, 128, 32), ([130, 250, 70] * 40, [40, 33, 60] * 40, 8, 4, 128, 16), ([100] * 300, [40] * 300, 4, 4, 128, 32),
+    ([390] * 60, [50] * 60, 8, 4, 64, 16), ([1000, 600] * 8, [300, 100] * 8, 8, 2, 128, 16), ([3000, 200] * 8, [5, 3] * 8, 16, 4, 128, 16),
+    ([700] * 20, [129, 64] * 10, 4, 4, 128, 16), ([900, 129] * 12, [7, 2] * 12, 16, 4, 64, 16),
+]
+
+
+@pytest.mark.parametrize("n", range(len(AGAIN)), ids=lambda n: "-".join(map(str, AGAIN[n][2:])) + f"x{len(AGAIN[n][0])}")
+def test_calls_behind_one_another_repeat_bit_for_bit(dev, n):
+    """Calls on two batches in turn, none waited for: the same bits each time,
+    and the right ones."""
+    cs = [ref.Cache(np.random.default_rng(590 + n + i), *AGAIN[n], "f16", fill=np.nan) for i in range(2)]
+    os = [OnDevice(dev, c) for c in cs]
+    os[1].space = os[0].space
+    os[0].attn()
+    dev.sync(0)
+    check_attn(os[0], True, "first")
+    first = [t.clone() for t in (os[0].out, os[0].lse)]
+    for _ in range(40):
+        os[0].out.fill_(0)
+        for o in (os[0], os[1], os[0], os[0], os[1]):
+            o.attn()
+        for t, f in zip((os[0].out, os[0].lse), first):
+            assert bool((t == f).all())
+    dev.sync(0)
+    check_attn(os[1], True, "second")
 
 
 # ----------------------------------------------------------------- errors
