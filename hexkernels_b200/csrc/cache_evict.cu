@@ -7,10 +7,14 @@
 // Two launches: the choice (a radix select on the scores' bits, then the places
 // in index order, so ties go to the lowest index), then the move of K, V and
 // score rows.  Both are bound by what they read and write once, and for few
-// sequences by latency.  Measured, 8 key heads of 128 to a quarter of their length:
-// 1 x 4099: 20 us (choice 15, move 9, overlapping); 32 x 8192: 105 us (25 and 78,
-// the move at 5.6 TB/s); 8 heads of 64, 1 x 131072 to 8192: 41 us (31 and 13; the
-// choice is three passes, each with barriers over the cluster).
+// sequences by latency.  Measured among other calls, to other pages, 8 key heads of 128
+// to a quarter of their length: 1 x 4099: 20 us (choice 15, move 9, overlapping); 32 x
+// 8192: 105 us (25 and 78, the move at 5.6 TB/s); 8 heads of 64, 1 x 131072 to 8192: 41
+// us (30 and 12; the choice is three passes, each with barriers over the cluster).
+// In place the move of few sequences takes longer, since a slice's chunks follow one
+// another (128-wide heads, L2 flushed: 1 x 131072 97 us for 50, 32 x 8192 130 for 122).
+// The choice's CTAs and shared memory go by the table's width: what it could name,
+// not the lengths, which the host cannot see.
 #include <math.h>
 
 #include <algorithm>
@@ -508,11 +512,11 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
     launch_begin(d);
     const int bh = batch * kv_heads;
     // CTAs a sequence and key head: as many as keep the device busy, while each has
-    // some thousands of places left (8 key heads, the whole call: 1 x 32768 with
-    // several 33 us, with one 51; 1 x 131072 49 and 59 with what shared memory needs;
-    // 1 x 4099 with two 24.5, with one 22.5).  More of them than SMs: of 512 threads, so
-    // that two are resident (64 x 4096: 129 us, with 1024 threads 145; fewer CTAs
-    // want the 1024: 1 x 131072 49 us, with 512 59).
+    // some thousands of places left (8 key heads of 128, the whole call, L2 flushed:
+    // 1 x 32768 with several 34 us, with one 52, and with twice as many 36; 1 x 131072 50
+    // and 60 with what shared memory needs; 1 x 4099 with one or two 24).  More of them
+    // than SMs: of 512 threads, so that two are resident (64 x 4096: 130 us, with 1024
+    // threads 147; fewer CTAs want the 1024: 1 x 131072 50 us, with 512 60).
     const int64_t longest = (int64_t)max_pages * page_size;
     int ranks = 1;
     while (ranks < kMaxCluster && (bh * 2 * ranks <= d->sms || longest > (int64_t)ranks * kSmemKeys) &&
@@ -529,7 +533,7 @@ HX_EXPORT int hexcuda_cache_evict(int dev, void *k_pages, void *v_pages, float *
     if (rc) return rc;
     const bool vec = head_dim % 8 == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15u) == 0;
     // column slices of 64 bytes, as far as CTAs are missing (in place, 1 x 131072 to
-    // 8192: 96 us, unsliced 160; 32 x 8192 unsliced 127, always sliced 139)
+    // 8192: 97 us, unsliced 161; 64 x 4096 to 1024: unsliced 130, always sliced 149)
     int slices = 1;
     while (vec && head_dim % (64 * slices) == 0 && bh * 2 * slices < 2 * d->sms && slices < 4) slices *= 2;
     // to other pages: a chunk of tokens a CTA

@@ -328,10 +328,10 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
     const int group = heads / kv_heads;
     // Up to 32 query rows share a key head: the decoding kernel, of 16 or 32 rows.
     // More: 128-row tiles.  Measured with tiles of 16 / 32 / 128 rows (dim 128, 8 key
-    // heads): 4 sequences of 1000, 8 rows: 18.4 / 22.5 / 22.5 us, 32 rows: 24.6 /
-    // 22.5 / 22.5, 40 rows: 24.6 / 24.6 / 24.6, 128 rows: 36.9 / 28.6 / 26.6; 32 of
-    // 8192, 16 rows: 192 / 192 / 192, 32 rows: 350 / 197 / 195, 40 rows: 504 / 352 /
-    // 197.  (Two tiles of rows read the keys twice.)
+    // heads, L2 flushed): 4 sequences of 1000, 8 rows: 21.5 / 21.5 / 25.6 us, 32 rows:
+    // 25.6 / 23.6 / 27.6, 40 rows: 25.6 / 25.6 / 27.7, 128 rows: 37.9 / 29.7 / 29.7; 32
+    // of 8192, 16 rows: 198 / 198 / 200, 32 rows: 364 / 202 / 202, 40 rows: 517 / 360 /
+    // 202.  (Two tiles of rows read the keys twice.)
     const int64_t rows = (int64_t)(max_q < 1 ? 1 : max_q) * group;
     if (paged_tc_fits(q, k_pages, v_pages, out, heads, kv_heads, head_dim, num_pages, page_size)) {
         const bool few = rows <= 32;
@@ -345,7 +345,7 @@ HX_EXPORT int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *
         const int low = page_size & -page_size;
         a.frag = low < kKeys ? low : kKeys;
         a.map_rows = num_pages * kv_heads * page_size;
-        a.min_units = 2;        // (4: one sequence of 777 in 20.5 us for 18.4, longer ones the same)
+        a.min_units = 2;        // (4: one sequence of 777 in 16.8 us for 14.5, longer ones the same)
         a.scale_log2 = scale * 1.4426950408889634f;
         a.q = q;
         a.k = k_pages;

@@ -27,9 +27,9 @@
 // Bound by the chain scores -> maximum -> exponentials -> P V of a key tile, which
 // the other tile's overlaps but does not hide: 128 x 128 exponentials take 1024
 // cycles of the MUFU, the two products 1024 (dim 128) of the tensor pipe.  Measured
-// with the join: 4096 new tokens of 16384, 32 heads of 128 over 8 key heads: 1.04 ms,
-// 930 TFLOP/s, tensor pipe 51 % busy; 11 sequences of up to 301 new tokens of up to
-// 4099, 16 heads of 64: 75 us, a key tile of two query tiles taking 3650 cycles.
+// with the join: 4096 new tokens of 16384, 32 heads of 128 over 8 key heads: 1.00 ms,
+// 960 TFLOP/s, tensor pipe 53 % busy; 11 sequences of up to 301 new tokens of up to
+// 4099, 16 heads of 64: 74 us, a key tile of two query tiles taking some 3600 cycles.
 //
 // Every wait is bounded; see mbar_wait.
 #include <math.h>

@@ -10,8 +10,8 @@
 //
 // Everything between the load and the one rounding at the store is fp32.
 // HBM-bound: each row is read once and written once, 4 bytes a value.  Measured
-// with 32 + 2 x 8 heads of 128: 16384 tokens 80 us for 411 MB, 5.2 TB/s (a copy 6.5);
-// one token 4.5 us on the device.
+// with 32 + 2 x 8 heads of 128: 16384 tokens 78 to 83 us from box to box for 411 MB, 5.0
+// to 5.3 TB/s (a copy 6.5); one token 5 us on the device.
 #include "ew_launch.cuh"
 #include "paged.cuh"
 
@@ -325,8 +325,8 @@ void launch_wide(Dev *d, const NormRope &a) {
     constexpr int kRows = kWideThreads / LPR;
     const int all = (rows + kRows - 1) / kRows;
     // few tokens: a block per pass, so that a token's rows go out at once (16 and 64
-    // tokens 6.1 us, with U passes a block 8.2; 4096 tokens 32.7 and 26.6, from 253
-    // to 1200 the same)
+    // tokens 8.2 us, with U passes a block 10.2; 4096 tokens 34.9 and 28.7, from 253
+    // to 1200 the same; L2 flushed)
     const int passes = a.tokens < 4 * d->sms ? 1 : all < U ? all : U;
     const dim3 grid((unsigned)a.tokens, (unsigned)((all + passes - 1) / passes));
     norm_rope_kernel<T, LPR, HALVES><<<grid, kWideThreads, 0, d->stream>>>(a, passes);

@@ -20,11 +20,13 @@
 // tiles in tensor memory.  256 keys to a query tile, because the query tiles
 // come from L2 again and again: with 128 keys they asked for more than L2
 // gives.  With few rows the kernel is bound by HBM (each key once): 64 sequences of
-// 8192, one new token, 32 heads of 128 over 8 key heads: 101 us for 563 MB, 5.6
-// TB/s.  With many it is bound by the exponentials, one per score: 3 x 1000 new tokens
-// of 6000: 129 us, a unit of 256 keys x 128 rows taking 3000 cycles, 2048 of them
-// the MUFU's.  Items are not cut (a key's sum would need a second pass or lose its
-// fixed order): there the busiest CTA has 64 units for 54 on average.
+// up to 8192 (half that on average), one new token, 32 heads of 128 over 8 key heads:
+// 101 to 107 us from box to box for 563 MB, 5.2 to 5.6 TB/s.  With many it is bound by
+// the exponentials, one per score: 3 sequences of up to 1000 new tokens of 6000: 130
+// us, a unit of 256 keys x 128 rows taking 3000 cycles, 2048 of them the MUFU's.  Items
+// are not cut (a key's sum then needs a second pass in a fixed order): there the
+// busiest CTA has 71 units for 56 on average, and 4 CTAs do all of 1000 new tokens of
+// 1000 with one key head.
 //
 // Every wait is bounded; see mbar_wait.
 #include <math.h>
@@ -594,8 +596,8 @@ int launch_scores_tc(Dev *d, const PagedSeqs &s, int dtype, const void *q, const
     a.group = heads / kv_heads;
     const int64_t need = (int64_t)(max_q < 1 ? 1 : max_q) * a.group;
     // Query tiles of 16, 32 or 128 rows.  Measured (us, dim 128, 8 key heads): 64
-    // sequences of 8192, 4 rows to a key head: 195 / 201 / 393; 16 of 4096, 32 rows: 47
-    // / 39 / 59, 64 rows: 74 / 49 / 61, 80 rows: 86 / 64 / 61, 128 rows: 119 / 74 / 57.
+    // sequences of 8192, 4 rows to a key head: 197 / 201 / 430; 16 of 4096, 32 rows: 48
+    // / 42 / 62, 64 rows: 73 / 50 / 63, 80 rows: 85 / 64 / 63, 128 rows: 122 / 76 / 57.
     // A tile holds a token's heads.
     const int rows = need <= 16 ? 16 : need <= 64 && a.group <= 32 ? 32 : 128;
     a.tok = rows / a.group;
