@@ -75,7 +75,8 @@ def test_neighbours_are_not(lib, fine):
     assert attn(lib, 3, 64, **fine) == 0 and lib.launches() == 2
 
 
-LAST = 4 * 1536 * 2       # bytes from the first token to the fifth
+ROW = 2 * (8 + 2 + 2) * 128      # bytes of a token
+LAST = 4 * ROW                  # from the first to the fifth
 
 
 @pytest.mark.parametrize("bad", [
@@ -89,7 +90,7 @@ def test_queries_over_what_is_still_read(lib, bad):
 
 
 @pytest.mark.parametrize("fine", [
-    dict(), dict(tokens=1, out=Q), dict(q_stride=1024, k=K + (1 << 30), v=V + (1 << 30), out=Q), dict(out=Q + LAST + 3072),
+    dict(), dict(tokens=1, out=Q), dict(q_stride=1024, k=K + (1 << 30), v=V + (1 << 30), out=Q), dict(out=Q + LAST + ROW),
     dict(out=Q - 5 * 2048)], ids=str)
 def test_queries_in_place_or_beside(lib, fine):
     lib.refuse(0)
