@@ -31,9 +31,9 @@ int check_paged(const char *name, int dtype, const void *table, const void *kv_l
         (int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > kMaxTokens)
         return fail(HEXCUDA_ERR_ARG, "%s: num_pages %d page_size %d max_pages %d", name, num_pages,
                     page_size, max_pages);
-    if (!(scale > 0.0f) || isinf(scale))
-        return fail(HEXCUDA_ERR_ARG, "%s: scale %g is not positive and finite", name,
-                    (double)scale);
+    if (!(scale > 0.0f) || isinf(scale * 1.4426950408889634f))
+        return fail(HEXCUDA_ERR_ARG, "%s: scale %g is not positive and finite (log2(e) times it)",
+                    name, (double)scale);
     if (batch > 0 && total_q > 0 && (!table || !kv_lens || !q_offs))
         return fail(HEXCUDA_ERR_ARG, "%s: null pointer", name);
     return HEXCUDA_OK;

@@ -548,7 +548,7 @@ int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_stride, co
 /* Attention of new tokens over the cache: out [total_q][heads][head_dim] =
  * softmax(scale * q K^T) V over the tokens a row sees, lse [total_q][heads]
  * (fp32, may be null) = log sum exp of its scaled scores.  A row that sees
- * nothing gets zeros and minus infinity.  out overlaps no input.  scale > 0.  max_q: the largest
+ * nothing gets zeros and minus infinity.  out overlaps no input.  scale > 0, finite times log2(e).  max_q: the largest
  * number of new tokens of a sequence as far as known (it chooses between
  * kernels; a wrong one costs time only).  workspace: device memory of
  * hexcuda_paged_attn_workspace bytes, 16-byte aligned, its contents free;

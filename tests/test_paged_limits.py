@@ -22,3 +22,11 @@ def test_a_budget_beyond_the_kernels_steps(lib, over):  # noqa: F811
     assert evict(lib, **({} if "dst_wide" in over else {"dst": None}) | over) == 1
     assert b"cache_evict" in lib.hexcuda_last_error_string()
     assert evict(lib, dst=None, budget=MOST) != 1
+
+
+@pytest.mark.parametrize("call", [attn, scores])
+def test_a_scale_whose_product_with_log2_e_is_infinite(lib, call):  # noqa: F811
+    """2^(scale log2(e) x) of a zero score would be not-a-number."""
+    assert call(lib, scale=3e38) == 1
+    assert b"scale" in lib.hexcuda_last_error_string()
+    assert call(lib, scale=2e38) != 1
