@@ -293,6 +293,61 @@ def test_calls_behind_one_another_repeat_bit_for_bit(dev, n):
     check_attn(os[1], True, "second")
 
 
+def test_captured_calls_take_what_is_there_when_they_are_replayed(dev):
+    """A captured step, replayed with values that are not finite, with a page
+    that is not there, and again with good ones."""
+    import torch
+    from hexkernels_b200 import HexcudaError
+    c = ref.Cache(np.random.default_rng(601), [700, 90, 300], [40, 3, 70], 8, 2, 128, 16, "bf16", fill=np.nan)
+    o = OnDevice(dev, c)
+    s = up(np.zeros(c.k.shape[:3], np.float32))
+    side = torch.cuda.Stream()
+    good_v, good_table = o.v.clone(), o.table.clone()
+    g = None
+    try:
+        dev.bind_stream(0, side)
+        with torch.cuda.stream(side):
+            o.attn()
+            o.scores(s)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            o.attn()
+            o.scores(s)
+
+        def replay():
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                g.replay()
+            torch.cuda.synchronize()
+
+        for _ in range(2):
+            v = ref.to64(c.v)
+            keep = c.v
+            v[..., 3] = np.inf
+            v[c.table[0, 42], :, 5, 9] = np.nan      # token 677 of 700: among the new ones
+            c.v = ref.to16(v, "bf16")
+            o.v.copy_(up(c.v))
+            replay()
+            out, lse = o.results()
+            want, z, b_out, b_lse = attn_odd(c, True)
+            near(out, want, b_out, "not finite")
+            near(lse, z, b_lse)
+            c.v = keep
+            o.v.copy_(good_v)
+            o.table[1, 2] = -1
+            replay()
+            with pytest.raises(HexcudaError, match="out of range"):
+                dev.sync(0)
+            o.table.copy_(good_table)
+            replay()
+            dev.sync(0)
+            check_attn(o, True, "good again")
+    finally:
+        del g
+        dev.bind_stream(0)
+
+
 # ----------------------------------------------------------------- errors
 
 def test_a_call_after_one_that_ran_out_of_memory(hx):
