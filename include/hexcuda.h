@@ -548,11 +548,12 @@ int hexcuda_qk_norm_rope(int dev, int dtype, const void *q, int64_t q_stride, co
 /* Attention of new tokens over the cache: out [total_q][heads][head_dim] =
  * softmax(scale * q K^T) V over the tokens a row sees, lse [total_q][heads]
  * (fp32, may be null) = log sum exp of its scaled scores.  A row that sees
- * nothing gets zeros and minus infinity.  out overlaps no input.  scale > 0, finite times log2(e).  max_q: the largest
- * number of new tokens of a sequence as far as known (it chooses between
- * kernels; a wrong one costs time only).  workspace: device memory of
- * hexcuda_paged_attn_workspace bytes, 16-byte aligned, its contents free;
- * calls that may run at the same time (two streams, two graphs) need one each. */
+ * nothing gets zeros and minus infinity.  out overlaps no input.  scale > 0, and
+ * finite times log2(e).  max_q: the largest number of new tokens of a sequence as
+ * far as known (it chooses between kernels; a wrong one costs time only).
+ * workspace: device memory of hexcuda_paged_attn_workspace bytes, 16-byte
+ * aligned, its contents free; calls that may run at the same time (two streams,
+ * two graphs) need one each. */
 int hexcuda_paged_attn(int dev, int dtype, const void *q, const void *k_pages, const void *v_pages,
                        const int32_t *block_table, const int32_t *kv_lens, const int32_t *q_offs,
                        void *out, float *lse, void *workspace, size_t workspace_bytes, int batch,
