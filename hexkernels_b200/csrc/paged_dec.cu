@@ -28,7 +28,7 @@
 //
 // Measured with the join: 96 sequences of up to 16384 tokens, 32 heads of 128 over
 // 8 key heads: 493 to 504 us from box to box for 3.26 GB, 6.5 to 6.6 TB/s, what a copy
-// reaches; one sequence of 777: 14.5 us, the latency of a plan (4500 cycles), one chain
+// reaches; one sequence of 777: 14.5 to 16, the latency of a plan (4500 cycles), one chain
 // of loads and MMAs, and the join.
 //
 // Every wait is bounded; see mbar_wait.
